@@ -193,6 +193,55 @@ NVA_API int nva_paged_decode_noalloc(const void* q, int64_t q_row_stride, const 
                                      float softmax_scale, void* out, int64_t out_row_stride, void* stream);
 
 /*
+ * 8-bit KV cache.  k_cache / v_cache hold e4m3 values [NB, BS, KVH, D]; k_scale / v_scale float32
+ * [NB, KVH, BS / scale_block], one scale for each block of scale_block consecutive slots and kv head, all contiguous:
+ * the value held in slot s of block b is cache[b, s, h, :] * scale[b, h, s / scale_block].  scale_block is a power of
+ * two from NVA_MIN_SCALE_BLOCK to NVA_MAX_SCALE_BLOCK that divides BS; NB * BS < 2^31.  head_dim 128.
+ *
+ * nva_store_kvcache_fp8: nva_store_kvcache's scatter of bf16 rows (8-byte aligned, row strides multiples of 4), rounded
+ * on the way.  With amax the largest finite magnitude that the call writes to a scale block (per head, k and v apart)
+ * and e the least whole number with amax <= 448 * 2^e, kept in [-40, 40]:
+ *     scale' = 2^e when the call writes the block's first slot (the block starts afresh), else max(scale, 2^e)
+ *     values the block held: rounded to e4m3 again as c * scale / scale' when the scale grew (not when it starts afresh)
+ *     values written:        x / scale' rounded to e4m3 (nearest even), clamped to 448; NaN and infinities become NaN
+ * Magnitudes above 448 * 2^40 are clamped.  A slot named more than once takes the last of its tokens.  Slot -1 is
+ * skipped; other slots outside the cache are skipped and set bit 1 of the error word.
+ *
+ * nva_paged_decode_fp8, nva_varlen_attention_fp8: nva_paged_decode and the paged nva_varlen_attention over such a cache
+ * (bf16 q and out).  Scales outside [2^-40, 2^40] are taken as those bounds for v.  bt_width is the number of entries
+ * in a row of block_tables: a sequence that needs more, or names a block outside the cache, sets bit 4 of the error
+ * word and reads zeros there.  The number of sequences is not bounded; in the varlen call num_heads / num_kv_heads <= 48
+ * and query runs may have any length.  Workspace: the same zero-filled-once contract, and the same one may serve all
+ * attention calls.
+ */
+#define NVA_MIN_SCALE_BLOCK 8
+#define NVA_MAX_SCALE_BLOCK 256
+NVA_API int nva_store_kvcache_fp8(const void* key, int64_t key_row_stride, const void* value, int64_t value_row_stride,
+                                  void* k_cache, void* v_cache, float* k_scale, float* v_scale, int32_t num_blocks,
+                                  int32_t block_size, int32_t scale_block, const int32_t* slot_mapping,
+                                  int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim, void* stream);
+
+NVA_API int nva_paged_decode_fp8(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                 const float* k_scale, const float* v_scale, int32_t num_blocks, int32_t block_size,
+                                 int32_t scale_block, const int32_t* context_lens, const int32_t* block_tables,
+                                 int32_t bt_row_stride, int32_t bt_width, int32_t num_seqs, int32_t q_per_seq,
+                                 int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float softmax_scale,
+                                 void* out, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+NVA_API size_t nva_paged_decode_fp8_workspace_bytes(int32_t q_per_seq, int32_t num_heads, int32_t num_kv_heads,
+                                                    int32_t head_dim);
+
+NVA_API int nva_varlen_attention_fp8(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                     const float* k_scale, const float* v_scale, int32_t num_blocks,
+                                     int32_t block_size, int32_t scale_block, const int32_t* cu_seqlens_q,
+                                     const int32_t* cu_seqlens_k, int32_t num_seqs, int32_t total_q,
+                                     const int32_t* block_tables, int32_t bt_row_stride, int32_t bt_width,
+                                     int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float softmax_scale,
+                                     void* out, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+NVA_API size_t nva_varlen_fp8_workspace_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim);
+
+/*
  * Device error word.  Kernels never trap: a slot or block id out of range, or a pipeline wait that ran past its
  * time limit, sets a bit here and the kernel skips the access or returns.  Reading it synchronises the device.
  * Bits: 1 = scatter slot out of range, 2 = pipeline wait timed out, 4 = block id out of range.

@@ -37,15 +37,13 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// Rank-3 bf16 view {128 dims, heads, rows} with the given row stride (bytes), 64 x 1 x 128 boxes, 128B swizzle.
-int encode_rows(CUtensorMap* tm, const void* base, int64_t heads, int64_t rows, int64_t row_stride_bytes) {
+// A tensor map of the given type with 128-byte swizzle and unit element strides.
+int encode_tiled(CUtensorMap* tm, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+                 const cuuint64_t* strides, const cuuint32_t* box) {
   auto fn = encode_fn();
   if (fn == nullptr) return NVA_ERR_CUDA;
-  cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
-  cuuint64_t strides[2] = {128 * 2, static_cast<cuuint64_t>(row_stride_bytes)};
-  cuuint32_t box[3] = {64, 1, 128};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(tm, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
@@ -55,13 +53,13 @@ int encode_rows(CUtensorMap* tm, const void* base, int64_t heads, int64_t rows, 
   return NVA_OK;
 }
 
-}  // namespace nva
-
-namespace {
-
-using nva::cuda_fail;
-using nva::encode_rows;
-using nva::g_last_cuda_error;
+// Rank-3 bf16 view {128 dims, heads, rows} with the given row stride (bytes), 64 x 1 x 128 boxes, 128B swizzle.
+int encode_rows(CUtensorMap* tm, const void* base, int64_t heads, int64_t rows, int64_t row_stride_bytes) {
+  const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[2] = {128 * 2, static_cast<cuuint64_t>(row_stride_bytes)};
+  const cuuint32_t box[3] = {64, 1, 128};
+  return encode_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box);
+}
 
 int sm_count() {
   int dev = 0;
@@ -73,6 +71,15 @@ int sm_count() {
   if (dev < 64) cached[dev] = n;
   return n;
 }
+
+}  // namespace nva
+
+namespace {
+
+using nva::cuda_fail;
+using nva::encode_rows;
+using nva::g_last_cuda_error;
+using nva::sm_count;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 // The attention kernels take row maxima of unscaled scores and scale them afterwards: the scale must be positive

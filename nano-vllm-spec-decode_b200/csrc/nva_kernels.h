@@ -43,6 +43,8 @@ struct DecodeParams {
   int32_t pdl;       // 1: launched with a programmatic dependency on the preceding kernel (launch_paged_decode sets it)
 };
 
+// Merge tickets at the start of every attention workspace: room for two CTAs on each of `sms` SMs.
+size_t decode_ticket_bytes(int sms);
 size_t decode_workspace_bytes(int grid, int np);
 // Carve the workspace (decode_workspace_bytes(grid, np) bytes) into the partials and the merge counters.
 void decode_workspace_layout(void* ws, int grid, int np, DecodeParams* p);
@@ -69,6 +71,37 @@ cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
   cfg.numAttrs = pdl ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
+
+// One attention step over a paged 8-bit cache (paged_decode_fp8.cu).  Modes as in DecodeParams; in varlen mode every
+// sequence is handled here, runs of more than max_n queries piece by piece.
+struct Fp8DecodeParams {
+  const __nv_bfloat16* q;
+  int64_t q_row_stride;
+  __nv_bfloat16* out;
+  int64_t out_row_stride;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  const int32_t* ctx_lens;
+  const int32_t* block_tables;
+  int32_t bt_stride;
+  int32_t bt_width;     // blocks a row of block_tables names
+  int32_t num_seqs;
+  int32_t n_fixed;
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t group;
+  int32_t max_n;        // queries per piece: tile rows / group
+  int32_t block_size;
+  int32_t num_blocks;
+  const float* k_scale; // [num_blocks, num_kv_heads, page_blocks]
+  const float* v_scale;
+  int32_t page_blocks;  // scale blocks per cache block
+  int32_t lg_block;     // log2 of the tokens per scale block
+  float scale_log2;
+  float* part_o;        // [2 * grid, NP, 128], [2 * grid, NP]: as in DecodeParams
+  float* part_lse;
+  int32_t* counters;    // [grid][4] merge tickets: zero on entry and on exit
+};
 
 // Varlen prefill kernel (long query runs) — q rows tiled by 128 per (sequence, q head).
 struct PrefillParams {
@@ -131,7 +164,11 @@ cudaError_t launch_greedy_accept(const void* target, int64_t target_row_stride, 
 // Host helpers of the C ABI (capi.cu): record a CUDA error's text for nva_last_cuda_error() and return NVA_ERR_CUDA;
 // encode a rank-3 bf16 tensor map {128 dims, heads, rows} (row stride in bytes) with 64 x 1 x 128 boxes and 128-byte
 // swizzle, the layout every TMA load of the kernels uses (an encoder failure is recorded the same way).
+// encode_tiled is the general form (128-byte swizzle, unit element strides).  sm_count: the current device's, 0 on error.
 int cuda_fail(cudaError_t e);
+int sm_count();
+int encode_tiled(CUtensorMap* tm, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+                 const cuuint64_t* strides, const cuuint32_t* box);
 int encode_rows(CUtensorMap* tm, const void* base, int64_t heads, int64_t rows, int64_t row_stride_bytes);
 
 // Qwen3's attention prologue in one pass (q/k RMSNorm, rotary, KV scatter); see qk_prologue.cu.

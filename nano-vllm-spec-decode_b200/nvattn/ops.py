@@ -7,10 +7,15 @@
                          causal=True, block_table=)                 flash-attn call at attention.py:67-70
   greedy_accept(target_ids, draft_ids, num_drafts)                  greedy core of verify_drafts, sampler.py:66-82
 
+The first three also take an 8-bit cache: float8_e4m3fn k_cache / v_cache with k_scale= / v_scale= (float32
+[NB, KVH, BS / G], a power of two for each block of G consecutive slots and kv head; kvcache_scales() makes them).
+
 Every op runs on the caller's current CUDA stream, allocates only its output and never syncs.  The attention ops
 share one workspace per device (split-KV partials and the merge tickets, see _workspace); there is no CPU path:
 non-CUDA tensors raise.
 """
+import contextlib
+
 import torch
 
 from . import _lib
@@ -18,6 +23,13 @@ from . import _lib
 
 def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+def _on(device: torch.device):
+    """The context in which `device` is the current one (nothing to do when it already is)."""
+    if device.type != "cuda" or device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def _need_cuda(*ts):
@@ -54,16 +66,19 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
 
 
 def reserve_workspace(max_num_seqs: int, max_num_tokens: int, num_heads: int, num_kv_heads: int,
-                      head_dim: int = 128, device: torch.device | None = None) -> int:
+                      head_dim: int = 128, device: torch.device | None = None, fp8_cache: bool = False) -> int:
     """Allocate (zero-filled) the workspace every later decode / verify / varlen call of up to max_num_seqs
-    sequences and max_num_tokens query rows needs on `device`, so that no call, captured or not, allocates.
-    Returns its size in bytes.  nano-vllm: max_num_seqs and max_num_batched_tokens of its Config."""
+    sequences and max_num_tokens query rows needs on `device`, so that no call, captured or not, allocates; with
+    fp8_cache, also for calls over an 8-bit cache.  Returns its size in bytes.  nano-vllm: max_num_seqs and
+    max_num_batched_tokens of its Config."""
     device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     lib = _lib.load()
     with torch.cuda.device(device):
         need = max(lib.nva_varlen_workspace_bytes(max_num_seqs, max_num_tokens, num_heads, num_kv_heads, head_dim),
                    max(lib.nva_paged_decode_workspace_bytes(max_num_seqs, n, num_heads, num_kv_heads, head_dim)
                        for n in range(1, 49)))
+        if fp8_cache:
+            need = max(need, lib.nva_varlen_fp8_workspace_bytes(num_heads, num_kv_heads, head_dim))
     return _workspace(need, device).numel()
 
 
@@ -75,12 +90,52 @@ def reset_workspaces() -> None:
         ws.zero_()
 
 
+SCALE_BLOCKS = (8, 16, 32, 64, 128, 256)   # tokens per scale of an 8-bit cache (include/nvattn.h)
+
+
+def kvcache_scales(k_cache: torch.Tensor, scale_block: int = 16):
+    """Zero-filled (k_scale, v_scale) for an 8-bit cache [NB, BS, KVH, 128]: one scale for each block of scale_block
+    consecutive slots and kv head, set by store_kvcache.  16 costs 0.2% of the cache's bytes; a larger block has less
+    to read and rounds again more rows when a louder token joins it."""
+    NB, BS, KVH, _ = k_cache.shape
+    assert scale_block in SCALE_BLOCKS and BS % scale_block == 0
+    return tuple(torch.zeros(NB, KVH, BS // scale_block, dtype=torch.float32, device=k_cache.device) for _ in range(2))
+
+
+def _scale_block(k_cache, v_cache, k_scale, v_scale) -> int:
+    """Checks an 8-bit cache against its scales; returns the tokens per scale."""
+    assert k_cache.dtype == v_cache.dtype == torch.float8_e4m3fn, "k_scale / v_scale go with a float8_e4m3fn cache"
+    assert k_scale is not None and v_scale is not None, "an 8-bit cache needs both k_scale and v_scale"
+    assert k_cache.dim() == 4 and v_cache.shape == k_cache.shape
+    NB, BS, KVH, _ = k_cache.shape
+    assert k_scale.dtype == v_scale.dtype == torch.float32
+    assert k_scale.is_contiguous() and v_scale.is_contiguous() and k_scale.shape == v_scale.shape
+    blocks = k_scale.shape[-1]
+    assert k_scale.shape == (NB, KVH, blocks) and blocks > 0 and BS % blocks == 0, "scales are [NB, KVH, BS / G]"
+    assert BS // blocks in SCALE_BLOCKS
+    assert k_cache.is_contiguous() and v_cache.is_contiguous()
+    assert k_cache.device == v_cache.device == k_scale.device == v_scale.device
+    return BS // blocks
+
+
+def _is_fp8(k_cache, k_scale, v_scale) -> bool:
+    return k_scale is not None or v_scale is not None or k_cache.dtype == torch.float8_e4m3fn
+
+
 def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
-                  slot_mapping: torch.Tensor) -> None:
-    """Scatter this step's K/V rows into the paged cache (attention.py:33-40; same asserts)."""
+                  slot_mapping: torch.Tensor, k_scale: torch.Tensor | None = None,
+                  v_scale: torch.Tensor | None = None) -> None:
+    """Scatter this step's K/V rows into the paged cache (attention.py:33-40; same asserts).
+
+    With a float8_e4m3fn cache and its scales the bf16 rows are rounded on the way: a scale block takes the scale of
+    its largest value (a power of two, at least 2^-40 and at most 2^40); when a louder token joins it the scale grows
+    and what it held is rounded again; a token in its first slot starts it afresh.  See include/nvattn.h."""
     N, num_heads, head_dim = key.shape
     D = num_heads * head_dim
     assert key.stride(-1) == 1 and value.stride(-1) == 1
+    if _is_fp8(k_cache, k_scale, v_scale):
+        _store_kvcache_fp8(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+        return
     assert key.stride(1) == head_dim and value.stride(1) == head_dim
     assert k_cache.stride(1) == D and v_cache.stride(1) == D
     assert slot_mapping.numel() == N
@@ -95,12 +150,34 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
         "store_kvcache")
 
 
+def _store_kvcache_fp8(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale) -> None:
+    N, num_heads, head_dim = key.shape
+    G = _scale_block(k_cache, v_cache, k_scale, v_scale)
+    NB, BS, KVH, D = k_cache.shape
+    assert value.shape == key.shape and (KVH, D) == (num_heads, head_dim)
+    assert key.dtype == value.dtype == torch.bfloat16
+    if N > 0:
+        assert key.stride(1) == head_dim and value.stride(1) == head_dim
+    assert slot_mapping.numel() == N and slot_mapping.dtype == torch.int32 and slot_mapping.is_contiguous()
+    _need_cuda(key, value, k_cache, v_cache, slot_mapping)
+    assert key.device == value.device == slot_mapping.device == k_cache.device
+    with _on(key.device):
+        _lib.check(_lib.load().nva_store_kvcache_fp8(
+            key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), NB, BS, G, slot_mapping.data_ptr(), N, num_heads, head_dim,
+            _stream()), "store_kvcache (8-bit cache)")
+
+
 def flash_attn_with_kvcache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cache_seqlens: torch.Tensor,
                             block_table: torch.Tensor, softmax_scale: float, causal: bool = True,
-                            out: torch.Tensor | None = None) -> torch.Tensor:
+                            out: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
+                            v_scale: torch.Tensor | None = None) -> torch.Tensor:
     """Paged decode / verify attention.  q [B, n, H, D] bf16; k_cache/v_cache [NB, BS, KVH, D]; cache_seqlens
-    [B] int32 (including the n new tokens); block_table [B, W] int32.  Causal, bottom-right aligned."""
+    [B] int32 (including the n new tokens); block_table [B, W] int32.  Causal, bottom-right aligned.  With k_scale /
+    v_scale the cache is float8_e4m3fn (q and the output stay bf16)."""
     assert causal, "nano-vllm always calls with causal=True"
+    if _is_fp8(k_cache, k_scale, v_scale):
+        return _decode_fp8(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, softmax_scale, out)
     B, n, H, D = q.shape
     NB, BS, KVH, _ = k_cache.shape
     _need_cuda(q, k_cache, v_cache, cache_seqlens, block_table)
@@ -127,13 +204,84 @@ def flash_attn_with_kvcache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     return out
 
 
+def _decode_fp8(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, softmax_scale, out):
+    B, n, H, D = q.shape
+    G = _scale_block(k_cache, v_cache, k_scale, v_scale)
+    NB, BS, KVH, Dc = k_cache.shape
+    _need_cuda(q, k_cache, v_cache, cache_seqlens, block_table)
+    assert q.dtype == torch.bfloat16 and Dc == D and H % KVH == 0
+    assert q.stride(-1) == 1 and q.stride(2) == D and q.stride(0) == n * q.stride(1)
+    assert cache_seqlens.dtype == torch.int32 and cache_seqlens.is_contiguous() and cache_seqlens.numel() == B
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == B
+    assert block_table.stride(-1) == 1 or block_table.shape[1] == 1
+    assert q.device == k_cache.device == cache_seqlens.device == block_table.device
+    if out is None:
+        out = torch.empty(B, n, H, D, dtype=q.dtype, device=q.device)
+    else:   # rows are addressed as (b * n + i) * out.stride(1): the same layout rules as q
+        _need_cuda(out)
+        assert out.dtype == q.dtype and out.shape == q.shape and out.device == q.device
+        assert out.stride(-1) == 1 and out.stride(2) == D and out.stride(0) == n * out.stride(1)
+    lib = _lib.load()
+    with _on(q.device):
+        ws_bytes = lib.nva_paged_decode_fp8_workspace_bytes(n, H, KVH, D)
+        if ws_bytes == 0:
+            raise _lib.NvattnError(f"paged decode over an 8-bit cache does not support q_per_seq={n} with {H // KVH} "
+                                   f"q heads per kv head and head_dim {D}")
+        ws = _workspace(ws_bytes, q.device)
+        _lib.check(lib.nva_paged_decode_fp8(
+            q.data_ptr(), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            NB, BS, G, cache_seqlens.data_ptr(), block_table.data_ptr(), max(block_table.stride(0), block_table.shape[1]),
+            block_table.shape[1], B, n, H, KVH, D, float(softmax_scale), out.data_ptr(), out.stride(1), ws.data_ptr(),
+            ws_bytes, _stream()), "paged decode (8-bit cache)")
+    return out
+
+
+def _varlen_fp8(q, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, cu_seqlens_k, block_table, softmax_scale, out):
+    Tq, H, D = q.shape
+    G = _scale_block(k_cache, v_cache, k_scale, v_scale)
+    NB, BS, KVH, Dc = k_cache.shape
+    _need_cuda(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_table)
+    B = cu_seqlens_q.numel() - 1
+    assert q.dtype == torch.bfloat16 and Dc == D and H % KVH == 0
+    assert q.stride(-1) == 1 and q.stride(1) == D
+    assert cu_seqlens_q.dtype == cu_seqlens_k.dtype == torch.int32 and cu_seqlens_k.numel() == B + 1
+    assert cu_seqlens_q.is_contiguous() and cu_seqlens_k.is_contiguous()
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] >= B
+    assert block_table.stride(-1) == 1 or block_table.shape[1] == 1
+    assert q.device == k_cache.device == cu_seqlens_q.device == cu_seqlens_k.device == block_table.device
+    if out is None:
+        out = torch.empty(Tq, H, D, dtype=q.dtype, device=q.device)
+    else:
+        _need_cuda(out)
+        assert out.dtype == q.dtype and out.shape == q.shape and out.device == q.device
+        assert out.stride(-1) == 1 and out.stride(1) == D
+    lib = _lib.load()
+    with _on(q.device):
+        ws_bytes = lib.nva_varlen_fp8_workspace_bytes(H, KVH, D)
+        if ws_bytes == 0:
+            raise _lib.NvattnError(f"varlen attention over an 8-bit cache does not support {H // KVH} q heads per kv "
+                                   f"head with head_dim {D}")
+        ws = _workspace(ws_bytes, q.device)
+        _lib.check(lib.nva_varlen_attention_fp8(
+            q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            NB, BS, G, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), B, Tq, block_table.data_ptr(),
+            max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], H, KVH, D, float(softmax_scale),
+            out.data_ptr(), out.stride(0), ws.data_ptr(), ws_bytes, _stream()), "varlen attention (8-bit cache)")
+    return out
+
+
 def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, max_seqlen_q: int,
                            cu_seqlens_q: torch.Tensor, max_seqlen_k: int, cu_seqlens_k: torch.Tensor,
                            softmax_scale: float, causal: bool = True, block_table: torch.Tensor | None = None,
-                           out: torch.Tensor | None = None) -> torch.Tensor:
+                           out: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
+                           v_scale: torch.Tensor | None = None) -> torch.Tensor:
     """Varlen causal attention.  q [Tq, H, D]; with block_table, k/v are the paged caches [NB, BS, KVH, D],
-    else contiguous [Tk, KVH, D] rows (any row stride).  max_seqlen_* are upper bounds only."""
+    else contiguous [Tk, KVH, D] rows (any row stride).  max_seqlen_* are upper bounds only.  With k_scale / v_scale
+    (and a block_table) the cache is float8_e4m3fn (q and the output stay bf16)."""
     assert causal, "nano-vllm always calls with causal=True"
+    if _is_fp8(k, k_scale, v_scale):
+        assert block_table is not None, "an 8-bit cache is read through a block_table"
+        return _varlen_fp8(q, k, v, k_scale, v_scale, cu_seqlens_q, cu_seqlens_k, block_table, softmax_scale, out)
     Tq, H, D = q.shape
     _need_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, block_table)
     assert q.dtype == k.dtype == v.dtype == torch.bfloat16
