@@ -210,8 +210,8 @@ NVA_API int nva_paged_decode_noalloc(const void* q, int64_t q_row_stride, const 
  * nva_paged_decode_fp8, nva_varlen_attention_fp8: nva_paged_decode and the paged nva_varlen_attention over such a cache
  * (bf16 q and out).  Scales outside [2^-40, 2^40] are taken as those bounds for v.  bt_width is the number of entries
  * in a row of block_tables: a sequence that needs more, or names a block outside the cache, sets bit 4 of the error
- * word and reads zeros there.  The number of sequences is not bounded; in the varlen call num_heads / num_kv_heads <= 48
- * and query runs may have any length.  Workspace: the same zero-filled-once contract, and the same one may serve all
+ * word and reads zeros there.  Neither the number of sequences nor the length of a query run is bounded; max_seqlen_q only picks the
+ * row width of the kernel.  num_heads / num_kv_heads <= 40.  Workspace: the same zero-filled-once contract, and the same one may serve all
  * attention calls.
  */
 #define NVA_MIN_SCALE_BLOCK 8
@@ -228,18 +228,19 @@ NVA_API int nva_paged_decode_fp8(const void* q, int64_t q_row_stride, const void
                                  int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float softmax_scale,
                                  void* out, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
                                  void* stream);
-NVA_API size_t nva_paged_decode_fp8_workspace_bytes(int32_t q_per_seq, int32_t num_heads, int32_t num_kv_heads,
-                                                    int32_t head_dim);
-
 NVA_API int nva_varlen_attention_fp8(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
                                      const float* k_scale, const float* v_scale, int32_t num_blocks,
                                      int32_t block_size, int32_t scale_block, const int32_t* cu_seqlens_q,
                                      const int32_t* cu_seqlens_k, int32_t num_seqs, int32_t total_q,
-                                     const int32_t* block_tables, int32_t bt_row_stride, int32_t bt_width,
+                                     int32_t max_seqlen_q, const int32_t* block_tables, int32_t bt_row_stride,
+                                     int32_t bt_width,
                                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float softmax_scale,
                                      void* out, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
                                      void* stream);
-NVA_API size_t nva_varlen_fp8_workspace_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim);
+
+/* Workspace of both calls; max_q: q_per_seq, or the varlen call's max_seqlen_q. */
+NVA_API size_t nva_paged_attention_fp8_workspace_bytes(int32_t max_q, int32_t num_heads, int32_t num_kv_heads,
+                                                       int32_t head_dim);
 
 /*
  * Device error word.  Kernels never trap: a slot or block id out of range, or a pipeline wait that ran past its

@@ -91,6 +91,7 @@ struct Fp8DecodeParams {
   int32_t num_kv_heads;
   int32_t group;
   int32_t max_n;        // queries per piece: tile rows / group
+  int32_t head_set;     // kv heads that as many CTAs walk side by side (divides num_kv_heads and the grid)
   int32_t block_size;
   int32_t num_blocks;
   const float* k_scale; // [num_blocks, num_kv_heads, page_blocks]

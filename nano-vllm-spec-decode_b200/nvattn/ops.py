@@ -78,7 +78,8 @@ def reserve_workspace(max_num_seqs: int, max_num_tokens: int, num_heads: int, nu
                    max(lib.nva_paged_decode_workspace_bytes(max_num_seqs, n, num_heads, num_kv_heads, head_dim)
                        for n in range(1, 49)))
         if fp8_cache:
-            need = max(need, lib.nva_varlen_fp8_workspace_bytes(num_heads, num_kv_heads, head_dim))
+            need = max(need, lib.nva_paged_attention_fp8_workspace_bytes(max_num_tokens, num_heads, num_kv_heads,
+                                                                         head_dim))
     return _workspace(need, device).numel()
 
 
@@ -223,10 +224,10 @@ def _decode_fp8(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_tabl
         assert out.stride(-1) == 1 and out.stride(2) == D and out.stride(0) == n * out.stride(1)
     lib = _lib.load()
     with _on(q.device):
-        ws_bytes = lib.nva_paged_decode_fp8_workspace_bytes(n, H, KVH, D)
+        ws_bytes = lib.nva_paged_attention_fp8_workspace_bytes(n, H, KVH, D)
         if ws_bytes == 0:
-            raise _lib.NvattnError(f"paged decode over an 8-bit cache does not support q_per_seq={n} with {H // KVH} "
-                                   f"q heads per kv head and head_dim {D}")
+            raise _lib.NvattnError(f"paged decode over an 8-bit cache does not support {H // KVH} q heads per kv head "
+                                   f"with head_dim {D}")
         ws = _workspace(ws_bytes, q.device)
         _lib.check(lib.nva_paged_decode_fp8(
             q.data_ptr(), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
@@ -236,7 +237,8 @@ def _decode_fp8(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_tabl
     return out
 
 
-def _varlen_fp8(q, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, cu_seqlens_k, block_table, softmax_scale, out):
+def _varlen_fp8(q, k_cache, v_cache, k_scale, v_scale, max_seqlen_q, cu_seqlens_q, cu_seqlens_k, block_table,
+                softmax_scale, out):
     Tq, H, D = q.shape
     G = _scale_block(k_cache, v_cache, k_scale, v_scale)
     NB, BS, KVH, Dc = k_cache.shape
@@ -257,16 +259,16 @@ def _varlen_fp8(q, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, cu_seqlens_
         assert out.stride(-1) == 1 and out.stride(1) == D
     lib = _lib.load()
     with _on(q.device):
-        ws_bytes = lib.nva_varlen_fp8_workspace_bytes(H, KVH, D)
+        ws_bytes = lib.nva_paged_attention_fp8_workspace_bytes(int(max_seqlen_q), H, KVH, D)
         if ws_bytes == 0:
             raise _lib.NvattnError(f"varlen attention over an 8-bit cache does not support {H // KVH} q heads per kv "
                                    f"head with head_dim {D}")
         ws = _workspace(ws_bytes, q.device)
         _lib.check(lib.nva_varlen_attention_fp8(
             q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            NB, BS, G, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), B, Tq, block_table.data_ptr(),
-            max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], H, KVH, D, float(softmax_scale),
-            out.data_ptr(), out.stride(0), ws.data_ptr(), ws_bytes, _stream()), "varlen attention (8-bit cache)")
+            NB, BS, G, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), B, Tq, int(max_seqlen_q),
+            block_table.data_ptr(), max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], H, KVH, D,
+            float(softmax_scale), out.data_ptr(), out.stride(0), ws.data_ptr(), ws_bytes, _stream()), "varlen attention (8-bit cache)")
     return out
 
 
@@ -281,7 +283,8 @@ def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ma
     assert causal, "nano-vllm always calls with causal=True"
     if _is_fp8(k, k_scale, v_scale):
         assert block_table is not None, "an 8-bit cache is read through a block_table"
-        return _varlen_fp8(q, k, v, k_scale, v_scale, cu_seqlens_q, cu_seqlens_k, block_table, softmax_scale, out)
+        return _varlen_fp8(q, k, v, k_scale, v_scale, max_seqlen_q, cu_seqlens_q, cu_seqlens_k, block_table,
+                           softmax_scale, out)
     Tq, H, D = q.shape
     _need_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, block_table)
     assert q.dtype == k.dtype == v.dtype == torch.bfloat16
