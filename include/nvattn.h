@@ -243,6 +243,41 @@ NVA_API size_t nva_paged_attention_fp8_workspace_bytes(int32_t max_q, int32_t nu
                                                        int32_t head_dim);
 
 /*
+ * Sampling from given uniform numbers.  Replaces the random branches of Sampler.forward (nanovllm/layers/sampler.py:7-16)
+ * and verify_drafts (:68-78, 83-102).  logits [rows, vocab] (bf16 when elem_bytes == 2, float when 4, row stride in
+ * elements, any alignment).  Per row, temperature T > 0, optional top_k (<= 0 or >= vocab: off), top_p (>= 1: off),
+ * min_p (<= 0: off), each an array or NULL, and a uniform number u in [0, 1) (float when uniform_bytes == 4, double
+ * when 8; others are brought into the range):
+ *     w_i = exp((l_i - max l) / T), 1 where l_i equals the maximum (also for an infinite one); NaN counts as -inf
+ *     tokens with w_i < min_p go; of the others the top_k largest stay (equals: lowest index first); of those, in
+ *     falling order, a token stays while the weight before it is less than top_p times their sum
+ *     ids = first index at which the running sum of the kept weights passes u times their sum
+ * T <= 0: the argmax (torch's rule: lowest index, NaN above everything).  Sums are exact integer sums of weights rounded
+ * to 2^-44, so a result depends on nothing but the arguments.
+ *
+ * nva_verify_sampled: rows of logits [num_seqs * (k + 1), vocab], settings and u per sequence, drafts [num_seqs, k],
+ * num_drafts [num_seqs], accept_uniform [num_seqs, k].  Draft j of a sequence (j < num_drafts) is accepted when
+ * accept_uniform * (sum of row j's kept weights) < the draft's kept weight (T <= 0: when it is the argmax);
+ * num_accepted = unbroken run of accepts; next_token = the draw from row num_accepted without the draft that was turned
+ * down there, or, behind the last draft, the plain draw.  Drafts outside the vocabulary are never accepted.  This is
+ * speculative sampling for proposals that are fixed tokens (n-gram matches, a greedy draft model): the tokens are
+ * distributed as if drawn one by one.  Ids int32 (id_bytes 4) or int64 (8).  workspace needs no initial value.
+ */
+#define NVA_MAX_SAMPLE_VOCAB 393216
+#define NVA_MAX_SAMPLE_ROWS (1 << 20)
+NVA_API int nva_sample_tokens(const void* logits, int64_t row_stride, int32_t rows, int32_t vocab, int32_t elem_bytes,
+                              const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                              const void* uniform, int32_t uniform_bytes, int64_t* ids, void* stream);
+NVA_API int nva_verify_sampled(const void* logits, int64_t row_stride, int32_t num_seqs, int32_t k, int32_t vocab,
+                               int32_t elem_bytes, const void* draft_ids, int64_t draft_row_stride,
+                               const void* num_drafts, int32_t id_bytes, const float* temperature,
+                               const int32_t* top_k, const float* top_p, const float* min_p,
+                               const void* accept_uniform, int64_t accept_row_stride, const void* uniform,
+                               int32_t uniform_bytes, void* num_accepted, void* next_tokens, void* workspace,
+                               size_t workspace_bytes, void* stream);
+NVA_API size_t nva_verify_sampled_workspace_bytes(int32_t num_seqs, int32_t k);
+
+/*
  * Device error word.  Kernels never trap: a slot or block id out of range, or a pipeline wait that ran past its
  * time limit, sets a bit here and the kernel skips the access or returns.  Reading it synchronises the device.
  * Bits: 1 = scatter slot out of range, 2 = pipeline wait timed out, 4 = block id out of range.

@@ -374,6 +374,74 @@ def shard_accept(keys: torch.Tensor, draft_ids: torch.Tensor, num_drafts: torch.
     return acc, nxt
 
 
+def _settings(rows: int, device, temperatures, top_k, top_p, min_p):
+    """Checks the per-row sampling settings; returns their pointers (0: off)."""
+    out = []
+    for x, dt in ((temperatures, torch.float32), (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32)):
+        if x is None:
+            out.append(0)
+            continue
+        assert x.dtype == dt and x.shape == (rows,) and x.is_contiguous() and x.device == device
+        out.append(x.data_ptr())
+    return out
+
+
+def sample_tokens(logits: torch.Tensor, temperatures: torch.Tensor, uniforms: torch.Tensor,
+                  top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
+                  min_p: torch.Tensor | None = None) -> torch.Tensor:
+    """One token per row of logits [R, V] (bf16 or float32, unit column stride), int64 [R], from the uniform numbers
+    uniforms [R] in [0, 1) (float32 or float64).  temperatures [R] float32 (<= 0: argmax), top_k [R] int32 (<= 0: off),
+    top_p [R] float32 (>= 1: off), min_p [R] float32 (<= 0: off).  The rules are in include/nvattn.h."""
+    _need_cuda(logits, temperatures, uniforms, top_k, top_p, min_p)
+    assert logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32)
+    R, V = logits.shape
+    assert logits.stride(1) == 1 or V == 1
+    assert uniforms.dtype in (torch.float32, torch.float64) and uniforms.shape == (R,) and uniforms.is_contiguous()
+    assert temperatures is not None and uniforms.device == logits.device
+    t, k, p, m = _settings(R, logits.device, temperatures, top_k, top_p, min_p)
+    ids = torch.empty(R, dtype=torch.int64, device=logits.device)
+    with _on(logits.device):
+        _lib.check(_lib.load().nva_sample_tokens(
+            logits.data_ptr(), logits.stride(0) if R > 1 else max(logits.stride(0), V), R, V, logits.element_size(), t,
+            k, p, m, uniforms.data_ptr(), uniforms.element_size(), ids.data_ptr(), _stream()), "sample tokens")
+    return ids
+
+
+def verify_sampled(logits: torch.Tensor, draft_ids: torch.Tensor, num_drafts: torch.Tensor,
+                   temperatures: torch.Tensor, accept_uniforms: torch.Tensor, uniforms: torch.Tensor,
+                   top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
+                   min_p: torch.Tensor | None = None):
+    """Speculative sampling of fixed drafts: logits [S * (K+1), V], draft_ids [S, K] and num_drafts [S] (both int32 or
+    both int64), settings and uniforms [S] per sequence, accept_uniforms [S, K] (the uniforms' dtype).  Returns
+    (num_accepted [S], next_token [S]) in the ids' dtype.  The rules are in include/nvattn.h."""
+    _need_cuda(logits, draft_ids, num_drafts, temperatures, accept_uniforms, uniforms, top_k, top_p, min_p)
+    S, K = draft_ids.shape
+    dt = draft_ids.dtype
+    assert logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32) and logits.shape[0] == S * (K + 1)
+    V = logits.shape[1]
+    assert logits.stride(1) == 1 or V == 1
+    assert dt in (torch.int32, torch.int64) and num_drafts.dtype == dt
+    assert num_drafts.shape == (S,) and num_drafts.is_contiguous()
+    assert K <= 1 or (draft_ids.stride(1) == 1 and accept_uniforms.stride(1) == 1)
+    assert uniforms.dtype in (torch.float32, torch.float64) and uniforms.shape == (S,) and uniforms.is_contiguous()
+    assert accept_uniforms.dtype == uniforms.dtype and accept_uniforms.shape == (S, K)
+    assert temperatures is not None
+    assert logits.device == draft_ids.device == num_drafts.device == accept_uniforms.device == uniforms.device
+    t, k, p, m = _settings(S, logits.device, temperatures, top_k, top_p, min_p)
+    acc = torch.empty(S, dtype=dt, device=logits.device)
+    nxt = torch.empty(S, dtype=dt, device=logits.device)
+    lib = _lib.load()
+    ws = torch.empty(S * (K + 1), 2, dtype=torch.int32, device=logits.device)
+    with _on(logits.device):
+        _lib.check(lib.nva_verify_sampled(
+            logits.data_ptr(), max(logits.stride(0), V), S, K, V, logits.element_size(),
+            draft_ids.data_ptr() if K else 0, max(draft_ids.stride(0), K) if K else 0, num_drafts.data_ptr(),
+            draft_ids.element_size(), t, k, p, m, accept_uniforms.data_ptr() if K else 0,
+            max(accept_uniforms.stride(0), K) if K else 0, uniforms.data_ptr(), uniforms.element_size(),
+            acc.data_ptr(), nxt.data_ptr(), ws.data_ptr(), ws.numel() * 4, _stream()), "verify sampled")
+    return acc, nxt
+
+
 def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, cos_sin_cache: torch.Tensor,
                        q_norm_weight: torch.Tensor, k_norm_weight: torch.Tensor, eps: float, num_heads: int,
                        num_kv_heads: int, k_cache: torch.Tensor | None = None, v_cache: torch.Tensor | None = None,
