@@ -29,6 +29,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "../../include/nvattn.h"
@@ -45,9 +46,11 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 1024;
 constexpr int kTable = 256;
+constexpr int kList = 1024;            // tokens of a crossing bin kept aside per CTA
 constexpr int kMaxCluster = 8;
 constexpr float kReach = 31.5f;        // exp(-31.5) < 2^-45: weight 0
 constexpr uint32_t kAll = 0xffffffffu;
+constexpr uint32_t kNone = 0xffffffffu;
 using u64 = unsigned long long;
 
 struct SampleParams {
@@ -75,43 +78,57 @@ struct SampleParams {
 
 // What a cluster agrees on; every CTA holds a copy.
 struct Control {
-  u64 before;                          // count or weight above the current key range
-  uint32_t lo, hi;                     // its keys
-  uint32_t bin;
+  u64 before;                          // count or weight above the crossing bin
+  double target;                       // where the running count or weight has to get
+  uint32_t bin;                        // the crossing bin (kNone: everything stays)
+  uint32_t last;                       // this CTA's tokens in the last bin
   u64 draft_weight;
-  u64 sum;                             // this CTA's kept weight (equals of the threshold key apart) ...
-  uint32_t ties;                       // ... and number of tokens at that key
-  uint32_t top;                        // its largest key
-  uint32_t first;                      // its first index of the row's largest key
+  u64 sum;                             // this CTA's kept weight (equals of the threshold apart) ...
+  uint32_t ties;                       // ... and number of tokens at the threshold
+  float top;                           // its largest logit
+  uint32_t first;                      // its first index of the row's largest logit
 };
 
+// Rows are held as they come, two bf16 or one float to a word; NaN as -inf (unless greedy), padding as NaN, which fails
+// every comparison.  Keys are whole numbers in the logits' order, -0 equal to +0.
 template <typename T>
-struct KeyOf;
-// Order-preserving keys; 0 is padding.  -0 equals +0.  NaN: above everything when greedy, else -inf.
+struct Row;
 template <>
-struct KeyOf<__nv_bfloat16> {
+struct Row<__nv_bfloat16> {
   static constexpr int kPerWord = 2;
-  static __device__ __forceinline__ uint32_t one(uint32_t b, bool greedy) {
-    if ((b & 0x7FFFu) > 0x7F80u) b = greedy ? 0x7FFFu : 0xFF80u;
-    if (b == 0x8000u) b = 0u;
-    return (b & 0x8000u) ? (~b & 0xFFFFu) : (b | 0x8000u);
+  static constexpr uint32_t kPad = 0xFFFFu;
+  static __device__ __forceinline__ uint32_t numbers(uint32_t w) {   // NaN to -inf
+    const uint32_t low = 0xFF80FF80u;
+    const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&low));
+    return *reinterpret_cast<const uint32_t*>(&v);
   }
-  static __device__ __forceinline__ uint32_t word(uint32_t w, bool greedy) {
-    return one(w & 0xFFFFu, greedy) | (one(w >> 16, greedy) << 16);
+  template <class F>
+  static __device__ __forceinline__ void each(uint32_t w, F&& f) {
+    f(__uint_as_float(w << 16), 0);
+    f(__uint_as_float(w & 0xFFFF0000u), 1);
+  }
+  static __device__ __forceinline__ uint32_t key(float l) {
+    const uint32_t b = __float_as_uint(l + 0.f);
+    return ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) >> 16;
   }
   static __device__ __forceinline__ float value(uint32_t k) {
     return __uint_as_float(((k & 0x8000u) ? (k & 0x7FFFu) : (~k & 0xFFFFu)) << 16);
   }
 };
 template <>
-struct KeyOf<float> {
+struct Row<float> {
   static constexpr int kPerWord = 1;
-  static __device__ __forceinline__ uint32_t one(uint32_t b, bool greedy) {
-    if ((b & 0x7FFFFFFFu) > 0x7F800000u) b = greedy ? 0x7FFFFFFFu : 0xFF800000u;
-    if (b == 0x80000000u) b = 0u;
+  static constexpr uint32_t kPad = 0xFFFFFFFFu;
+  static __device__ __forceinline__ uint32_t numbers(uint32_t w) {
+    return __float_as_uint(fmaxf(__uint_as_float(w), __uint_as_float(0xFF800000u)));
+  }
+  template <class F>
+  static __device__ __forceinline__ void each(uint32_t w, F&& f) { f(__uint_as_float(w), 0); }
+  static __device__ __forceinline__ uint32_t key(float l) {
+    const uint32_t b = __float_as_uint(l + 0.f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
   }
-  static __device__ __forceinline__ uint32_t word(uint32_t w, bool greedy) { return one(w, greedy); }
   static __device__ __forceinline__ float value(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
   }
@@ -125,30 +142,29 @@ __device__ __forceinline__ int64_t read_id(const void* p, int64_t at, int bytes)
   return bytes == 8 ? static_cast<const int64_t*>(p)[at] : static_cast<const int32_t*>(p)[at];
 }
 
-// w * 2^44 of one logit, rounded: 2^(u / 256) with u = 256 log2(e) (l - m) / T = 256 e + j + r, |r| <= 1/2.
+// w * 2^44 of a logit within reach of the maximum, rounded, as the low 52 bits of a double in [2^52, 2^53):
+// 2^(u / 256) with u = 256 log2(e) (l - m) / T = 256 e + j + r, |r| <= 1/2, from a table of 2^(j / 256 + 44), e added to
+// its exponent, and three terms of the exponential series in r ln 2 / 256 (the fourth is below 1.5e-13: a running sum is
+// off by as little, against gaps of 1e-6 between a vocabulary's sums).
 struct Weight {
   double m, c;           // row maximum, 256 log2(e) / T
-  float mf, reach;       // row maximum, kReach * T
-  const double* table;   // 2^(j / 256)
-  __device__ __forceinline__ u64 operator()(float l) const {
-    if (l == mf) return 1ull << 44;
-    if (!(mf - l <= reach)) return 0ull;
-    const double u = (static_cast<double>(l) - m) * c;
-    const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are rint(u)
-    const double n = u + magic;
-    const double r = u - (n - magic);
-    const int k = __double2loint(n);           // >= -256 * 45.5
-    // 2^(r / 256), four terms in a = r ln 2 / 256 (|a| <= 0.00136: the fifth is below 4e-17)
-    const double a = r * 0.0027076061740622863;
-    double s = fma(a, 0.041666666666666664, 0.16666666666666666);
-    s = fma(a, s, 0.5);
-    s = fma(a, s, 1.0);
-    s = fma(a, s, 1.0);
-    // times 2^(j / 256) * 2^(e + 44), rounded to a whole number by adding 2^52
-    const double scale = __hiloint2double(((k >> 8) + 44 + 1023) << 20, 0);
-    const double y = fma(s * table[k & 255], scale, 4503599627370496.0);
-    return __double_as_longlong(y) & 0xFFFFFFFFFFFFFull;
+  float low;             // logits above it have a weight
+  const double* table;
+  __device__ __forceinline__ u64 bits(float l) const {   // (only for l > low)
+    const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the nearest whole number
+    const double d = static_cast<double>(l) - m;
+    const double n = fma(d, c, magic);
+    const double r = fma(d, c, magic - n);
+    const int k = __double2loint(n);
+    double s = fma(r, 3.308302680541371e-09, 3.665565596910106e-06);   // (ln 2 / 256)^3 / 6, (ln 2 / 256)^2 / 2
+    s = fma(s, r, 0.0027076061740622863);                                // ln 2 / 256
+    s = fma(s, r, 1.0);
+    const double t = table[k & 255];
+    const double scaled = __hiloint2double(__double2hiint(t) + ((k >> 8) << 20), __double2loint(t));
+    return __double_as_longlong(fma(s, scaled, 4503599627370496.0));
   }
+  static constexpr u64 kZero = 0x4330000000000000ull;   // the bits of 2^52
+  __device__ __forceinline__ u64 operator()(float l) const { return l > low ? bits(l) - kZero : 0ull; }
 };
 
 // Block-wide exclusive prefix sums of a weight and a count; `tot` receives the block's sums.
@@ -190,9 +206,9 @@ __device__ __forceinline__ void block_scan(u64& mass, uint32_t& count, u64* wm, 
 
 template <typename T, bool kVerify>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
-  using K = KeyOf<T>;
-  constexpr int kPer = K::kPerWord;
-  constexpr uint32_t kKeyMask = kPer == 2 ? 0xFFFFu : 0xFFFFFFFFu;
+  using R = Row<T>;
+  constexpr int kPer = R::kPerWord;
+  const float kInf = __int_as_float(0x7F800000);
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank());
   const int ranks = static_cast<int>(cluster.num_blocks());
@@ -201,9 +217,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
 
   extern __shared__ __align__(16) uint8_t smem[];
   const int words = p.run_words * kThreads;
-  uint32_t* keys = reinterpret_cast<uint32_t*>(smem);
-  __shared__ uint32_t hist[3][kBins];          // counts; weights, low and high words
+  uint32_t* data = reinterpret_cast<uint32_t*>(smem);
+  __shared__ uint32_t hist[2][kBins];          // counts, or weights: low and high words
   __shared__ double table[kTable];
+  __shared__ uint32_t list[kList];
+  __shared__ uint32_t list_count;
   __shared__ u64 scan_m[kWarps];
   __shared__ uint32_t scan_c[kWarps];
   __shared__ Control ctrl;
@@ -215,15 +233,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const float temp = __ldg(p.temperature + set);
   const bool greedy = !(temp > 0.f);
 
-  // ---------------------------------------------------------------- the row, as keys
+  // ---------------------------------------------------------------- the row
   const int e0 = rank * words * kPer;          // first token of this CTA
   const int n = max(0, min(p.vocab - e0, words * kPer));
-  uint32_t top = 0;
+  float top = -kInf;
   {
     const T* src = static_cast<const T*>(p.logits) + row * p.row_stride + e0;
     const uint32_t* src32 = reinterpret_cast<const uint32_t*>(src);
-    auto best = [&](uint32_t w) {
-      top = kPer == 2 ? __vmaxu2(top, w) : max(top, w);
+    bool nan = false;
+    auto keep = [&](uint32_t w) -> uint32_t {
+      if (greedy) {
+        R::each(w, [&](float l, int) { nan |= l != l; });
+      }
+      const uint32_t x = R::numbers(w);
+      R::each(x, [&](float l, int) { top = fmaxf(top, l); });
+      return greedy ? w : x;
     };
     int done = 0;   // words in place
     if ((reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
@@ -236,54 +260,48 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           if (v0 + i * kThreads < nv) raw[i] = __ldg(reinterpret_cast<const uint4*>(src32) + v0 + i * kThreads);
 #pragma unroll
         for (int i = 0; i < kUnroll; ++i)
-          if (v0 + i * kThreads < nv) {
-            uint4 k;
-            k.x = K::word(raw[i].x, greedy);
-            k.y = K::word(raw[i].y, greedy);
-            k.z = K::word(raw[i].z, greedy);
-            k.w = K::word(raw[i].w, greedy);
-            best(k.x);
-            best(k.y);
-            best(k.z);
-            best(k.w);
-            reinterpret_cast<uint4*>(keys)[v0 + i * kThreads] = k;
-          }
+          if (v0 + i * kThreads < nv)
+            reinterpret_cast<uint4*>(data)[v0 + i * kThreads] =
+                make_uint4(keep(raw[i].x), keep(raw[i].y), keep(raw[i].z), keep(raw[i].w));
       }
       done = nv * 4;
     }
     for (int w = done + tid; w < words; w += kThreads) {
-      uint32_t k = 0;
+      // (the row's end) padding takes no part in the maximum
+      uint32_t x = kPer == 2 ? 0xFF80FF80u : 0xFF800000u, pad = 0;
 #pragma unroll
       for (int h = 0; h < kPer; ++h) {
         const int e = w * kPer + h;
+        const uint32_t mask = (kPer == 2 ? 0xFFFFu : 0xFFFFFFFFu) << (16 * h);
         if (e < n) {
-          const uint32_t b = kPer == 2 ? static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(src) + e))
+          const uint32_t v = kPer == 2 ? static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(src) + e))
                                        : __ldg(src32 + e);
-          k |= K::one(b, greedy) << (16 * h);
+          x = (x & ~mask) | (v << (16 * h));
+        } else {
+          pad |= (R::kPad << (16 * h)) & mask;
         }
       }
-      best(k);
-      keys[w] = k;
+      data[w] = keep(x) | pad;   // (-inf's bits are among the padding's NaN's)
     }
-    if (tid < kTable) table[tid] = exp2(static_cast<double>(tid) / kTable);
-    if (kPer == 2) top = max(top & 0xFFFFu, top >> 16);
-    top = __reduce_max_sync(kAll, top);
-    if (lane == 0) scan_c[warp] = top;
+    if (tid < kTable) table[tid] = exp2(static_cast<double>(tid) / kTable + 44.0);
+    if (nan) top = __int_as_float(0x7FFFFFFF);
+    // (as keys: NaN, possible only when greedy, above +inf)
+    uint32_t k = __float_as_uint(top + 0.f);
+    k = (k & 0x80000000u) ? ~k : (k | 0x80000000u);
+    k = __reduce_max_sync(kAll, k);
+    if (lane == 0) scan_c[warp] = k;
     __syncthreads();
     if (tid == 0) {
-      for (int w = 1; w < kWarps; ++w) top = max(top, scan_c[w]);
-      ctrl.top = top;
+      for (int w = 1; w < kWarps; ++w) k = max(k, scan_c[w]);
+      ctrl.first = k;
     }
   }
   cluster.sync();
-  top = 0;
-  for (int r = 0; r < ranks; ++r) top = max(top, cluster.map_shared_rank(&ctrl, r)->top);
-
-  // this CTA's tokens of one word
-  auto each = [&](uint32_t w, auto&& f) {
-    f(w & kKeyMask, 0);
-    if constexpr (kPer == 2) f(w >> 16, 1);
-  };
+  {
+    uint32_t k = 0;
+    for (int r = 0; r < ranks; ++r) k = max(k, cluster.map_shared_rank(&ctrl, r)->first);
+    top = __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+  }
   const int run0 = tid * p.run_words;          // this thread's run of words
 
   int draft = -1;
@@ -296,11 +314,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   }
 
   if (greedy) {
-    // ---------------------------------------------------------------- argmax: the first index of the largest key
-    uint32_t first = 0xFFFFFFFFu;
-    for (int w = run0; w < run0 + p.run_words && first == 0xFFFFFFFFu; ++w)
-      each(keys[w], [&](uint32_t k, int h) {
-        if (k == top && first == 0xFFFFFFFFu) first = static_cast<uint32_t>(e0 + w * kPer + h);
+    // ---------------------------------------------------------------- argmax: the first index of the largest logit
+    cluster.sync();   // (ctrl.first is read; below it is written again)
+    const bool nan = top != top;
+    uint32_t first = kNone;
+    for (int w = run0; w < run0 + p.run_words && first == kNone; ++w)
+      R::each(data[w], [&](float l, int h) {
+        const int e = w * kPer + h;
+        if (first == kNone && e < n && (nan ? l != l : l == top)) first = static_cast<uint32_t>(e0 + e);
       });
     first = __reduce_min_sync(kAll, first);
     if (lane == 0) scan_c[warp] = first;
@@ -322,183 +343,248 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     return;
   }
 
+  if (top - top != 0.f) {
+    // an infinite maximum: its equals weigh 1, all others nothing
+    for (int w = tid; w < words; w += kThreads) {
+      uint32_t x = 0;
+      R::each(data[w], [&](float l, int h) {
+        const uint32_t v = l != l ? R::kPad : l == top ? 0u : (kPer == 2 ? 0xFF80u : 0xFF800000u);
+        x |= v << (16 * h);
+      });
+      data[w] = x;
+    }
+    top = 0.f;
+    __syncthreads();
+  }
+
   // ---------------------------------------------------------------- thresholds
   Weight weight;
-  weight.mf = K::value(top);
-  weight.m = weight.mf;
+  weight.m = top;
   weight.c = 369.3299304675746 / static_cast<double>(temp);   // 256 log2(e)
-  weight.reach = fminf(kReach * temp, 3.0e38f);   // (-inf stays out at an infinite temperature)
+  // (below the maximum however large that is; at an infinite temperature everything but -inf)
+  weight.low = fminf(fmaxf(top - kReach * temp, -FLT_MAX), nextafterf(top, -kInf));
   weight.table = table;
-  // tokens below it are gone (the keys under -inf's are no numbers)
-  const uint32_t least = K::one(kPer == 2 ? 0xFF80u : 0xFF800000u, false);
-  uint32_t floor_key = least;
+  // kept: logits above `cut`, and the first `cut_ties` tokens at it
+  float cut = -kInf;
+  uint32_t cut_ties = 0;
   if (p.min_p != nullptr) {
     const double mp = fmin(static_cast<double>(__ldg(p.min_p + set)), 1.0);
     if (mp > 0.0) {
       const double at = weight.m + static_cast<double>(temp) * log(mp);   // l >= at
       float f = static_cast<float>(at);
-      if (static_cast<double>(f) < at) f = nextafterf(f, __int_as_float(0x7F800000));
-      if (f == f) {
-        if constexpr (kPer == 2) {
-          // the least bf16 at or above f: round its bits up (away from zero when positive, towards it when negative)
-          uint32_t b = __float_as_uint(f);
-          b = (b & 0x80000000u) ? (b >> 16) : ((b + 0xFFFFu) >> 16);
-          floor_key = max(least, K::one(b, false));
-        } else {
-          floor_key = max(least, K::one(__float_as_uint(f), false));
-        }
-      }
+      if (static_cast<double>(f) < at) f = nextafterf(f, kInf);
+      if (f == f) cut = nextafterf(f, -kInf);
     }
   }
-  uint32_t cut = floor_key - 1;                // kept: keys above it, and the first `cut_ties` tokens at it
-  uint32_t cut_ties = 0;
   const float bin_scale = (kBins / 32.0f) / temp;
-  auto linear_bin = [&](uint32_t k) {          // rises as the key falls
-    return min(kBins - 1, __float2int_rz((weight.mf - K::value(k)) * bin_scale));
+  auto linear_bin = [&](float l) {             // rises as the logit falls; bins of T / 32, the last takes the rest
+    return min(kBins - 1, __float2int_rz((top - l) * bin_scale));
   };
-  // The key at which the running count (or weight) from the top reaches `target`, and what lies above it.  Tokens
-  // eligible: keys above `cut`, and `cut_ties` tokens at it.
-  auto select = [&](auto by_weight, double target, u64& before) -> uint32_t {
+  // Sets the threshold to the logit at which the running count from the top reaches `k`, or the running weight `share`
+  // of the whole, with the number of its equals that still belong; leaves it where everything stays.
+  auto select = [&](auto by_weight, uint32_t k, double share) {
     constexpr bool kMass = decltype(by_weight)::value;
-    uint32_t lo = cut_ties > 0 ? cut : cut + 1, hi = top;
-    before = 0;
-    bool linear = true;
-    while (true) {
-      const int shift = linear ? 0 : max(0, 32 - __clz(hi - lo) - 10);
-      for (int i = tid; i < kBins; i += kThreads) {
-        hist[0][i] = 0;
-        if constexpr (kMass) hist[1][i] = hist[2][i] = 0;
-      }
+    const float floor = cut;                   // tokens eligible: above it, and (weights) cut_ties at it
+    const u64 w_floor = kMass && cut_ties > 0 ? cut_ties * weight(floor) : 0ull;
+    auto add_mass = [&](int b, u64 v) {
+      const uint32_t x = static_cast<uint32_t>(v);
+      const uint32_t old = atomicAdd(&hist[0][b], x);
+      const uint32_t up = static_cast<uint32_t>(v >> 32) + (old + x < old ? 1u : 0u);
+      if (up != 0) atomicAdd(&hist[1][b], up);
+    };
+    auto clear = [&]() {
+      for (int i = tid; i < 2 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
+      if (tid == 0) list_count = 0;
       __syncthreads();
-      auto bin_of = [&](uint32_t k) { return linear ? linear_bin(k) : static_cast<int>((hi - k) >> shift); };
-      auto add_mass = [&](int b, u64 v) {
-        const uint32_t x = static_cast<uint32_t>(v);
-        const uint32_t old = atomicAdd(&hist[1][b], x);
-        const uint32_t up = static_cast<uint32_t>(v >> 32) + (old + x < old ? 1u : 0u);
-        if (up != 0) atomicAdd(&hist[2][b], up);
-      };
-      for (int w = tid; w < words; w += kThreads)
-        each(keys[w], [&](uint32_t k, int) {
-          if (k < lo || k > hi || (kMass && k == cut)) return;
-          if constexpr (kMass) {
-            const u64 v = weight(K::value(k));
-            if (v != 0) add_mass(bin_of(k), v);
-          } else {
-            atomicAdd(&hist[0][bin_of(k)], 1u);
-          }
-        });
-      if (kMass && rank == 0 && tid == 0 && cut_ties > 0 && lo <= cut && cut <= hi)
-        add_mass(bin_of(cut), cut_ties * weight(K::value(cut)));
-      cluster.sync();
-      if (rank == 0) {   // merge the CTAs' bins, two per thread, and find the crossing
+    };
+    // (rank 0) the CTAs' bins together, two per thread: the first at which the target is reached, to everyone
+    auto cross = [&](u64 before, bool linear) {
+      if (rank == 0) {
         u64 v[2] = {0, 0};
+        uint32_t last = 0;
         for (int r = 0; r < ranks; ++r) {
           const uint32_t* h = cluster.map_shared_rank(&hist[0][0], r);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int b = 2 * tid + i;
-            v[i] += kMass ? h[kBins + b] + (static_cast<u64>(h[2 * kBins + b]) << 32) : static_cast<u64>(h[b]);
-          }
+          for (int i = 0; i < 2; ++i)
+            v[i] += h[2 * tid + i] + (kMass ? static_cast<u64>(h[kBins + 2 * tid + i]) << 32 : 0ull);
+          if (!kMass && linear) last += cluster.map_shared_rank(&ctrl, r)->last;
         }
         u64 pre = v[0] + v[1], tot;
         uint32_t none = 0, none_t;
         block_scan(pre, none, scan_m, scan_c, &tot, &none_t, lane, warp);
+        // (the first token always stays: a target of 0 would find no crossing)
+        const double target = !linear ? ctrl.target : kMass ? fmax(share * static_cast<double>(tot), 1.0) : k;
+        auto tell = [&](uint32_t bin, u64 above) {
+          for (int r = 0; r < ranks; ++r) {
+            Control* c = cluster.map_shared_rank(&ctrl, r);
+            c->bin = bin;
+            c->before = above;
+            c->target = target;
+          }
+        };
         pre += before;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (v[i] != 0 && static_cast<double>(pre) < target && static_cast<double>(pre + v[i]) >= target)
-            for (int r = 0; r < ranks; ++r) {
-              Control* c = cluster.map_shared_rank(&ctrl, r);
-              c->bin = static_cast<uint32_t>(2 * tid + i);
-              c->before = pre;
-            }
+            tell(static_cast<uint32_t>(2 * tid + i), pre);
           pre += v[i];
         }
+        if (!kMass && linear && tid == 0 && tot < k)   // not within the bins counted
+          tell(tot + last > k ? static_cast<uint32_t>(kBins - 1) : kNone, tot);
       }
       cluster.sync();
+    };
+    clear();
+    uint32_t last = 0;
+    for (int w = tid; w < words; w += kThreads)
+      R::each(data[w], [&](float l, int) {
+        if (!(l > (kMass ? fmaxf(floor, weight.low) : floor))) return;
+        const int b = linear_bin(l);
+        if constexpr (kMass) {
+          add_mass(b, weight.bits(l) - Weight::kZero);
+        } else if (b < kBins - 1) {
+          atomicAdd(&hist[0][b], 1u);
+        } else {
+          ++last;   // (most of a vocabulary at a low temperature: not through one counter)
+        }
+      });
+    if constexpr (kMass) {
+      if (rank == 0 && tid == 0 && w_floor != 0) add_mass(linear_bin(floor), w_floor);
+    } else {
+      last = __reduce_add_sync(kAll, last);
+      if (lane == 0) scan_c[warp] = last;
+      __syncthreads();
+      if (tid == 0) {
+        for (int w = 1; w < kWarps; ++w) last += scan_c[w];
+        ctrl.last = last;
+      }
+    }
+    cluster.sync();
+    cross(0, true);
+    if (ctrl.bin == kNone) return;
+    // the crossing bin's keys: from the least with linear_bin <= bin to the last before linear_bin < bin, by 32-way
+    // searches
+    uint32_t lo = R::key(floor), hi = R::key(top);   // (the threshold itself may be no bf16 number: a bound)
+    {
+      auto search = [&](auto pred, uint32_t a, uint32_t b) {   // least key in [a, b] with pred, which holds at b
+        while (a < b) {
+          const uint32_t step = (b - a) / 32 + 1;
+          const u64 far = a + static_cast<u64>(step) * lane;
+          const uint32_t x = far < b ? static_cast<uint32_t>(far) : b;
+          const uint32_t yes = __ballot_sync(kAll, x == b || pred(R::value(x)));
+          const int f = yes != 0 ? __ffs(yes) - 1 : 32;   // points below f: no, point f: yes
+          const uint32_t below = __shfl_sync(kAll, x, f > 0 ? f - 1 : 0);
+          const uint32_t at = __shfl_sync(kAll, x, f < 32 ? f : 0);
+          if (f > 0) a = below + 1;
+          b = f == 0 ? a : f < 32 ? at : b;
+        }
+        return b;
+      };
+      const int ib = static_cast<int>(ctrl.bin);
+      lo = search([&](float l) { return linear_bin(l) <= ib; }, lo, hi);
+      if (ib > 0) hi = max(lo, search([&](float l) { return linear_bin(l) < ib; }, lo, hi) - 1);
+    }
+    u64 before = ctrl.before;
+    if (lo < hi) {
+      // its tokens, kept aside when they are few: the levels below read those instead of the row
+      const float flo = R::value(lo), fhi = R::value(hi);
+      for (int w = tid; w < words; w += kThreads)
+        R::each(data[w], [&](float l, int) {
+          if (l > floor && l >= flo && l <= fhi) {
+            const uint32_t at = atomicAdd(&list_count, 1u);
+            if (at < kList) list[at] = R::key(l);
+          }
+        });
+    }
+    while (lo < hi) {
+      __syncthreads();
+      const uint32_t listed = list_count;
+      for (int i = tid; i < 2 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
+      __syncthreads();
+      const int shift = max(0, 32 - __clz(hi - lo) - 10);
+      auto add = [&](uint32_t key) {
+        if (key < lo || key > hi) return;
+        const int b = static_cast<int>((hi - key) >> shift);
+        if constexpr (kMass) {
+          const u64 v = weight(R::value(key));
+          if (v != 0) add_mass(b, v);
+        } else {
+          atomicAdd(&hist[0][b], 1u);
+        }
+      };
+      if (listed <= kList) {
+        for (uint32_t i = tid; i < listed; i += kThreads) add(list[i]);
+      } else {
+        for (int w = tid; w < words; w += kThreads)
+          R::each(data[w], [&](float l, int) {
+            if (l > floor) add(R::key(l));
+          });
+      }
+      if (kMass && rank == 0 && tid == 0 && w_floor != 0 && R::key(floor) >= lo && R::key(floor) <= hi)
+        add_mass(static_cast<int>((hi - R::key(floor)) >> shift), w_floor);
+      cluster.sync();
+      cross(before, false);
       const uint32_t bin = ctrl.bin;
       before = ctrl.before;
-      if (linear) {
-        // the keys of the crossing bin: [least with linear_bin <= bin, largest with linear_bin >= bin], each by a
-        // 32-way search
-        auto search = [&](auto pred, uint32_t a, uint32_t b) {   // least key in [a, b] with pred, which holds at b
-          while (a < b) {
-            const uint32_t step = (b - a) / 32 + 1;
-            const u64 far = a + static_cast<u64>(step) * lane;
-            const uint32_t x = far < b ? static_cast<uint32_t>(far) : b;
-            const uint32_t yes = __ballot_sync(kAll, x == b || pred(x));
-            const int f = yes != 0 ? __ffs(yes) - 1 : 32;   // points below f: no, point f: yes
-            const uint32_t below = __shfl_sync(kAll, x, f > 0 ? f - 1 : 0);
-            const uint32_t at = __shfl_sync(kAll, x, f < 32 ? f : 0);
-            if (f > 0) a = below + 1;
-            b = f == 0 ? a : f < 32 ? at : b;
-          }
-          return b;
-        };
-        const int ib = static_cast<int>(bin);
-        const uint32_t nlo = search([&](uint32_t k) { return linear_bin(k) <= ib; }, lo, hi);
-        const uint32_t past = ib == 0 ? hi + 1 : search([&](uint32_t k) { return linear_bin(k) < ib; }, nlo, hi);
-        lo = nlo;
-        hi = ib == 0 ? hi : max(nlo, past - 1);
-        linear = false;
-      } else {
-        const uint32_t nhi = hi - (bin << shift);
-        lo = (nhi - lo) >> shift == 0 ? lo : nhi - ((1u << shift) - 1u);
-        hi = nhi;
-      }
-      if (lo == hi) return lo;
+      const uint32_t nhi = hi - (bin << shift);
+      lo = (nhi - lo) >> shift == 0 ? lo : nhi - ((1u << shift) - 1u);
+      hi = nhi;
     }
+    // equals of the threshold that still belong
+    cut = R::value(lo);
+    if constexpr (kMass) {
+      const double w = static_cast<double>(weight(cut));
+      const double want = fmax(ceil((ctrl.target - static_cast<double>(before)) / w), 1.0);
+      const uint32_t limit = cut == floor ? cut_ties : kNone;
+      cut_ties = min(limit, static_cast<uint32_t>(fmin(want, 4.0e9)));
+    } else {
+      cut_ties = k - static_cast<uint32_t>(before);
+    }
+    __syncthreads();   // (ctrl is read)
   };
 
   if (p.top_k != nullptr) {
     const int k = __ldg(p.top_k + set);
-    if (k > 0 && k < p.vocab) {
-      // fewer than k tokens may have passed min-p: count them first
-      uint32_t c = 0;
-      if (floor_key > least) {
-        for (int w = tid; w < words; w += kThreads)
-          each(keys[w], [&](uint32_t key, int) { c += key > cut ? 1u : 0u; });
-        u64 none = 0, tm;
-        uint32_t tc;
-        block_scan(none, c, scan_m, scan_c, &tm, &tc, lane, warp);
-        if (tid == 0) ctrl.ties = tc;
-        cluster.sync();
-        c = 0;
-        for (int r = 0; r < ranks; ++r) c += cluster.map_shared_rank(&ctrl, r)->ties;
-        cluster.sync();
-      } else {
-        c = static_cast<uint32_t>(p.vocab);
-      }
-      if (c > static_cast<uint32_t>(k)) {
-        u64 above;
-        cut = select(std::false_type{}, static_cast<double>(k), above);
-        cut_ties = static_cast<uint32_t>(k - static_cast<int>(above));
-      }
+    if (k > 0 && k < p.vocab) select(std::false_type{}, static_cast<uint32_t>(k), 0.0);
+  }
+  if (p.top_p != nullptr) {
+    const double tp = __ldg(p.top_p + set);
+    if (tp < 1.0) {
+      cluster.sync();   // (rank 0 has read every CTA's bins)
+      select(std::true_type{}, 0, fmax(tp, 0.0));
     }
   }
-  // kept weight of this thread's run and of the runs and CTAs before it
-  u64 mine, total, pre_m;
-  uint32_t ties, pre_c, total_c;
-  auto sums = [&](u64 w_cut) {
-    mine = 0;
-    ties = 0;
+
+  // ---------------------------------------------------------------- the draw
+  // kept weight of this thread's run, of the runs and CTAs before it, and of all
+  const u64 w_cut = cut_ties > 0 ? weight(cut) : 0ull;
+  u64 mine = 0;
+  uint32_t ties = 0;
+  {
+    const float above = fmaxf(cut, weight.low);
+    uint32_t heavy = 0;
     for (int w = run0; w < run0 + p.run_words; ++w)
-      each(keys[w], [&](uint32_t k, int) {
-        if (k > cut) mine += weight(K::value(k));
-        ties += k == cut ? 1u : 0u;
+      R::each(data[w], [&](float l, int) {
+        if (l > above) {
+          mine += weight.bits(l);
+          ++heavy;
+        }
+        ties += l == cut ? 1u : 0u;
       });
-    pre_m = mine;
-    pre_c = ties;
+    mine -= heavy * Weight::kZero;
+  }
+  u64 pre_m = mine, total = 0;
+  uint32_t pre_c = ties, total_c = 0;
+  {
     u64 tm;
     uint32_t tc;
     block_scan(pre_m, pre_c, scan_m, scan_c, &tm, &tc, lane, warp);
     if (tid == 0) {
       ctrl.sum = tm;
       ctrl.ties = tc;
+      ctrl.draft_weight = 0;
     }
     cluster.sync();
-    total = 0;
-    total_c = 0;
     for (int r = 0; r < ranks; ++r) {
       const Control* c = cluster.map_shared_rank(&ctrl, r);
       const u64 s = c->sum;
@@ -510,53 +596,28 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       total += s;
       total_c += t;
     }
-    // the first cut_ties tokens at the cut, in index order
     total += w_cut * min(cut_ties, total_c);
-  };
-  auto cut_weight = [&]() { return cut_ties > 0 ? weight(K::value(cut)) : 0ull; };
-
-  if (p.top_p != nullptr) {
-    const double tp = __ldg(p.top_p + set);
-    if (tp < 1.0) {
-      sums(cut_weight());
-      cluster.sync();   // (the controls are read; select writes them)
-      u64 above;
-      const double target = fmax(tp, 0.0) * static_cast<double>(total);
-      // (the first token always stays: a target of 0 would find no crossing)
-      const uint32_t key = select(std::true_type{}, fmax(target, 1.0), above);
-      const double w = static_cast<double>(weight(K::value(key)));
-      const double want = ceil((fmax(target, 1.0) - static_cast<double>(above)) / w);
-      const uint32_t limit = key == cut ? cut_ties : 0xFFFFFFFFu;
-      cut = key;
-      cut_ties = min(limit, static_cast<uint32_t>(fmin(fmax(want, 1.0), 4.0e9)));
-    }
   }
-
-  // ---------------------------------------------------------------- the draw
-  const u64 w_cut = cut_weight();
-  sums(w_cut);
   const uint32_t own_ties = min(cut_ties, pre_c + ties) - min(cut_ties, pre_c);   // of this run, kept
   u64 kept = mine + w_cut * own_ties;
   u64 at = pre_m + w_cut * min(cut_ties, pre_c);   // kept weight before this run
-  u64 draft_w = 0;
   bool accepted = false;
   if constexpr (kVerify) {
     // the draft's own weight, from the thread whose run holds it, to everyone
     const int dw = draft >= 0 && draft < p.vocab ? draft / kPer - e0 / kPer : -1;   // its word in this CTA
-    if (tid == 0) ctrl.draft_weight = 0;
-    cluster.sync();
     if (dw >= run0 && dw < run0 + p.run_words) {
-      uint32_t seen = pre_c, key = 0;
+      uint32_t seen = pre_c;
+      float l = 0.f;
       for (int w = run0; w <= dw; ++w)
-        each(keys[w], [&](uint32_t k, int h) {
-          if (w == dw && h == draft % kPer) key = k;
-          if (w < dw || h < draft % kPer) seen += k == cut ? 1u : 0u;
+        R::each(data[w], [&](float x, int h) {
+          if (w == dw && h == draft % kPer) l = x;
+          if (w < dw || h < draft % kPer) seen += x == cut ? 1u : 0u;
         });
-      const u64 v = key > cut ? weight(K::value(key)) : (key == cut && seen < cut_ties) ? w_cut : 0ull;
+      const u64 v = l > cut ? weight(l) : (l == cut && seen < cut_ties) ? w_cut : 0ull;
       for (int r = 0; r < ranks; ++r) cluster.map_shared_rank(&ctrl, r)->draft_weight = v;
     }
     cluster.sync();
-    draft_w = ctrl.draft_weight;
+    const u64 draft_w = ctrl.draft_weight;
     if (draft >= 0) {
       const double ua = read_uniform(p.accept_uniform, set * p.accept_stride + (row - set * p.group), p.uniform_bytes);
       accepted = ua * static_cast<double>(total) < static_cast<double>(draft_w);
@@ -592,15 +653,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     uint32_t seen = found_ties;
     for (int base = 0; base < count; base += 32) {
       const int e = base + lane;
-      uint32_t k = 0;
-      if (e < count) {
-        const uint32_t w = keys[first_word + e / kPer];
-        k = kPer == 2 ? ((e & 1) ? w >> 16 : w & 0xFFFFu) : w;
-      }
-      const bool tie = k == cut;
+      float l = __int_as_float(0x7FFFFFFF);
+      if (e < count)
+        R::each(data[first_word + e / kPer], [&](float x, int h) { l = h == e % kPer ? x : l; });
+      const bool tie = l == cut;
       const uint32_t tie_vote = __ballot_sync(kAll, tie);
       const bool tie_kept = tie && seen + __popc(tie_vote & ((1u << lane) - 1u)) < cut_ties;
-      u64 v = k > cut ? weight(K::value(k)) : tie_kept ? w_cut : 0ull;
+      u64 v = l > cut ? weight(l) : tie_kept ? w_cut : 0ull;
       const int token = e0 + first_word * kPer + e;
       if (kVerify && token == draft) v = 0;
       u64 x = v;
@@ -644,7 +703,7 @@ __global__ void __launch_bounds__(128) verify_merge_kernel(const int2* __restric
 
 template <typename T, bool kVerify>
 cudaError_t launch_rows(SampleParams p, int sms, cudaStream_t stream) {
-  constexpr int kPer = KeyOf<T>::kPerWord;
+  constexpr int kPer = Row<T>::kPerWord;
   const int words = (p.vocab + kPer - 1) / kPer;
   // CTAs per row: a share of at most 80 KB, so that two CTAs fit an SM and one row's exchange runs beside another's
   // loads; more of them when there are few rows (but at least 4 KB each)
