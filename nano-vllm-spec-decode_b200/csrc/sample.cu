@@ -97,10 +97,9 @@ template <>
 struct Row<__nv_bfloat16> {
   static constexpr int kPerWord = 2;
   static constexpr uint32_t kPad = 0xFFFFu;
-  static __device__ __forceinline__ uint32_t numbers(uint32_t w) {   // NaN to -inf
-    const uint32_t low = 0xFF80FF80u;
-    const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w),
-                                     *reinterpret_cast<const __nv_bfloat162*>(&low));
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {   // the number where one is NaN
+    const __nv_bfloat162 v =
+        __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
   template <class F>
@@ -120,8 +119,8 @@ template <>
 struct Row<float> {
   static constexpr int kPerWord = 1;
   static constexpr uint32_t kPad = 0xFFFFFFFFu;
-  static __device__ __forceinline__ uint32_t numbers(uint32_t w) {
-    return __float_as_uint(fmaxf(__uint_as_float(w), __uint_as_float(0xFF800000u)));
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
   }
   template <class F>
   static __device__ __forceinline__ void each(uint32_t w, F&& f) { f(__uint_as_float(w), 0); }
@@ -160,7 +159,7 @@ struct Weight {
     s = fma(s, r, 0.0027076061740622863);                                // ln 2 / 256
     s = fma(s, r, 1.0);
     const double t = table[k & 255];
-    const double scaled = __hiloint2double(__double2hiint(t) + ((k >> 8) << 20), __double2loint(t));
+    const double scaled = __hiloint2double(__double2hiint(t) + ((k & ~255) << 12), __double2loint(t));   // + e << 20
     return __double_as_longlong(fma(s, scaled, 4503599627370496.0));
   }
   static constexpr u64 kZero = 0x4330000000000000ull;   // the bits of 2^52
@@ -218,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   extern __shared__ __align__(16) uint8_t smem[];
   const int words = p.run_words * kThreads;
   uint32_t* data = reinterpret_cast<uint32_t*>(smem);
-  __shared__ uint32_t hist[2][kBins];          // counts, or weights: low and high words
+  __shared__ __align__(16) uint32_t hist[2][kBins];          // counts, or weights: low and high words
   __shared__ double table[kTable];
   __shared__ uint32_t list[kList];
   __shared__ uint32_t list_count;
@@ -241,13 +240,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     const T* src = static_cast<const T*>(p.logits) + row * p.row_stride + e0;
     const uint32_t* src32 = reinterpret_cast<const uint32_t*>(src);
     bool nan = false;
+    const uint32_t low = kPer == 2 ? 0xFF80FF80u : 0xFF800000u;   // -inf
+    uint32_t best = low;
     auto keep = [&](uint32_t w) -> uint32_t {
-      if (greedy) {
-        R::each(w, [&](float l, int) { nan |= l != l; });
-      }
-      const uint32_t x = R::numbers(w);
-      R::each(x, [&](float l, int) { top = fmaxf(top, l); });
-      return greedy ? w : x;
+      const uint32_t x = R::larger(w, low);
+      best = R::larger(best, x);
+      if (!greedy) return x;
+      R::each(w, [&](float l, int) { nan |= l != l; });
+      return w;
     };
     int done = 0;   // words in place
     if ((reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     }
     for (int w = done + tid; w < words; w += kThreads) {
       // (the row's end) padding takes no part in the maximum
-      uint32_t x = kPer == 2 ? 0xFF80FF80u : 0xFF800000u, pad = 0;
+      uint32_t x = low, pad = 0;
 #pragma unroll
       for (int h = 0; h < kPer; ++h) {
         const int e = w * kPer + h;
@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       data[w] = keep(x) | pad;   // (-inf's bits are among the padding's NaN's)
     }
     if (tid < kTable) table[tid] = exp2(static_cast<double>(tid) / kTable + 44.0);
+    R::each(best, [&](float l, int) { top = fmaxf(top, l); });
     if (nan) top = __int_as_float(0x7FFFFFFF);
     // (as keys: NaN, possible only when greedy, above +inf)
     uint32_t k = __float_as_uint(top + 0.f);
@@ -298,8 +299,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   }
   cluster.sync();
   {
-    uint32_t k = 0;
-    for (int r = 0; r < ranks; ++r) k = max(k, cluster.map_shared_rank(&ctrl, r)->first);
+    // (lane r reads CTA r's: one trip, not one per CTA)
+    const uint32_t k = __reduce_max_sync(kAll, lane < ranks ? cluster.map_shared_rank(&ctrl, lane)->first : 0u);
     top = __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
   }
   const int run0 = tid * p.run_words;          // this thread's run of words
@@ -401,13 +402,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     auto cross = [&](u64 before, bool linear) {
       if (rank == 0) {
         u64 v[2] = {0, 0};
-        uint32_t last = 0;
-        for (int r = 0; r < ranks; ++r) {
-          const uint32_t* h = cluster.map_shared_rank(&hist[0][0], r);
+        uint2 low[kMaxCluster], high[kMaxCluster];   // (every CTA's bins on their way at once)
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            v[i] += h[2 * tid + i] + (kMass ? static_cast<u64>(h[kBins + 2 * tid + i]) << 32 : 0ull);
-          if (!kMass && linear) last += cluster.map_shared_rank(&ctrl, r)->last;
+        for (int r = 0; r < kMaxCluster; ++r) {
+          low[r] = high[r] = make_uint2(0u, 0u);
+          if (r < ranks) {
+            const uint2* h = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[0][0], r));
+            low[r] = h[tid];
+            if constexpr (kMass) high[r] = h[kBins / 2 + tid];
+          }
+        }
+        uint32_t last = 0;
+        if (!kMass && linear && warp == 0)
+          last = __reduce_add_sync(kAll, lane < ranks ? cluster.map_shared_rank(&ctrl, lane)->last : 0u);
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {
+          v[0] += low[r].x + (static_cast<u64>(high[r].x) << 32);
+          v[1] += low[r].y + (static_cast<u64>(high[r].y) << 32);
         }
         u64 pre = v[0] + v[1], tot;
         uint32_t none = 0, none_t;
@@ -496,6 +507,55 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           }
         });
     }
+    if (lo < hi) {
+      // Few tokens in all: rank 0 takes everyone's, one per thread, and each thread adds up what lies above its token
+      // and what equals it.
+      cluster.sync();
+      const uint32_t mine = lane < ranks ? *cluster.map_shared_rank(&list_count, lane) : 0u;
+      const uint32_t all = __reduce_add_sync(kAll, mine);
+      const uint32_t longest = __reduce_max_sync(kAll, mine);
+      if (all + 1 <= kThreads && longest <= kList) {
+        if (rank == 0) {
+          uint32_t* keys = &hist[0][0];                                     // (the histogram has been read)
+          u64* masses = reinterpret_cast<u64*>(&hist[1][0]);
+          uint32_t first = 0, key = 0;
+          u64 v = 0;
+          for (int r = 0; r < ranks; ++r) {   // the CTA whose list holds this thread's token
+            const uint32_t c = __shfl_sync(kAll, mine, r);
+            if (static_cast<uint32_t>(tid) >= first && static_cast<uint32_t>(tid) < first + c)
+              key = cluster.map_shared_rank(&list[0], r)[tid - first];
+            first += c;
+          }
+          if (key != 0) v = kMass ? weight(R::value(key)) : 1ull;
+          if (kMass && static_cast<uint32_t>(tid) == all && w_floor != 0 && R::key(floor) >= lo && R::key(floor) <= hi) {
+            key = R::key(floor);
+            v = w_floor;
+          }
+          keys[tid] = key;
+          if constexpr (kMass) masses[tid] = v;
+          __syncthreads();
+          u64 above = before, same = 0;
+          const int count = static_cast<int>(all) + (kMass ? 1 : 0);
+          if (v != 0)
+            for (int i = 0; i < count; ++i) {
+              const uint32_t k = keys[i];
+              const u64 x = kMass ? masses[i] : 1ull;
+              above += k > key ? x : 0ull;
+              same += k == key ? x : 0ull;
+            }
+          const double target = ctrl.target;
+          if (v != 0 && static_cast<double>(above) < target && static_cast<double>(above + same) >= target)
+            for (int r = 0; r < ranks; ++r) {   // (equal tokens say the same)
+              Control* c = cluster.map_shared_rank(&ctrl, r);
+              c->bin = key;
+              c->before = above;
+            }
+        }
+        cluster.sync();
+        lo = hi = ctrl.bin;
+        before = ctrl.before;
+      }
+    }
     while (lo < hi) {
       __syncthreads();
       const uint32_t listed = list_count;
@@ -561,17 +621,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   u64 mine = 0;
   uint32_t ties = 0;
   {
-    const float above = fmaxf(cut, weight.low);
-    uint32_t heavy = 0;
-    for (int w = run0; w < run0 + p.run_words; ++w)
-      R::each(data[w], [&](float l, int) {
-        if (l > above) {
-          mine += weight.bits(l);
-          ++heavy;
-        }
-        ties += l == cut ? 1u : 0u;
-      });
-    mine -= heavy * Weight::kZero;
+    if (cut <= weight.low) {
+      // nothing cut off: (nearly) every token has a weight, so all lanes take one and the few without drop theirs
+      const float low = weight.low;
+#pragma unroll 4
+      for (int w = run0; w < run0 + p.run_words; ++w)
+        R::each(data[w], [&](float l, int) {
+          const bool on = l > low;
+          const u64 b = weight.bits(on ? l : top);
+          mine += on ? b : Weight::kZero;
+        });
+      mine -= static_cast<u64>(p.run_words * kPer) * Weight::kZero;
+    } else {
+      for (int w = run0; w < run0 + p.run_words; ++w)
+        R::each(data[w], [&](float l, int) {
+          if (l > cut) mine += weight.bits(l) - Weight::kZero;
+        });
+    }
+    if (cut_ties > 0)
+      for (int w = run0; w < run0 + p.run_words; ++w)
+        R::each(data[w], [&](float l, int) { ties += l == cut ? 1u : 0u; });
   }
   u64 pre_m = mine, total = 0;
   uint32_t pre_c = ties, total_c = 0;
@@ -585,17 +654,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       ctrl.draft_weight = 0;
     }
     cluster.sync();
-    for (int r = 0; r < ranks; ++r) {
-      const Control* c = cluster.map_shared_rank(&ctrl, r);
-      const u64 s = c->sum;
-      const uint32_t t = c->ties;
-      if (r < rank) {
-        pre_m += s;
-        pre_c += t;
-      }
-      total += s;
-      total_c += t;
+    u64 s = 0;
+    uint32_t t = 0;
+    if (lane < ranks) {
+      const Control* c = cluster.map_shared_rank(&ctrl, lane);
+      s = c->sum;
+      t = c->ties;
     }
+    u64 before = lane < rank ? s : 0ull;
+#pragma unroll
+    for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(kAll, before, o);
+      s += __shfl_xor_sync(kAll, s, o);
+    }
+    pre_m += __shfl_sync(kAll, before, 0);
+    total = __shfl_sync(kAll, s, 0);
+    pre_c += __reduce_add_sync(kAll, lane < rank ? t : 0u);
+    total_c = __reduce_add_sync(kAll, t);
     total += w_cut * min(cut_ties, total_c);
   }
   const uint32_t own_ties = min(cut_ties, pre_c + ties) - min(cut_ties, pre_c);   // of this run, kept
