@@ -285,10 +285,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     }
     if (tid < kTable) table[tid] = exp2(static_cast<double>(tid) / kTable + 44.0);
     R::each(best, [&](float l, int) { top = fmaxf(top, l); });
-    if (nan) top = __int_as_float(0x7FFFFFFF);
-    // (as keys: NaN, possible only when greedy, above +inf)
+    // as a key (NaN, which only a greedy row looks for, above +inf)
     uint32_t k = __float_as_uint(top + 0.f);
-    k = (k & 0x80000000u) ? ~k : (k | 0x80000000u);
+    k = nan ? kNone : (k & 0x80000000u) ? ~k : (k | 0x80000000u);
     k = __reduce_max_sync(kAll, k);
     if (lane == 0) scan_c[warp] = k;
     __syncthreads();

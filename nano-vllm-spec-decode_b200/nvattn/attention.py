@@ -7,6 +7,9 @@ Same constructor, attributes and forward contract as the reference's Attention (
     per-step Context: slot_mapping for the KV scatter (skipped while the cache is empty, e.g. warmup),
     then either the varlen branch (is_prefill; paged cache when block_tables is set) or the decode / verify
     branch (every sequence brings T / num_seqs query tokens, causal bottom-right over context_lens).
+With an 8-bit cache (k_cache / v_cache float8_e4m3fn) k_scale / v_scale hold its scales (ops.kvcache_scales makes them):
+K/V rows are rounded as they are stored, and every branch that reads the cache reads the 8-bit values; a prefill without
+a block table still attends over its own bf16 K/V.
 The work runs in libnvattn.so kernels on the current stream; nothing here syncs or reads device values, so the
 decode branch can be captured in CUDA graphs exactly as the reference's is.
 """
@@ -27,12 +30,13 @@ class Attention(nn.Module):
         self.scale = scale
         self.num_kv_heads = num_kv_heads
         self.k_cache = self.v_cache = torch.tensor([])
+        self.k_scale = self.v_scale = None      # 8-bit cache: float32 [NB, KVH, BS / G]
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
         context = get_context()
         k_cache, v_cache = self.k_cache, self.v_cache
         if k_cache.numel() and v_cache.numel():
-            ops.store_kvcache(k, v, k_cache, v_cache, context.slot_mapping)
+            ops.store_kvcache(k, v, k_cache, v_cache, context.slot_mapping, self.k_scale, self.v_scale)
         return self.forward_stored(q, k, v)
 
     def forward_stored(self, q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None):
@@ -42,16 +46,18 @@ class Attention(nn.Module):
         context = get_context()
         k_cache, v_cache = self.k_cache, self.v_cache
         if context.is_prefill:
+            k_scale = v_scale = None
             if context.block_tables is not None:    # prefix cache / chunked prefill / mixed batch
-                k, v = k_cache, v_cache
+                k, v, k_scale, v_scale = k_cache, v_cache, self.k_scale, self.v_scale
             o = ops.flash_attn_varlen_func(q, k, v, max_seqlen_q=context.max_seqlen_q,
                                            cu_seqlens_q=context.cu_seqlens_q, max_seqlen_k=context.max_seqlen_k,
                                            cu_seqlens_k=context.cu_seqlens_k, softmax_scale=self.scale, causal=True,
-                                           block_table=context.block_tables)
+                                           block_table=context.block_tables, k_scale=k_scale, v_scale=v_scale)
         else:    # decode: every sequence brings the same number of query tokens (1, or 1+k when verifying)
             num_seqs = context.context_lens.size(0)
             q = q.reshape(num_seqs, -1, self.num_heads, self.head_dim)
             o = ops.flash_attn_with_kvcache(q, k_cache, v_cache, cache_seqlens=context.context_lens,
-                                            block_table=context.block_tables, softmax_scale=self.scale, causal=True)
+                                            block_table=context.block_tables, softmax_scale=self.scale, causal=True,
+                                            k_scale=self.k_scale, v_scale=self.v_scale)
             o = o.view(-1, self.num_heads, self.head_dim)
         return o

@@ -85,7 +85,7 @@ def install_attention() -> None:
         allocate_kv_cache(self)
         attn = next(m for m in self.model.modules() if isinstance(m, vattn.Attention))
         ops.reserve_workspace(self.config.max_num_seqs, self.config.max_num_batched_tokens, attn.num_heads,
-                              attn.num_kv_heads, attn.head_dim)
+                              attn.num_kv_heads, attn.head_dim, fp8_cache=attn.k_scale is not None)
 
     mr.ModelRunner.allocate_kv_cache = runner_allocate_kv_cache
     _installed.add("attention")
@@ -228,12 +228,15 @@ def install_fused_prologue() -> None:
         qkv = self.qkv_proj(hidden_states)
         attn = self.attn
         ctx = get_context() if scatter else None
-        cache = scatter and attn.k_cache.numel() > 0
-        contiguous_kv = not scatter or (ctx.is_prefill and ctx.block_tables is None)
+        stored = scatter and attn.k_cache.numel() > 0
+        cache = stored and attn.k_scale is None     # an 8-bit cache is written by its own scatter below
+        contiguous_kv = not scatter or stored != cache or (ctx.is_prefill and ctx.block_tables is None)
         q, k, v = ops.qk_norm_rope_store(
             qkv, positions, self.rotary_emb.cos_sin_cache, self.q_norm.weight, self.k_norm.weight, self.q_norm.eps,
             self.num_heads, self.num_kv_heads, attn.k_cache if cache else None, attn.v_cache if cache else None,
             ctx.slot_mapping if cache else None, want_k=contiguous_kv)
+        if stored and not cache:
+            ops.store_kvcache(k, v, attn.k_cache, attn.v_cache, ctx.slot_mapping, attn.k_scale, attn.v_scale)
         return q, k, v
 
     def attention_forward(self, positions, hidden_states):

@@ -1,0 +1,278 @@
+"""Sampling and speculative sampling against the float64 restatement, token for token.  A draw whose uniform number lies
+within 1e-9 of a boundary between tokens (relative to the sum) may go either way in float64 itself; the cases are made
+with fixed seeds and none of them does (asserted)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import sampling
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(R, V, dtype, seed, size=2.5):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(R, V, generator=g) * size
+    return x.to(dtype), g
+
+
+def run(x, t, u, **kw):
+    from nvattn.sampler import sample_tokens
+    dev = {k: v.cuda() for k, v in kw.items() if v is not None}
+    return sample_tokens(x.cuda() if not x.is_cuda else x, t.cuda(), u.cuda(), **dev).cpu()
+
+
+def check(x, t, u, top_k=None, top_p=None, min_p=None, got=None):
+    R = x.shape[0]
+    got = run(x, t, u, top_k=top_k, top_p=top_p, min_p=min_p) if got is None else got
+    host = x.float().cpu().numpy()
+    for r in range(R):
+        want, margin = sampling.sample(host[r], float(t[r]), float(u[r]),
+                                       int(top_k[r]) if top_k is not None else 0,
+                                       float(top_p[r]) if top_p is not None else 1.0,
+                                       float(min_p[r]) if min_p is not None else 0.0)
+        assert margin > 1e-9 or got[r] == want, "the case itself is undecided"
+        assert int(got[r]) == want, (r, int(got[r]), want)
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [1, 2, 7, 31, 33, 255, 1000, 4097, 32003])
+def test_vocabularies(cuda, V, dtype):
+    R = 12
+    x, g = rows(R, V, dtype, V)
+    u = torch.rand(R, generator=g)
+    t = torch.rand(R, generator=g) * 1.5 + 0.2
+    check(x, t, u)
+    check(x, t, u, top_k=torch.randint(0, max(V, 2), (R,), generator=g).int())
+    check(x, t, u, top_p=torch.rand(R, generator=g))
+    check(x, t, u, min_p=torch.rand(R, generator=g) * 0.3)
+    t[::3] = 0
+    check(x, t, u.double(), top_k=torch.randint(0, 60, (R,), generator=g).int(), top_p=torch.rand(R, generator=g),
+          min_p=torch.rand(R, generator=g) * 0.05)
+
+
+@pytest.mark.parametrize("R,dtype", [(1, torch.bfloat16), (5, torch.float32), (40, torch.bfloat16)])
+def test_a_whole_vocabulary(cuda, R, dtype):
+    x, g = rows(R, 151936, dtype, R)
+    u = torch.rand(R, generator=g, dtype=torch.float64)
+    t = torch.rand(R, generator=g) + 0.4
+    check(x, t, u)
+    check(x, t, u, top_p=torch.full((R,), 0.97), top_k=torch.randint(0, 5000, (R,), generator=g).int())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_any_alignment_and_row_stride(cuda, dtype):
+    base = torch.randn(9, 5003, generator=torch.Generator().manual_seed(1)).to(dtype).cuda() * 2
+    g = torch.Generator().manual_seed(2)
+    u, t = torch.rand(9, generator=g), torch.ones(9)
+    for lo, hi in ((0, 5003), (1, 4001), (3, 5000), (8, 1000)):
+        check(base[:, lo:hi], t, u, top_p=torch.full((9,), 0.9))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_equal_logits(cuda, dtype):
+    """Flat rows and rows of a few values: ties at every threshold go to the lowest indices."""
+    V = 4000
+    R = 24
+    g = torch.Generator().manual_seed(3)
+    flat = torch.full((R, V), 1.5).to(dtype)
+    few = torch.randint(0, 4, (R, V), generator=g).to(dtype)
+    u = torch.rand(R, generator=g, dtype=torch.float64)
+    t = torch.ones(R)
+    for x in (flat, few):
+        check(x, t, u)
+        check(x, t, u, top_k=torch.arange(1, R + 1).int() * 37)
+        check(x, t, u, top_k=torch.full((R,), 700).int(), top_p=torch.arange(R) / R)
+    # thresholds that fall on a whole number of equal weights
+    check(flat, t, u, top_p=torch.full((R,), 0.5))
+    got = run(flat, t, torch.full((R,), 0.9999), top_p=torch.full((R,), 0.25))
+    assert (got == 999).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_infinities_nan_and_masks(cuda, dtype):
+    g = torch.Generator().manual_seed(4)
+    V = 3000
+    x = (torch.randn(12, V, generator=g) * 2).to(dtype)
+    low = torch.finfo(dtype).min
+    x[0] = float("-inf")                                   # nothing left: every token alike
+    x[1] = float("-inf")
+    x[1, 2222] = -3.0                                      # one token left
+    x[2, 7] = x[2, 1999] = float("inf")                    # the infinite ones share everything
+    x[3, ::2] = float("nan")                               # no numbers: never drawn
+    x[4] = low                                             # the type's lowest value everywhere
+    x[5] = low
+    x[5, 100:105] = 1.0
+    x[6, 50:] = float("-inf")
+    x[7] = float("nan")
+    x[8] = torch.finfo(dtype).max
+    x[9, :] = -0.0
+    x[9, ::3] = 0.0
+    u = torch.rand(12, generator=g)
+    t = torch.tensor([1.0, 0.5, 1.0, 1.0, 1.0, 1.0, 0.7, 1.0, 1.0, 1.0, 1e-30, 3e38])
+    none = dict(top_k=None, top_p=None, min_p=None)
+    check(x, t, u, **none)
+    check(x, t, u, top_k=torch.full((12,), 5).int())
+    check(x, t, u, top_p=torch.full((12,), 0.5), min_p=torch.full((12,), 0.01))
+    got = run(x, torch.zeros(12), u)                       # greedy: torch's argmax, NaN above everything
+    assert got.tolist() == [sampling.argmax(r) for r in x.float().numpy()]
+    assert got.tolist() == x.float().argmax(-1).tolist()
+
+
+def test_extreme_settings(cuda):
+    x, g = rows(10, 5000, torch.float32, 6)
+    one = torch.ones(10)
+    best = x.argmax(-1)
+    u = torch.rand(10, generator=g)
+    assert torch.equal(run(x, one, u, top_k=torch.ones(10).int()), best)
+    assert torch.equal(run(x, one, u, top_p=torch.zeros(10)), best)
+    assert torch.equal(run(x, one, u, min_p=one), best)
+    assert torch.equal(run(x, one, u, min_p=one * 7), best)
+    assert torch.equal(run(x, one * -1, u), best) and torch.equal(run(x, one * float("nan"), u), best)
+    off = dict(top_k=torch.full((10,), -1).int(), top_p=one * 2, min_p=-one)
+    assert torch.equal(run(x, one, u, **off), run(x, one, u))
+    assert torch.equal(run(x, one, u, top_k=torch.full((10,), 5000).int()), run(x, one, u))
+    # the ends of the uniform numbers' range, and numbers outside it
+    kept = dict(top_k=torch.full((10,), 3).int())
+    three = x.topk(3).indices.sort(-1).values
+    assert torch.equal(run(x, one, torch.zeros(10), **kept), three[:, 0])
+    assert torch.equal(run(x, one, one * 1.5, **kept), three[:, 2])
+    assert torch.equal(run(x, one, one * float("nan"), **kept), three[:, 0])
+    assert torch.equal(run(x, one, -one, **kept), three[:, 0])
+    check(x, one * float("inf"), u)                         # an infinite temperature: all alike
+
+
+def test_low_temperatures_and_far_ranks(cuda):
+    """top-k whose last rank lies far below the maximum, and weights that vanish."""
+    x, g = rows(8, 30000, torch.float32, 7)
+    u = torch.rand(8, generator=g)
+    check(x, torch.full((8,), 0.05), u, top_k=torch.full((8,), 20000).int())
+    check(x, torch.full((8,), 0.01), u, top_p=torch.full((8,), 0.999))
+    check(x * 1000, torch.full((8,), 1.0), u, top_k=torch.full((8,), 25000).int(), top_p=torch.full((8,), 0.9999))
+
+
+# ---------------------------------------------------------------------------------------------- drafts
+def run_verify(x, d, nd, t, au, u, dtype=torch.int64, **kw):
+    from nvattn import ops
+    dev = {k: v.cuda() for k, v in kw.items()}
+    a, n = ops.verify_sampled(x.cuda(), d.to(dtype).cuda(), nd.to(dtype).cuda(), t.cuda(), au.cuda(), u.cuda(), **dev)
+    assert a.dtype == n.dtype == dtype
+    return a.cpu(), n.cpu()
+
+
+def check_verify(x, d, nd, t, au, u, dtype=torch.int64, **kw):
+    a, n = run_verify(x, d, nd, t, au, u, dtype, **kw)
+    S, K = d.shape
+    host = x.float().numpy().reshape(S, K + 1, -1)
+    for s in range(S):
+        want = sampling.verify(host[s], d[s].tolist(), int(nd[s]), float(t[s]), au[s].double().tolist(), float(u[s]),
+                               *(kw[k][s].item() if k in kw else z for k, z in (("top_k", 0), ("top_p", 1.0), ("min_p", 0.0))))
+        assert (int(a[s]), int(n[s])) == want, s
+    return a, n
+
+
+@pytest.mark.parametrize("S,K,V,dtype", [(1, 1, 50, torch.float32), (7, 2, 1000, torch.bfloat16),
+                                         (33, 4, 5001, torch.float32), (3, 8, 151936, torch.bfloat16),
+                                         (5, 0, 300, torch.bfloat16)])
+def test_verify(cuda, S, K, V, dtype):
+    x, g = rows(S * (K + 1), V, dtype, S * 17 + K)
+    x[:, ::97] += 4
+    likely = x.float().view(S, K + 1, V)[:, :K].argmax(-1)
+    d = torch.where(torch.rand(S, K, generator=g) < 0.7, likely, torch.randint(0, V, (S, K), generator=g))
+    nd = torch.randint(0, K + 1, (S,), generator=g)
+    nd[::2] = K
+    t = torch.rand(S, generator=g) + 0.3
+    t[2::4] = 0
+    au, u = torch.rand(S, K, generator=g) * 0.7, torch.rand(S, generator=g)
+    check_verify(x, d, nd, t, au, u)
+    check_verify(x, d, nd, t, au.double(), u.double(), torch.int32, top_k=torch.randint(1, 40, (S,), generator=g).int(),
+                 top_p=torch.rand(S, generator=g) * 0.5 + 0.5)
+    check_verify(x, d, nd, t, au, u, min_p=torch.full((S,), 0.05))
+
+
+def test_verify_drafts_at_the_edges(cuda):
+    """Drafts outside the vocabulary, drafts that the settings removed, a draft that holds all the weight, the same
+    token drafted again, ties with the draft among them."""
+    V = 600
+    x, g = rows(6 * 3, V, torch.float32, 9)
+    d = x.view(6, 3, V)[:, :2].argmax(-1)
+    d[0, 0] = V
+    d[1, 0] = -1
+    d[2, 0] = x.view(6, 3, V)[2, 0].argmin()                # removed by top-k
+    d[3] = d[3, 0]
+    x[4 * 3:] = 0.25                                       # flat rows: ties at the cut, the draft among them
+    d[4, 0], d[5, 0] = 9, 10
+    nd, one = torch.full((6,), 2), torch.ones(6)
+    au, u = torch.full((6, 2), 0.05), torch.rand(6, generator=g)
+    k = torch.full((6,), 10).int()
+    check_verify(x, d, nd, one, au, u, top_k=k)
+    check_verify(x, d, nd, one, au, u, top_k=torch.ones(6).int())
+    check_verify(x, d, nd, one, torch.full((6, 2), 0.9999), u, top_k=k, top_p=torch.full((6,), 0.7))
+
+
+def test_greedy_verify_is_verify_drafts_greedy(cuda):
+    from nvattn.sampler import verify_drafts_greedy, verify_drafts_sampled
+    x, g = rows(20 * 4, 3001, torch.bfloat16, 10)
+    x = (x * 2).round().cuda()                              # many ties
+    d = x.view(20, 4, -1)[:, :3].argmax(-1)
+    d[::3, 1] += 1
+    nd = torch.randint(0, 4, (20,), generator=g).cuda()
+    z = torch.zeros(20, device="cuda")
+    want = verify_drafts_greedy(x, d, nd)
+    got = verify_drafts_sampled(x, d, nd, z, torch.zeros(20, 3, device="cuda"), z)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+def test_speculation_draws_like_sampling(cuda):
+    """Over a grid of both uniform numbers: a token comes out (accepted or drawn instead) with its own probability."""
+    V, N = 9, 256
+    logits = torch.randn(1, V, generator=torch.Generator().manual_seed(11)) * 1.5
+    w = sampling.kept_weights(logits[0].numpy(), 0.8, top_p=0.95)
+    p = torch.from_numpy(w / w.sum())
+    grid = (torch.arange(N) + 0.5) / N
+    x = logits.repeat(2 * N * N, 1)
+    d = torch.full((N * N, 1), 4)
+    one = torch.ones(N * N)
+    a, n = run_verify(x, d, one.long(), one * 0.8, grid.repeat_interleave(N)[:, None], grid.repeat(N),
+                      top_p=one * 0.95)
+    first = torch.where(a > 0, d[:, 0], n)
+    freq = torch.bincount(first, minlength=V).double() / (N * N)
+    assert float((freq - p).abs().max()) <= 2 / N           # a grid of N points is off by 1 / N per boundary
+
+
+def test_replayed_graph_and_another_stream(cuda):
+    from nvattn import ops, sampler
+    S, K, V = 16, 3, 20000
+    x, g = rows(S * (K + 1), V, torch.bfloat16, 12)
+    xd = x.cuda()
+    u, au = torch.zeros(S, device="cuda"), torch.zeros(S, K, device="cuda")
+    t = torch.full((S,), 0.9, device="cuda")
+    p = torch.full((S,), 0.9, device="cuda")
+    d = xd.float().view(S, K + 1, V)[:, :K].argmax(-1)
+    nd = torch.full((S,), K, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            ids = sampler.sample_tokens(xd[:S], t, u, top_p=p)
+            held = ops.verify_sampled(xd, d, nd, t, au, u, top_p=p)
+        for _ in range(4):
+            u.copy_(torch.rand(S, generator=g))
+            au.copy_(torch.rand(S, K, generator=g))
+            graph.replay()
+            want = sampler.sample_tokens(xd[:S], t, u, top_p=p), *ops.verify_sampled(xd, d, nd, t, au, u, top_p=p)
+            for a, b in zip((ids, *held), want):
+                assert torch.equal(a, b)
+    side.synchronize()
+    check(x[:S], t.cpu(), u.cpu(), top_p=p.cpu(), got=ids.cpu())
+
+
+def test_no_rows(cuda):
+    from nvattn import ops, sampler
+    e = torch.zeros(0, device="cuda")
+    assert sampler.sample_tokens(torch.zeros(0, 50, device="cuda"), e, e).shape == (0,)
+    a, n = ops.verify_sampled(torch.zeros(0, 50, device="cuda"), torch.zeros(0, 2, dtype=torch.int64, device="cuda"),
+                              torch.zeros(0, dtype=torch.int64, device="cuda"), e, torch.zeros(0, 2, device="cuda"), e)
+    assert a.shape == n.shape == (0,)
