@@ -198,7 +198,7 @@ NVA_API int nva_paged_decode_noalloc(const void* q, int64_t q_row_stride, const 
  * the value held in slot s of block b is cache[b, s, h, :] * scale[b, h, s / scale_block].  scale_block is a power of
  * two from NVA_MIN_SCALE_BLOCK to NVA_MAX_SCALE_BLOCK that divides BS; NB * BS < 2^31.  head_dim 128.
  *
- * nva_store_kvcache_fp8: nva_store_kvcache's scatter of bf16 rows (8-byte aligned, row strides multiples of 4), rounded
+ * nva_store_kvcache_fp8: nva_store_kvcache's scatter of bf16 rows (16-byte aligned, row strides multiples of 8), rounded
  * on the way.  With amax the largest finite magnitude that the call writes to a scale block (per head, k and v apart)
  * and e the least whole number with amax <= 448 * 2^e, kept in [-40, 40]:
  *     scale' = 2^e when the call writes the block's first slot (the block starts afresh), else max(scale, 2^e)

@@ -19,6 +19,8 @@
 // second launch, no workspace, and a result that depends on nothing but the arguments (a slot named twice keeps its
 // last token).  The rows of a block of 16 stay in registers between the two passes over them.
 #include <algorithm>
+#include <climits>
+#include <type_traits>
 #include <cuda_fp8.h>
 
 #include "../../include/nvattn.h"
@@ -29,11 +31,11 @@ namespace nva {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxChunk = 64;          // tokens of the call per CTA
 constexpr int kBitmapWords = 128;      // 4096 bits over block ids
-constexpr int kHeld = 16;              // rows of a block in registers at a time
+constexpr int kHeld = 8;               // row pairs of a block in registers at a time
 constexpr int kExpMin = -40, kExpMax = 40;
 
 struct StoreFp8Params {
@@ -50,14 +52,18 @@ struct StoreFp8Params {
   int32_t page_blocks;  // scale blocks per page
 };
 
-// Largest finite |x| of four bf16 values, as its 15 bits (ordered like the magnitudes).
-__device__ __forceinline__ uint32_t amax4(uint2 v) {
-  uint32_t m = 0;
+// Largest |x| of eight bf16 values with `m`'s, as their 15 bits (ordered like the magnitudes), two to a word.
+__device__ __forceinline__ uint32_t amax8(uint32_t m, uint4 v) {
+  m = __vmaxu2(m, __vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu));
+  return __vmaxu2(m, __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+}
+// The same over finite values only.
+__device__ __forceinline__ uint32_t amax8_finite(uint32_t m, uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t w = i < 2 ? v.x : v.y;
-    const uint32_t a = ((i & 1) ? (w >> 16) : w) & 0x7FFFu;
-    m = max(m, a < 0x7F80u ? a : 0u);
+    const uint32_t a = w[i] & 0x7FFF7FFFu;
+    m = __vmaxu2(m, a & __vcmpltu2(a, 0x7F807F80u));
   }
   return m;
 }
@@ -70,19 +76,23 @@ __device__ __forceinline__ float scale_of(uint32_t bits) {
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
-// Four bf16 values times inv, rounded to e4m3 (nearest even, saturating; NaN and infinities to NaN).
-__device__ __forceinline__ uint32_t quant4(uint2 v, float inv) {
-  uint32_t out = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t w = i == 0 ? v.x : v.y;
-    float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
-    // x * 0 is NaN for NaN and infinities, 0 otherwise
+// Two bf16 values times inv, rounded to e4m3 (nearest even, saturating; NaN and, with kAny, infinities to NaN).
+template <bool kAny>
+__device__ __forceinline__ uint32_t quant2(uint32_t w, float inv) {
+  float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+  if constexpr (kAny) {   // x * 0 is NaN for NaN and infinities, 0 otherwise
     f.x = fmaf(f.x, inv, f.x * 0.f);
     f.y = fmaf(f.y, inv, f.y * 0.f);
-    out |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3)) << (16 * i);
+  } else {
+    f.x *= inv;
+    f.y *= inv;
   }
-  return out;
+  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3));
+}
+template <bool kAny>
+__device__ __forceinline__ uint2 quant8(uint4 v, float inv) {
+  return make_uint2(quant2<kAny>(v.x, inv) | (quant2<kAny>(v.y, inv) << 16),
+                    quant2<kAny>(v.z, inv) | (quant2<kAny>(v.w, inv) << 16));
 }
 
 // Four e4m3 values times f (a power of two at most 1), rounded to e4m3.
@@ -101,7 +111,7 @@ __device__ __forceinline__ uint32_t requant4(uint32_t c, float f) {
 
 __device__ __forceinline__ uint32_t hash_block(int32_t b) { return (static_cast<uint32_t>(b) * 0x9E3779B1u) >> 20; }
 
-__global__ void __launch_bounds__(kThreads) store_fp8_kernel(const StoreFp8Params p) {
+__global__ void __launch_bounds__(kThreads, 2) store_fp8_kernel(const StoreFp8Params p) {
   extern __shared__ int32_t winner[];          // [entries][G]: 1 + the last token of the call written to the slot
   __shared__ int32_t blk[kMaxChunk];           // distinct blocks of this CTA's tokens
   __shared__ int32_t own_blk[kMaxChunk];       // block of each of its tokens (-1: none)
@@ -146,8 +156,15 @@ __global__ void __launch_bounds__(kThreads) store_fp8_kernel(const StoreFp8Param
   if (entries == 0) return;
 
   // the whole call's slots: who else writes these blocks
+  int32_t lo_slot = INT_MAX, hi_slot = -1;
+  for (int e = lane; e < entries; e += 32) {
+    lo_slot = min(lo_slot, blk[e]);
+    hi_slot = max(hi_slot, blk[e]);
+  }
+  lo_slot = __reduce_min_sync(0xffffffffu, lo_slot) << p.lg_block;
+  hi_slot = (__reduce_max_sync(0xffffffffu, hi_slot) << p.lg_block) + (G - 1);
   auto visit = [&](int i, int32_t slot) {
-    if (slot < 0 || slot >= p.num_slots) return;
+    if (slot < lo_slot || slot > hi_slot) return;   // (most of a call: other sequences' pages)
     const int32_t b = slot >> p.lg_block;
     const uint32_t h = hash_block(b);
     if (!((bitmap[h >> 5] >> (h & 31)) & 1u)) return;
@@ -160,13 +177,22 @@ __global__ void __launch_bounds__(kThreads) store_fp8_kernel(const StoreFp8Param
   };
   if ((reinterpret_cast<uintptr_t>(p.slots) & 15u) == 0) {
     const int nv = p.num_tokens >> 2;
-#pragma unroll 2
-    for (int v = tid; v < nv; v += kThreads) {
-      const int4 s = __ldg(reinterpret_cast<const int4*>(p.slots) + v);
-      visit(4 * v, s.x);
-      visit(4 * v + 1, s.y);
-      visit(4 * v + 2, s.z);
-      visit(4 * v + 3, s.w);
+    constexpr int kAhead = 4;
+    for (int v0 = tid; v0 < nv; v0 += kAhead * kThreads) {
+      int4 s[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        s[i] = v0 + i * kThreads < nv ? __ldg(reinterpret_cast<const int4*>(p.slots) + v0 + i * kThreads)
+                                      : make_int4(-1, -1, -1, -1);
+#pragma unroll 1
+      for (int i = 0; i < kAhead; ++i) {
+        const int v = v0 + i * kThreads;
+        const int4 t = i == 0 ? s[0] : i == 1 ? s[1] : i == 2 ? s[2] : s[3];
+        visit(4 * v, t.x);
+        visit(4 * v + 1, t.y);
+        visit(4 * v + 2, t.z);
+        visit(4 * v + 3, t.w);
+      }
     }
     for (int i = 4 * nv + tid; i < p.num_tokens; i += kThreads) visit(i, __ldg(p.slots + i));
   } else {
@@ -174,12 +200,15 @@ __global__ void __launch_bounds__(kThreads) store_fp8_kernel(const StoreFp8Param
   }
   __syncthreads();
 
-  // one warp per (block, head, k or v)
+  // one warp per (block, head, k or v), neighbouring warps on neighbouring heads: half a warp reads a row (16 bytes a
+  // lane), so that the 16 rows of a block are eight loads in flight
   const int tasks = entries * p.kv_heads * 2;
+  const int half = lane >> 4, col = (lane & 15) * 8;
+  const int64_t row = static_cast<int64_t>(p.kv_heads) * kHeadDim;
   for (int task = warp; task < tasks; task += kWarps) {
-    const int kv = task & 1;
-    const int e = (task >> 1) / p.kv_heads;
-    const int head = (task >> 1) - e * p.kv_heads;
+    const int head = task % p.kv_heads;
+    const int kv = (task / p.kv_heads) & 1;
+    const int e = task / (2 * p.kv_heads);
     if (earlier[e]) continue;
     const int32_t b = blk[e];
     const int32_t* win = winner + e * G;
@@ -187,45 +216,55 @@ __global__ void __launch_bounds__(kThreads) store_fp8_kernel(const StoreFp8Param
     float* scale = p.scale[kv] + (static_cast<int64_t>(page) * p.kv_heads + head) * p.page_blocks +
                    (b - page * p.page_blocks);
     const float old = *scale;
-    const __nv_bfloat16* src = p.src[kv] + head * kHeadDim + lane * 4;
+    const __nv_bfloat16* src = p.src[kv] + head * kHeadDim + col;
     const int64_t stride = p.src_stride[kv];
-    uint8_t* dst = p.cache[kv] + ((static_cast<int64_t>(b) << p.lg_block) * p.kv_heads + head) * kHeadDim + lane * 4;
-    const int64_t row = static_cast<int64_t>(p.kv_heads) * kHeadDim;
+    uint8_t* dst = p.cache[kv] + ((static_cast<int64_t>(b) << p.lg_block) * p.kv_heads + head) * kHeadDim + col;
     const bool fresh = win[0] != 0;
-    // pass 1: the largest magnitude
-    uint2 held[kHeld];
-    uint32_t m = 0;
-    for (int base = 0; base < G; base += kHeld) {
+    uint4 held[kHeld];
+    auto fetch = [&](int base) {
 #pragma unroll
-      for (int s = 0; s < kHeld; ++s) {
-        held[s] = make_uint2(0u, 0u);
-        const int w = base + s < G ? win[base + s] : 0;
-        if (w != 0) held[s] = __ldg(reinterpret_cast<const uint2*>(src + (w - 1) * stride));
+      for (int i = 0; i < kHeld; ++i) {
+        const int s = base + 2 * i + half;
+        const int w = s < G ? win[s] : 0;
+        held[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (w != 0) held[i] = __ldg(reinterpret_cast<const uint4*>(src + (w - 1) * stride));
       }
+    };
+    // pass 1: the largest magnitude
+    auto largest = [&](auto finite) {
+      uint32_t m = 0;
+      for (int base = 0; base < G; base += 2 * kHeld) {
+        if (G > 2 * kHeld || !decltype(finite)::value) fetch(base);
 #pragma unroll
-      for (int s = 0; s < kHeld; ++s) m = max(m, amax4(held[s]));
-    }
-    m = __reduce_max_sync(0xffffffffu, m);
+        for (int i = 0; i < kHeld; ++i) m = decltype(finite)::value ? amax8_finite(m, held[i]) : amax8(m, held[i]);
+      }
+      return __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
+    };
+    uint32_t m = largest(std::false_type{});
+    const bool any = m >= 0x7F80u;   // NaN or infinities among them: they have no say in the scale
+    if (any) m = largest(std::true_type{});
     const float now = fresh ? scale_of(m) : fmaxf(old, scale_of(m));
     const float inv = 1.0f / now;
-    const bool grew = !fresh && now > old;
-    const float factor = old * inv;
-    // pass 2: write the rows, round what the block held to the larger scale (blocks of more than 16 slots read their
-    // rows again, out of L1 / L2)
-    for (int base = 0; base < G; base += kHeld) {
+    // pass 2: write the rows (blocks of more than 16 slots read theirs again, out of L1 / L2)
+    for (int base = 0; base < G; base += 2 * kHeld) {
+      if (G > 2 * kHeld) fetch(base);
 #pragma unroll
-      for (int s = 0; s < kHeld; ++s) {
-        if (base + s >= G) break;
-        const int w = win[base + s];
-        uint8_t* at = dst + (base + s) * row;
-        if (w != 0) {
-          const uint2 x = G <= kHeld ? held[s] : __ldg(reinterpret_cast<const uint2*>(src + (w - 1) * stride));
-          *reinterpret_cast<uint32_t*>(at) = quant4(x, inv);
-        } else if (grew) {
-          const uint32_t c = *reinterpret_cast<const uint32_t*>(at);
-          *reinterpret_cast<uint32_t*>(at) = requant4(c, factor);
-        }
+      for (int i = 0; i < kHeld; ++i) {
+        const int s = base + 2 * i + half;
+        if (s < G && win[s] != 0)
+          *reinterpret_cast<uint2*>(dst + s * row) = any ? quant8<true>(held[i], inv) : quant8<false>(held[i], inv);
       }
+    }
+    if (!fresh && now > old) {
+      // the scale grew: what the block holds besides is rounded to it
+      const float factor = old * inv;
+#pragma unroll 4
+      for (int s = half; s < G; s += 2)
+        if (win[s] == 0) {
+          uint2* at = reinterpret_cast<uint2*>(dst + s * row);
+          const uint2 c = *at;
+          *at = make_uint2(requant4(c.x, factor), requant4(c.y, factor));
+        }
     }
     if (lane == 0) *scale = now;
   }
@@ -254,10 +293,10 @@ extern "C" NVA_API int nva_store_kvcache_fp8(const void* key, int64_t key_row_st
     return NVA_ERR_INVALID_ARGUMENT;
   const int64_t row_elems = static_cast<int64_t>(num_kv_heads) * head_dim;
   if (key_row_stride < row_elems || value_row_stride < row_elems) return NVA_ERR_INVALID_ARGUMENT;
-  // 8-byte vectors of the rows, 4-byte vectors of the cache
+  // 16-byte vectors of the rows, 8-byte vectors of the cache
   auto misaligned = [](const void* ptr, uintptr_t a) { return (reinterpret_cast<uintptr_t>(ptr) & (a - 1)) != 0; };
-  if (misaligned(key, 8) || misaligned(value, 8) || key_row_stride % 4 != 0 || value_row_stride % 4 != 0 ||
-      misaligned(k_cache, 4) || misaligned(v_cache, 4) || misaligned(k_scale, 4) || misaligned(v_scale, 4) ||
+  if (misaligned(key, 16) || misaligned(value, 16) || key_row_stride % 8 != 0 || value_row_stride % 8 != 0 ||
+      misaligned(k_cache, 8) || misaligned(v_cache, 8) || misaligned(k_scale, 4) || misaligned(v_scale, 4) ||
       misaligned(slot_mapping, 4))
     return NVA_ERR_ALIGNMENT;
   const int sms = nva::sm_count();
@@ -277,8 +316,9 @@ extern "C" NVA_API int nva_store_kvcache_fp8(const void* key, int64_t key_row_st
   p.kv_heads = num_kv_heads;
   p.lg_block = __builtin_ctz(static_cast<unsigned>(scale_block));
   p.page_blocks = block_size / scale_block;
-  // tokens per CTA: about four CTAs per SM over the call, and a winner table of at most 32 KB
-  const int64_t want = (static_cast<int64_t>(num_tokens) + 4 * sms - 1) / (4 * sms);
+  // tokens per CTA: about two CTAs per SM over the call (8192 tokens: 28, 21 us; one or three per SM 27 and 29 us), and
+  // a winner table of at most 32 KB
+  const int64_t want = (static_cast<int64_t>(num_tokens) + 2 * sms - 1) / (2 * sms);
   const int most = std::min(nva::kMaxChunk, 32768 / 4 / scale_block);
   p.chunk = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(want, most)));
   const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(num_tokens) + p.chunk - 1) / p.chunk);

@@ -380,6 +380,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   auto linear_bin = [&](float l) {             // rises as the logit falls; bins of T / 32, the last takes the rest
     return min(kBins - 1, __float2int_rz((top - l) * bin_scale));
   };
+  uint32_t kept_tokens = 0x7FFFFFFFu;          // an upper bound on the tokens kept
   // Sets the threshold to the logit at which the running count from the top reaches `k`, or the running weight `share`
   // of the whole, with the number of its equals that still belong; leaves it where everything stays.
   auto select = [&](auto by_weight, uint32_t k, double share) {
@@ -445,56 +446,61 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       cluster.sync();
     };
     clear();
-    uint32_t last = 0;
-    for (int w = tid; w < words; w += kThreads)
-      R::each(data[w], [&](float l, int) {
-        if (!(l > (kMass ? fmaxf(floor, weight.low) : floor))) return;
-        const int b = linear_bin(l);
-        if constexpr (kMass) {
-          add_mass(b, weight.bits(l) - Weight::kZero);
-        } else if (b < kBins - 1) {
-          atomicAdd(&hist[0][b], 1u);
-        } else {
-          ++last;   // (most of a vocabulary at a low temperature: not through one counter)
-        }
-      });
-    if constexpr (kMass) {
-      if (rank == 0 && tid == 0 && w_floor != 0) add_mass(linear_bin(floor), w_floor);
-    } else {
-      last = __reduce_add_sync(kAll, last);
-      if (lane == 0) scan_c[warp] = last;
-      __syncthreads();
-      if (tid == 0) {
-        for (int w = 1; w < kWarps; ++w) last += scan_c[w];
-        ctrl.last = last;
-      }
-    }
-    cluster.sync();
-    cross(0, true);
-    if (ctrl.bin == kNone) return;
-    // the crossing bin's keys: from the least with linear_bin <= bin to the last before linear_bin < bin, by 32-way
-    // searches
     uint32_t lo = R::key(floor), hi = R::key(top);   // (the threshold itself may be no bf16 number: a bound)
-    {
-      auto search = [&](auto pred, uint32_t a, uint32_t b) {   // least key in [a, b] with pred, which holds at b
-        while (a < b) {
-          const uint32_t step = (b - a) / 32 + 1;
-          const u64 far = a + static_cast<u64>(step) * lane;
-          const uint32_t x = far < b ? static_cast<uint32_t>(far) : b;
-          const uint32_t yes = __ballot_sync(kAll, x == b || pred(R::value(x)));
-          const int f = yes != 0 ? __ffs(yes) - 1 : 32;   // points below f: no, point f: yes
-          const uint32_t below = __shfl_sync(kAll, x, f > 0 ? f - 1 : 0);
-          const uint32_t at = __shfl_sync(kAll, x, f < 32 ? f : 0);
-          if (f > 0) a = below + 1;
-          b = f == 0 ? a : f < 32 ? at : b;
+    u64 before = 0;
+    // weights of no more tokens than a CTA has threads (what a top-k left): no need of bins
+    const bool direct = kMass && lo < hi && kept_tokens + 2 <= kThreads;
+    if (!direct) {
+      uint32_t last = 0;
+      for (int w = tid; w < words; w += kThreads)
+        R::each(data[w], [&](float l, int) {
+          if (!(l > (kMass ? fmaxf(floor, weight.low) : floor))) return;
+          const int b = linear_bin(l);
+          if constexpr (kMass) {
+            add_mass(b, weight.bits(l) - Weight::kZero);
+          } else if (b < kBins - 1) {
+            atomicAdd(&hist[0][b], 1u);
+          } else {
+            ++last;   // (most of a vocabulary at a low temperature: not through one counter)
+          }
+        });
+      if constexpr (kMass) {
+        if (rank == 0 && tid == 0 && w_floor != 0) add_mass(linear_bin(floor), w_floor);
+      } else {
+        last = __reduce_add_sync(kAll, last);
+        if (lane == 0) scan_c[warp] = last;
+        __syncthreads();
+        if (tid == 0) {
+          for (int w = 1; w < kWarps; ++w) last += scan_c[w];
+          ctrl.last = last;
         }
-        return b;
-      };
-      const int ib = static_cast<int>(ctrl.bin);
-      lo = search([&](float l) { return linear_bin(l) <= ib; }, lo, hi);
-      if (ib > 0) hi = max(lo, search([&](float l) { return linear_bin(l) < ib; }, lo, hi) - 1);
+      }
+      cluster.sync();
+      cross(0, true);
+      if (ctrl.bin == kNone) return;
+      // the crossing bin's keys: from the least with linear_bin <= bin to the last before linear_bin < bin, by 32-way
+      // searches
+      {
+        auto search = [&](auto pred, uint32_t a, uint32_t b) {   // least key in [a, b] with pred, which holds at b
+          while (a < b) {
+            const uint32_t step = (b - a) / 32 + 1;
+            const u64 far = a + static_cast<u64>(step) * lane;
+            const uint32_t x = far < b ? static_cast<uint32_t>(far) : b;
+            const uint32_t yes = __ballot_sync(kAll, x == b || pred(R::value(x)));
+            const int f = yes != 0 ? __ffs(yes) - 1 : 32;   // points below f: no, point f: yes
+            const uint32_t below = __shfl_sync(kAll, x, f > 0 ? f - 1 : 0);
+            const uint32_t at = __shfl_sync(kAll, x, f < 32 ? f : 0);
+            if (f > 0) a = below + 1;
+            b = f == 0 ? a : f < 32 ? at : b;
+          }
+          return b;
+        };
+        const int ib = static_cast<int>(ctrl.bin);
+        lo = search([&](float l) { return linear_bin(l) <= ib; }, lo, hi);
+        if (ib > 0) hi = max(lo, search([&](float l) { return linear_bin(l) < ib; }, lo, hi) - 1);
+      }
+      before = ctrl.before;
     }
-    u64 before = ctrl.before;
     if (lo < hi) {
       // its tokens, kept aside when they are few: the levels below read those instead of the row
       const float flo = R::value(lo), fhi = R::value(hi);
@@ -519,12 +525,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           u64* masses = reinterpret_cast<u64*>(&hist[1][0]);
           uint32_t first = 0, key = 0;
           u64 v = 0;
-          for (int r = 0; r < ranks; ++r) {   // the CTA whose list holds this thread's token
+          int from = -1, place = 0;           // the CTA whose list holds this thread's token, and where
+          for (int r = 0; r < ranks; ++r) {
             const uint32_t c = __shfl_sync(kAll, mine, r);
-            if (static_cast<uint32_t>(tid) >= first && static_cast<uint32_t>(tid) < first + c)
-              key = cluster.map_shared_rank(&list[0], r)[tid - first];
+            if (static_cast<uint32_t>(tid) >= first && static_cast<uint32_t>(tid) < first + c) {
+              from = r;
+              place = tid - static_cast<int>(first);
+            }
             first += c;
           }
+          if (from >= 0) key = cluster.map_shared_rank(&list[0], from)[place];
           if (key != 0) v = kMass ? weight(R::value(key)) : 1ull;
           if (kMass && static_cast<uint32_t>(tid) == all && w_floor != 0 && R::key(floor) >= lo && R::key(floor) <= hi) {
             key = R::key(floor);
@@ -533,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           keys[tid] = key;
           if constexpr (kMass) masses[tid] = v;
           __syncthreads();
-          u64 above = before, same = 0;
+          u64 above = before, same = 0, sum = 0;
           const int count = static_cast<int>(all) + (kMass ? 1 : 0);
           if (v != 0)
             for (int i = 0; i < count; ++i) {
@@ -541,13 +551,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
               const u64 x = kMass ? masses[i] : 1ull;
               above += k > key ? x : 0ull;
               same += k == key ? x : 0ull;
+              sum += x;
             }
-          const double target = ctrl.target;
+          const double target = direct ? fmax(share * static_cast<double>(sum), 1.0) : ctrl.target;
           if (v != 0 && static_cast<double>(above) < target && static_cast<double>(above + same) >= target)
             for (int r = 0; r < ranks; ++r) {   // (equal tokens say the same)
               Control* c = cluster.map_shared_rank(&ctrl, r);
               c->bin = key;
               c->before = above;
+              c->target = target;
             }
         }
         cluster.sync();
@@ -598,6 +610,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       cut_ties = min(limit, static_cast<uint32_t>(fmin(want, 4.0e9)));
     } else {
       cut_ties = k - static_cast<uint32_t>(before);
+      kept_tokens = k;
     }
     __syncthreads();   // (ctrl is read)
   };
@@ -608,10 +621,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   }
   if (p.top_p != nullptr) {
     const double tp = __ldg(p.top_p + set);
-    if (tp < 1.0) {
-      cluster.sync();   // (rank 0 has read every CTA's bins)
-      select(std::true_type{}, 0, fmax(tp, 0.0));
-    }
+    if (tp < 1.0) select(std::true_type{}, 0, fmax(tp, 0.0));
   }
 
   // ---------------------------------------------------------------- the draw
