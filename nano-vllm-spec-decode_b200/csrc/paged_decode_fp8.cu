@@ -80,8 +80,7 @@ struct Cfg8 {
   static constexpr int kM = kRed + 4 * NP * 4;                      // [NP] running maxima
   static constexpr int kNegM = kM + NP * 4;                         // [NP] kBase - maximum
   static constexpr int kAlpha = kNegM + NP * 4;                     // [NP]
-  static constexpr int kRowOut = kAlpha + NP * 4;                   // [NP] int64
-  static constexpr int kRowInv = kRowOut + NP * 8;                  // [NP]
+  static constexpr int kRowInv = kAlpha + NP * 4;                   // [NP] 1 / sum
   static constexpr int kStart = (kRowInv + NP * 4 + 15) / 16 * 16;  // Start
   static constexpr int kPending = kStart + 64;                      // [2] Pending
   static constexpr int kScan = kPending + 2 * 24;                   // [8] int64
@@ -251,6 +250,26 @@ struct Pending {
   int64_t out_base;
 };
 
+// One row of q (four bf16 values per lane) as its two e4m3 parts in the swizzled operand at qs, and its scale.
+__device__ __forceinline__ void put_q_row(uint2 x, uint8_t* qs, int half_bytes, float* scales, int r, int lane) {
+  uint32_t mx = max(max(x.x & 0x7FFFu, (x.x >> 16) & 0x7FFFu), max(x.y & 0x7FFFu, (x.y >> 16) & 0x7FFFu));
+  mx = __reduce_max_sync(kFull, mx);
+  // the row's largest value to [2^7, 2^8): times 2^(134 - E); NaN or infinity anywhere makes the row NaN
+  const int E = max(static_cast<int>(mx >> 7), 8);
+  const float f = __uint_as_float(static_cast<uint32_t>(261 - min(E, 254)) << 23);
+  const float back = E == 255 ? __uint_as_float(0x7FC00000u) : __uint_as_float(static_cast<uint32_t>(E - 7) << 23);
+  const float2 a01 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x.x));
+  const float2 a23 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x.y));
+  const float v0 = a01.x * f, v1 = a01.y * f, v2 = a23.x * f, v3 = a23.y * f;
+  const uint32_t h01 = pack_e4m3(v0, v1), h23 = pack_e4m3(v2, v3);
+  const float2 u01 = unpack_e4m3(h01), u23 = unpack_e4m3(h23);
+  const uint32_t l01 = pack_e4m3(v0 - u01.x, v1 - u01.y), l23 = pack_e4m3(v2 - u23.x, v3 - u23.y);
+  uint8_t* at = qs + sw128_offset(r, lane >> 2) + (lane & 3) * 4;
+  *reinterpret_cast<uint32_t*>(at) = h01 | (h23 << 16);
+  *reinterpret_cast<uint32_t*>(at + half_bytes) = l01 | (l23 << 16);
+  if (lane == 0) scales[r] = back;
+}
+
 // Softmax rows of a segment: NR, or 8 for the short runs of a batch of mixed lengths.  (Each further variant inside one
 // kernel costs the others registers.)
 template <int NR, bool kMixed, class F>
@@ -298,7 +317,6 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
   float* m_s = reinterpret_cast<float*>(smem + C::kM);
   float* negm_s = reinterpret_cast<float*>(smem + C::kNegM);
   float* alpha_s = reinterpret_cast<float*>(smem + C::kAlpha);
-  int64_t* row_out = reinterpret_cast<int64_t*>(smem + C::kRowOut);
   float* row_inv = reinterpret_cast<float*>(smem + C::kRowInv);
   Start* start = reinterpret_cast<Start*>(smem + C::kStart);
   Pending* pending = reinterpret_cast<Pending*>(smem + C::kPending);
@@ -328,7 +346,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       mbar_init(&bars[B_SEMPTY + s], 128);
       mbar_init(&bars[B_PFULL + s], 128);
       mbar_init(&bars[B_OFULL + s], 1);
-      mbar_init(&bars[B_QFULL + s], 32);
+      mbar_init(&bars[B_QFULL + s], 1);
       mbar_init(&bars[B_QEMPTY + s], 1);
     }
     for (int i = 0; i < kInfoRing; ++i) mbar_init(&bars[B_INFO + i], 1);
@@ -588,7 +606,9 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     }
   } else {
     // ------------------------------------------------------------ Q loader: bf16 rows -> two e4m3 parts + row scale
-    for (int qi = 0; w.valid; ++qi) {
+    // (the softmax warps, idle until the first scores, put the first segment's rows)
+    w.next_segment(p);
+    for (int qi = 1; w.valid; ++qi) {
       const int qb = qi % C::kQBuf;
       if (!mbar_wait_warp(&bars[B_QEMPTY + qb], ((qi / C::kQBuf) & 1) ^ 1, abort)) break;
       const int R = w.np * G;
@@ -623,28 +643,12 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
 #pragma unroll
         for (int v = 0; v < kBatch; ++v) {
           const int r = r0 + v;
-          uint32_t mx = max(max(x[v].x & 0x7FFFu, (x[v].x >> 16) & 0x7FFFu),
-                            max(x[v].y & 0x7FFFu, (x[v].y >> 16) & 0x7FFFu));
-          mx = __reduce_max_sync(kFull, mx);
-          // the row's largest value to [2^7, 2^8): times 2^(134 - E); NaN or infinity anywhere makes the row NaN
-          const int E = max(static_cast<int>(mx >> 7), 8);
-          const float f = __uint_as_float(static_cast<uint32_t>(261 - min(E, 254)) << 23);
-          const float back = E == 255 ? __uint_as_float(0x7FC00000u) : __uint_as_float(static_cast<uint32_t>(E - 7) << 23);
-          const float2 a01 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[v].x));
-          const float2 a23 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[v].y));
-          const float v0 = a01.x * f, v1 = a01.y * f, v2 = a23.x * f, v3 = a23.y * f;
-          const uint32_t h01 = pack_e4m3(v0, v1), h23 = pack_e4m3(v2, v3);
-          const float2 u01 = unpack_e4m3(h01), u23 = unpack_e4m3(h23);
-          const uint32_t l01 = pack_e4m3(v0 - u01.x, v1 - u01.y), l23 = pack_e4m3(v2 - u23.x, v3 - u23.y);
-          uint8_t* at = qs + sw128_offset(r, lane >> 2) + (lane & 3) * 4;
-          *reinterpret_cast<uint32_t*>(at) = h01 | (h23 << 16);
-          *reinterpret_cast<uint32_t*>(at + C::kQHalf) = l01 | (l23 << 16);
-          if (lane == 0) sc[r] = back;
+          put_q_row(x[v], qs, C::kQHalf, sc, r, lane);
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
-      mbar_arrive(&bars[B_QFULL + qb]);
+      if (lane == 0) mbar_arrive(&bars[B_QFULL + qb]);
       w.next_segment(p);
     }
   }
@@ -665,9 +669,12 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     // A piece of a cut segment is done (its rows written): take a ticket.  The CTA that brings
     // it to the number of pieces puts the counter back to zero and merges them all; a CTA has at most two cut segments,
     // so it notes them and merges after its last tile, out of the loop's registers.
-    auto arrive_piece = [&](int c0, int c1, int R, int64_t out_base) {
+    auto arrive_piece = [&](int p_first, int p_last, int R, int64_t out_base) {
       named_bar_sync(bar_id, 128);
       if (ct == 0) {
+        // the CTAs of the segment's first and last tile
+        const int c0 = member * teams + static_cast<int>((start->x0 + p_first) / start->per);
+        const int c1 = member * teams + static_cast<int>((start->x0 + p_last) / start->per);
         int32_t* ticket = p.counters + kTicketStride * c0;
         __threadfence();   // release: the group's partial rows before the ticket
         if (atomicAdd(ticket, 1) == c1 - c0) {
@@ -691,6 +698,26 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       }
     };
 
+    {
+      // the first segment's q, the four warps' rows apart: the Q loader alone took 3 us longer on 20 rows
+      const int rows = w.np * G;
+      const __nv_bfloat16* base = p.q + static_cast<int64_t>(w.q0 + w.piece * p.max_n) * p.q_row_stride +
+                                  static_cast<int64_t>(w.g * p.head_set + member) * G * kHeadDim + lane * 4;
+      constexpr int kOwn = NR / 4;
+      uint2 x[kOwn];
+#pragma unroll
+      for (int v = 0; v < kOwn; ++v) {
+        const int r = wq + 4 * v, i = r / G;
+        x[v] = make_uint2(0u, 0u);
+        if (r < rows) x[v] = __ldg(reinterpret_cast<const uint2*>(base + i * p.q_row_stride + (r - i * G) * kHeadDim));
+      }
+#pragma unroll
+      for (int v = 0; v < kOwn; ++v)
+        if (wq + 4 * v < rows) put_q_row(x[v], smem + C::kQ, C::kQHalf, qscale, wq + 4 * v, lane);
+      fence_proxy_async_smem();
+      named_bar_sync(bar_id, 128);
+      if (ct == 0) mbar_arrive(&bars[B_QFULL]);
+    }
     alive = mbar_wait_warp(&bars[B_INFO], 0, abort);
     if (alive) load_scales(info[0], info[1]);
     int jj = 0;   // tile of this CTA
@@ -881,48 +908,54 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       const int seg_g = info[3 * e].w;
       const int R = ib.x * G;
       // positions of the segment's first and last tile relative to this CTA's share: a segment inside it is finished
-      // here, one that is cut leaves a piece (the CTAs of its first and last tile name the others)
+      // here, one that is cut leaves a piece
       const int span = static_cast<int>(start->x1 - start->x0);
       const int p_first = ic.y + ic.z * kSegCost, p_last = p_first + ic.z * (ib.w - 1);
       const bool complete = p_first >= 0 && p_last < span;
-      int c0 = vcta, c1 = vcta;
-      if (!complete) {
-        c0 = member * teams + static_cast<int>((start->x0 + p_first) / start->per);
-        c1 = member * teams + static_cast<int>((start->x0 + p_last) / start->per);
-      }
+      const int slot = 2 * vcta + (p_first < 0 ? 0 : 1);   // (of a piece)
       const int64_t out_base = ib.z * p.out_row_stride + static_cast<int64_t>(seg_g) * G * kHeadDim;
       if (ct < R) {
         const float lt = red[ct] + red[NP + ct] + red[2 * NP + ct] + red[3 * NP + ct];
         row_inv[ct] = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);   // a NaN sum stays NaN
-        if (complete) {
-          const int i = ct / G, h = ct - i * G;
-          row_out[ct] = out_base + i * p.out_row_stride + h * kHeadDim;
-        } else {
-          const int slot = 2 * vcta + (p_first < 0 ? 0 : 1);
-          row_out[ct] = (static_cast<int64_t>(slot) * NP + ct) * kHeadDim;
-          p.part_lse[slot * NP + ct] = lt == 0.f ? kNegInf : m_s[ct] + __log2f(lt);
-        }
+        if (!complete) p.part_lse[slot * NP + ct] = lt == 0.f ? kNegInf : m_s[ct] + __log2f(lt);
       }
       named_bar_sync(bar_id, 128);
       tc_fence_after();
+      // the accumulated O, eight rows at a time; lane = dim
+      __nv_bfloat16* o = p.out + out_base + ct;
+      float* part = p.part_o + static_cast<int64_t>(slot) * NP * kHeadDim + ct;
+      int h = 0;
+#pragma unroll 1
       for (int c = 0; c < R; c += 8) {
         float ot[8];
         tmem_ld8(t_o + c, ot);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = c + i;
-          if (r < R) {
-            const float val = ot[i] * row_inv[r];
-            if (complete) {
-              p.out[row_out[r] + ct] = __float2bfloat16_rn(val);
+        for (int i = 0; i < 8; i += 4) {
+          const float4 inv = *reinterpret_cast<const float4*>(row_inv + c + i);
+          ot[i] *= inv.x;
+          ot[i + 1] *= inv.y;
+          ot[i + 2] *= inv.z;
+          ot[i + 3] *= inv.w;
+        }
+        if (complete) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (c + i < R) *o = __float2bfloat16_rn(ot[i]);
+            if (++h == G) {
+              h = 0;
+              o += p.out_row_stride - (G - 1) * kHeadDim;
             } else {
-              p.part_o[row_out[r] + ct] = val;
+              o += kHeadDim;
             }
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c + i < R) part[(c + i) * kHeadDim] = ot[i];
         }
       }
       tc_fence_before();
-      if (!complete) arrive_piece(c0, c1, R, out_base);
+      if (!complete) arrive_piece(p_first, p_last, R, out_base);
       done = ic.x & 4;
       ++jj;
     }
@@ -936,49 +969,84 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       // the piece of CTA c lies in its second slot where the segment begins (c0), in its first slot behind that
       const int pieces = d.c1 - d.c0 + 1;
       float* table = reinterpret_cast<float*>(smem + C::kK);   // [rows][pieces] weights; the rings are idle
-      // (a warp per row) weights 2^(lse - max) / sum of pieces that saw a key; partials come from other CTAs: past L1
+      auto piece_row = [&](int c, int r) { return static_cast<int64_t>(2 * (d.c0 + c) + (c == 0 ? 1 : 0)) * NP + r; };
+      // weights 2^(lse - max) / sum of pieces that saw a key; partials come from other CTAs: past L1
+      if (pieces <= 16) {   // (a thread per row)
+        if (ct < d.rows) {
+          float mx = kNegInf, den = 0.f;
+#pragma unroll 8
+          for (int c = 0; c < pieces; ++c) {
+            const float v = __ldcg(p.part_lse + piece_row(c, ct));
+            table[ct * pieces + c] = v;
+            mx = fmaxf(mx, v);
+          }
 #pragma unroll 1
-      for (int r = wq; r < d.rows; r += 4) {
-        float mx = kNegInf, den = 0.f;
+          for (int c = 0; c < pieces; ++c) {
+            const float v = table[ct * pieces + c];
+            const float e = v == kNegInf ? 0.f : fast_exp2(v - mx);
+            table[ct * pieces + c] = e;
+            den += e;
+          }
+          const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll 1
-        for (int c = lane; c < pieces; c += 32) {
-          const float v = __ldcg(p.part_lse + (2 * (d.c0 + c) + (c == 0 ? 1 : 0)) * NP + r);
-          table[r * pieces + c] = v;
-          mx = fmaxf(mx, v);
+          for (int c = 0; c < pieces; ++c) table[ct * pieces + c] *= inv;
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, o));
+      } else {              // (a warp per row)
 #pragma unroll 1
-        for (int c = lane; c < pieces; c += 32) {
-          const float v = table[r * pieces + c];
-          const float e = v == kNegInf ? 0.f : fast_exp2(v - mx);
-          table[r * pieces + c] = e;
-          den += e;
+        for (int r = wq; r < d.rows; r += 4) {
+          float mx = kNegInf, den = 0.f;
+#pragma unroll 1
+          for (int c = lane; c < pieces; c += 32) {
+            const float v = __ldcg(p.part_lse + piece_row(c, r));
+            table[r * pieces + c] = v;
+            mx = fmaxf(mx, v);
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, o));
+#pragma unroll 1
+          for (int c = lane; c < pieces; c += 32) {
+            const float v = table[r * pieces + c];
+            const float e = v == kNegInf ? 0.f : fast_exp2(v - mx);
+            table[r * pieces + c] = e;
+            den += e;
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(kFull, den, o);
+          const float inv = den == 0.f ? 0.f : 1.f / den;
+#pragma unroll 1
+          for (int c = lane; c < pieces; c += 32) table[r * pieces + c] *= inv;
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(kFull, den, o);
-        const float inv = den == 0.f ? 0.f : 1.f / den;
-#pragma unroll 1
-        for (int c = lane; c < pieces; c += 32) table[r * pieces + c] *= inv;
       }
       named_bar_sync(bar_id, 128);
+      // four rows of four dims a thread, their loads together
 #pragma unroll 1
-      for (int idx = ct; idx < d.rows * 32; idx += 128) {   // (row, 4 dims)
-        const int r = idx >> 5, l4 = idx & 31;
-        const float4* src = reinterpret_cast<const float4*>(p.part_o) + l4;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+      for (int r0 = wq; r0 < d.rows; r0 += 16) {
+        float4 acc[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
         for (int c = 0; c < pieces; ++c) {
-          const float4 v = __ldcg(src + static_cast<int64_t>((2 * (d.c0 + c) + (c == 0 ? 1 : 0)) * NP + r) * 32);
-          const float wgt = table[r * pieces + c];
-          acc.x = fmaf(wgt, v.x, acc.x);
-          acc.y = fmaf(wgt, v.y, acc.y);
-          acc.z = fmaf(wgt, v.z, acc.z);
-          acc.w = fmaf(wgt, v.w, acc.w);
+          const float4* src = reinterpret_cast<const float4*>(p.part_o) + piece_row(c, r0) * 32 + lane;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (r0 + 4 * k < d.rows) {
+              const float4 v = __ldcg(src + 4 * k * 32);
+              const float wgt = table[(r0 + 4 * k) * pieces + c];
+              acc[k].x = fmaf(wgt, v.x, acc[k].x);
+              acc[k].y = fmaf(wgt, v.y, acc[k].y);
+              acc[k].z = fmaf(wgt, v.z, acc[k].z);
+              acc[k].w = fmaf(wgt, v.w, acc[k].w);
+            }
         }
-        const int q = r / G, h = r - q * G;
-        *reinterpret_cast<uint2*>(p.out + d.out_base + q * p.out_row_stride + h * kHeadDim + l4 * 4) =
-            make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = r0 + 4 * k;
+          if (r < d.rows) {
+            const int q = r / G, h = r - q * G;
+            *reinterpret_cast<uint2*>(p.out + d.out_base + q * p.out_row_stride + h * kHeadDim + lane * 4) =
+                make_uint2(pack_bf16x2(acc[k].x, acc[k].y), pack_bf16x2(acc[k].z, acc[k].w));
+          }
+        }
       }
       named_bar_sync(bar_id, 128);
     }
