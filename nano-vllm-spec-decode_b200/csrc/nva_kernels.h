@@ -99,9 +99,9 @@ struct Fp8DecodeParams {
   int32_t page_blocks;  // scale blocks per cache block
   int32_t lg_block;     // log2 of the tokens per scale block
   float scale_log2;
-  float* part_o;        // [2 * grid, NP, 128], [2 * grid, NP]: as in DecodeParams
+  float* part_o;        // [slots * grid, NP, 128], [slots * grid, NP] as in DecodeParams; two slots a CTA and phase
   float* part_lse;
-  int32_t* counters;    // [grid][4] merge tickets: zero on entry and on exit
+  int32_t* counters;    // [grid][4] merge tickets (one a phase): zero on entry and on exit
 };
 
 // Varlen prefill kernel (long query runs) — q rows tiled by 128 per (sequence, q head).

@@ -82,9 +82,9 @@ struct Cfg8 {
   static constexpr int kAlpha = kNegM + NP * 4;                     // [NP]
   static constexpr int kRowInv = kAlpha + NP * 4;                   // [NP] 1 / sum
   static constexpr int kStart = (kRowInv + NP * 4 + 15) / 16 * 16;  // Start
-  static constexpr int kPending = kStart + 64;                      // [2] Pending
-  static constexpr int kScan = kPending + 2 * 24;                   // [8] int64
-  static constexpr int kTmem = kScan + 8 * 8;
+  static constexpr int kPending = kStart + 2 * 64;                  // [4] Pending
+  static constexpr int kScan = kPending + 4 * 24;                   // [2][8] int64
+  static constexpr int kTmem = kScan + 16 * 8;
   static constexpr int kAbort = kTmem + 4;
   static constexpr int kEnd = kAbort + 4;
   static constexpr int kBytes = kEnd + 1024;                        // + slack for 1024-byte alignment
@@ -149,44 +149,57 @@ __device__ __forceinline__ int piece_keys(int n, int L, int i, int max_n) {
 }
 __device__ __forceinline__ int tiles_of(int keys) { return (keys + 127) >> 7; }
 
-// Weight of a piece of np queries in the work split.  In batches of mixed lengths the tiles of a long run's pieces and
-// their start and end take about twice the time of a decode row's (40 rows against 8; 3.0 against 1.55 us a tile).
+// The kernel for batches of mixed lengths (kMixed) splits its work twice: phase 0 are the pieces of more than 8 packed
+// rows, which the softmax bounds, phase 1 the short ones, which HBM bounds.  Every CTA has its share of both, half of the
+// CTAs in the other order, so that the two kinds run beside each other on an SM and neither's cost has to be weighed
+// against the other's.
 template <bool kMixed>
-__device__ __forceinline__ int piece_weight(const Fp8DecodeParams& p, int np) {
-  return kMixed && np * p.group > 8 ? 2 : 1;
-}
+constexpr int kPhases = kMixed ? 2 : 1;
 
-// Cost of a sequence per head set.
-template <bool kMixed>
-__device__ __forceinline__ long long seq_cost(const Fp8DecodeParams& p, int n, int L) {
-  long long c = 0;
-  for (int i = 0; i * p.max_n < n; ++i) {
-    const int nt = tiles_of(piece_keys(n, L, i, p.max_n));
-    if (nt > 0) c += piece_weight<kMixed>(p, min(p.max_n, n - i * p.max_n)) * (nt + kSegCost);
+// Calls f(first piece, count, tiles) for the runs of pieces of equal tile count of a sequence that belong to the phase, in
+// order, until it returns true.  (By tiles, not by pieces: a prompt of 16,384 has 2048 pieces but 128 tile counts.)
+template <bool kMixed, class F>
+__device__ __forceinline__ void piece_runs(const Fp8DecodeParams& p, int n, int L, int phase, F&& f) {
+  const int m = p.max_n, full = n / m, before = L - n;   // piece i < full ends at key before + (i + 1) m
+  if (!kMixed || phase == 0) {                           // (whole pieces have more than 8 rows in a mixed batch)
+    int i = before + m >= 1 ? 1 : -before / m + 1;       // (1-based) the first with a key
+#pragma unroll 1
+    while (i <= full) {
+      const int t = (before + m * i + 127) >> 7;
+      const int last = min(full, (128 * t - before) / m);
+      if (f(i - 1, last - i + 1, t)) return;
+      i = last + 1;
+    }
   }
-  return c;
+  const int rest = n - full * m;
+  if (rest > 0 && L > 0 && (!kMixed || (rest * p.group > 8) == (phase == 0))) f(full, 1, tiles_of(L));
 }
 
-// Where a CTA starts.
+// Where a CTA starts in a phase.
 struct Start {
   long long segpos;   // cost position of the first segment
   long long x0, x1;   // the CTA's share of positions
   long long per;
   int b, piece, g, j; // (g: the head set)
-  int any;
+  int any, unused[3];
 };
-static_assert(sizeof(Start) <= 64, "Start");
+static_assert(sizeof(Start) == 64, "Start");
 
-// The tiles of one CTA in order.  Every lane of the warp holds the same state.  Tile j of a segment at segpos of weight
-// u sits at position segpos + u * (kSegCost + j); a CTA owns the tiles whose positions are in [x0, x1).  Positions are
-// kept relative to x0.
+// The tiles of one CTA in order.  Every lane of the warp holds the same state.  Tile j of a segment at segpos sits at
+// position segpos + kSegCost + j of its phase; a CTA owns the tiles whose positions are in [x0, x1).  Positions are kept
+// relative to x0.
 template <bool kMixed>
 struct Walk {
+  const Start* starts;
   int rel, span;      // segpos - x0, x1 - x0
   int b, piece, g, j;
   int n, L, q0;       // the sequence
-  int np, Lp, nt, u;  // the piece: queries, keys its last query sees, tiles, weight
+  int np, Lp, nt;     // the piece: queries, keys its last query sees, tiles
+  int phase;
+  bool more;          // the other phase is still to come
+  bool fresh;         // the first tile of this CTA's share of the phase
   bool valid;
+  int ahead, ahead_n, ahead_L, ahead_q0;   // sequences ahead .. ahead + 31, one per lane
 
   __device__ __forceinline__ void load_seq(const Fp8DecodeParams& p) {
     const Shape8 s = shape_of(p, b);
@@ -198,55 +211,115 @@ struct Walk {
     np = min(p.max_n, n - piece * p.max_n);
     Lp = piece_keys(n, L, piece, p.max_n);
     nt = tiles_of(Lp);
-    u = piece_weight<kMixed>(p, np);
   }
-  __device__ __forceinline__ void begin(const Fp8DecodeParams& p, const Start& s) {
-    rel = static_cast<int>(s.segpos - s.x0);
-    span = static_cast<int>(s.x1 - s.x0);
-    b = s.b;
-    piece = s.piece;
-    g = s.g;
-    j = s.j;
-    load_seq(p);
-    set_piece(p);
-    if (j < nt) {
-      valid = rel + u * (kSegCost + j) < span;
-    } else {   // (the share begins behind the position of the segment's last tile)
-      next_segment(p);
+  // the share of the current phase, or of the other one when it is empty
+  __device__ __forceinline__ void enter(const Fp8DecodeParams& p) {
+    while (true) {
+      const Start& s = starts[phase];
+      valid = s.any != 0;
+      if (valid) {
+        rel = static_cast<int>(s.segpos - s.x0);
+        span = static_cast<int>(s.x1 - s.x0);
+        b = s.b;
+        piece = s.piece;
+        g = s.g;
+        j = s.j;
+        load_seq(p);
+        set_piece(p);
+        valid = rel + kSegCost + j < span;
+      }
+      if (valid || !more) break;
+      more = false;
+      phase ^= 1;
+    }
+    fresh = valid;
+  }
+  __device__ __forceinline__ void begin(const Fp8DecodeParams& p, const Start* s, int first_phase) {
+    starts = s;
+    ahead = -64;
+    phase = kMixed ? first_phase : 0;
+    more = kMixed;
+    enter(p);
+  }
+  // Whether a sequence has a piece with keys in the phase.
+  __device__ __forceinline__ bool has_piece(const Fp8DecodeParams& p, int n_, int L_) const {
+    const int full = n_ / p.max_n, rest = n_ - full * p.max_n;
+    const bool whole = full > 0 && L_ - n_ + full * p.max_n > 0, part = rest > 0 && L_ > 0;
+    if constexpr (!kMixed) return whole || part;
+    return phase == 0 ? whole || (part && rest * p.group > 8) : part && rest * p.group <= 8;
+  }
+  // The next segment of the phase (all lanes of the warp together).
+  __device__ __forceinline__ void advance(const Fp8DecodeParams& p) {
+    rel += nt + kSegCost;
+    j = 0;
+    valid = rel + kSegCost < span;
+    if (!valid || ++g < p.num_kv_heads / p.head_set) return;
+    g = 0;
+    bool belongs;
+    do {
+      ++piece;
+      if (kMixed && phase == 1) piece = max(piece, n / p.max_n);   // (whole pieces are phase 0)
+      if (piece * p.max_n >= n) {
+        // the next sequence that has one: 32 at a time, read once
+        const int lane = threadIdx.x & 31;
+        uint32_t vote = 0;
+        int from = b + 1;
+        while (true) {
+          if (from < ahead || from >= ahead + 32) {
+            ahead = from;
+            ahead_n = ahead_L = ahead_q0 = 0;
+            if (from + lane < p.num_seqs) {
+              const Shape8 s = shape_of(p, from + lane);
+              ahead_n = s.n;
+              ahead_L = s.L;
+              ahead_q0 = s.q0;
+            }
+          }
+          vote = __ballot_sync(kFull, ahead + lane >= from && has_piece(p, ahead_n, ahead_L));
+          if (vote != 0 || ahead + 32 >= p.num_seqs) break;
+          from = ahead + 32;
+        }
+        if (vote == 0) {
+          valid = false;
+          return;
+        }
+        const int src = __ffs(vote) - 1;
+        b = ahead + src;
+        n = __shfl_sync(kFull, ahead_n, src);
+        L = __shfl_sync(kFull, ahead_L, src);
+        q0 = __shfl_sync(kFull, ahead_q0, src);
+        piece = kMixed && phase == 1 ? n / p.max_n : 0;
+      }
+      set_piece(p);
+      belongs = !kMixed || (np * p.group > 8) == (phase == 0);
+    } while (nt == 0 || !belongs);
+  }
+  __device__ __forceinline__ void other_phase(const Fp8DecodeParams& p) {
+    if (kMixed && !valid && more) {
+      more = false;
+      phase ^= 1;
+      enter(p);
     }
   }
   __device__ __forceinline__ void next_segment(const Fp8DecodeParams& p) {
-    rel += u * (nt + kSegCost);
-    j = 0;
-    if (++g == p.num_kv_heads / p.head_set) {
-      g = 0;
-      do {
-        ++piece;
-        while (piece * p.max_n >= n) {
-          piece = 0;
-          if (++b >= p.num_seqs) {
-            valid = false;
-            return;
-          }
-          load_seq(p);
-        }
-        set_piece(p);
-      } while (nt == 0);
-    }
-    valid = rel + u * kSegCost < span;
+    fresh = false;
+    advance(p);
+    other_phase(p);
   }
   __device__ __forceinline__ void next_tile(const Fp8DecodeParams& p) {
+    fresh = false;
     if (++j < nt) {
-      valid = rel + u * (kSegCost + j) < span;
+      valid = rel + kSegCost + j < span;
     } else {
-      next_segment(p);
+      advance(p);
     }
+    other_phase(p);
   }
 };
 
 // A cut segment that this CTA has to merge (c1 < 0: none).
 struct Pending {
-  int c0, c1, rows, unused;
+  int c0, c1, rows, phase;
   int64_t out_base;
 };
 
@@ -318,7 +391,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
   float* negm_s = reinterpret_cast<float*>(smem + C::kNegM);
   float* alpha_s = reinterpret_cast<float*>(smem + C::kAlpha);
   float* row_inv = reinterpret_cast<float*>(smem + C::kRowInv);
-  Start* start = reinterpret_cast<Start*>(smem + C::kStart);
+  Start* start = reinterpret_cast<Start*>(smem + C::kStart);   // [phase], 64 bytes apart
   Pending* pending = reinterpret_cast<Pending*>(smem + C::kPending);
   long long* scan = reinterpret_cast<long long*>(smem + C::kScan);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kTmem);
@@ -352,8 +425,8 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     for (int i = 0; i < kInfoRing; ++i) mbar_init(&bars[B_INFO + i], 1);
     mbar_init(&bars[B_KSTART], 1);
     *abort = 0;
-    start->any = 0;
-    for (int i = 0; i < 2; ++i) pending[i].c1 = -1;
+    for (int i = 0; i < 2; ++i) start[i].any = 0;
+    for (int i = 0; i < 4; ++i) pending[i].c1 = -1;
     fence_barrier_init();
     fence_proxy_async_smem();
     tma_prefetch_desc(&tm_k);
@@ -363,8 +436,8 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
   // Two scans over the sequences' costs: the total (hence each CTA's share), then the sequence that holds this CTA's
   // first position.  Batches of up to kThreads sequences keep the first scan's values in registers.
   {
-    constexpr int T = C::kThreads, W = T / 32;
-    long long total = 0, per = 1, x0 = 0, before = 0, mine = 0, excl = 0, sum = 0;
+    constexpr int T = C::kThreads, W = T / 32, kPh = kPhases<kMixed>;
+    long long total[kPh] = {}, x0[kPh] = {}, per[kPh] = {}, before[kPh] = {}, mine[kPh] = {}, excl[kPh] = {}, sum[kPh] = {};
     int n = 0, L = 0;
     const bool single = p.num_seqs <= T;
 #pragma unroll 1
@@ -373,66 +446,82 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       for (int base = 0; base < p.num_seqs; base += T) {
         if (pass == 0 || !single) {
           n = L = 0;
-          mine = 0;
           if (base + tid < p.num_seqs) {
             const Shape8 s = shape_of(p, base + tid);
             n = s.n;
             L = s.L;
-            mine = sets * seq_cost<kMixed>(p, n, L);
           }
-          long long x = mine;
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(kFull, x, o);
-            if (lane >= o) x += y;
+          for (int ph = 0; ph < kPh; ++ph) {
+            mine[ph] = 0;
+            piece_runs<kMixed>(p, n, L, ph, [&](int, int count, int nt) {
+              mine[ph] += static_cast<long long>(sets) * count * (nt + kSegCost);
+              return false;
+            });
+            long long x = mine[ph];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const long long y = __shfl_up_sync(kFull, x, o);
+              if (lane >= o) x += y;
+            }
+            if (lane == 31) scan[ph * W + warp] = x;
+            excl[ph] = x - mine[ph];
           }
-          if (lane == 31) scan[warp] = x;
           __syncthreads();
-          excl = x - mine;
-          sum = 0;
 #pragma unroll
-          for (int w = 0; w < W; ++w) {
-            const long long v = scan[w];
-            excl += w < warp ? v : 0;
-            sum += v;
+          for (int ph = 0; ph < kPh; ++ph) {
+            sum[ph] = 0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+              const long long v = scan[ph * W + w];
+              excl[ph] += w < warp ? v : 0;
+              sum[ph] += v;
+            }
           }
           __syncthreads();
         }
-        if (pass == 0) {
-          total += sum;
-          continue;
-        }
-        // the thread whose sequence holds position x0
-        const long long lo = before + excl;
-        before += sum;
-        if (mine > 0 && x0 >= lo && x0 < lo + mine) {
-          long long rem = x0 - lo;
-          int i = 0, seg = 0, u = 1;
-#pragma unroll 1
-          for (;; ++i) {
-            const int nt = tiles_of(piece_keys(n, L, i, p.max_n));
-            u = piece_weight<kMixed>(p, min(p.max_n, n - i * p.max_n));
-            seg = nt > 0 ? u * (nt + kSegCost) : 0;
-            if (rem < static_cast<long long>(sets) * seg) break;
-            rem -= static_cast<long long>(sets) * seg;
+#pragma unroll
+        for (int ph = 0; ph < kPh; ++ph) {
+          if (pass == 0) {
+            total[ph] += sum[ph];
+            continue;
           }
-          const int r = static_cast<int>(rem);   // (within one piece: < 2^31)
-          const int g = r / seg, o = r - g * seg;
-          start->segpos = x0 - o;
-          start->b = base + tid;
-          start->piece = i;
-          start->g = g;
-          start->j = max(0, (o + u - 1) / u - kSegCost);
-          start->any = 1;
+          // the thread whose sequence holds position x0
+          const long long lo = before[ph] + excl[ph];
+          before[ph] += sum[ph];
+          if (mine[ph] > 0 && x0[ph] >= lo && x0[ph] < lo + mine[ph]) {
+            long long rem = x0[ph] - lo;
+            piece_runs<kMixed>(p, n, L, ph, [&](int first, int count, int nt) {
+              const int seg = nt + kSegCost;
+              const long long run = static_cast<long long>(sets) * count * seg;
+              if (rem >= run) {
+                rem -= run;
+                return false;
+              }
+              const int i = static_cast<int>(rem / (sets * seg));
+              const int r = static_cast<int>(rem) - i * sets * seg, g = r / seg, o = r - g * seg;
+              Start* st = start + ph;
+              st->segpos = x0[ph] - o;
+              st->b = base + tid;
+              st->piece = first + i;
+              st->g = g;
+              st->j = max(0, o - kSegCost);
+              st->any = 1;
+              return true;
+            });
+          }
         }
       }
       if (pass == 0) {
-        per = total > 0 ? (total + teams - 1) / teams : 1;
-        x0 = per * team;
-        if (tid == 0) {
-          start->x0 = x0;
-          start->x1 = x0 + per;
-          start->per = per;
+#pragma unroll
+        for (int ph = 0; ph < kPh; ++ph) {
+          per[ph] = total[ph] > 0 ? (total[ph] + teams - 1) / teams : 1;
+          x0[ph] = per[ph] * team;
+          if (tid == 0) {
+            start[ph].x0 = x0[ph];
+            start[ph].x1 = min(x0[ph] + per[ph], total[ph]);
+            start[ph].per = per[ph];
+          }
         }
       }
     }
@@ -450,8 +539,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             make_uint4(0u, 0u, 0u, 0u);
   }
   Walk<kMixed> w;
-  w.valid = start->any != 0;
-  if (w.valid) w.begin(p, *start);
+  w.begin(p, start, blockIdx.x >= gridDim.x / 2 ? 1 : 0);
   if (!w.valid) return;   // nothing for this CTA: no TMEM, no pipeline
   if (warp < 4) {
   if (warp == 0 || warp == 3) {
@@ -464,14 +552,13 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     uint64_t* empty = bars + (is_k ? B_KEMPTY : B_VEMPTY);
     const int stages = is_k ? C::kKStages : C::kVStages;
     bool stop = !is_k && !mbar_wait_warp(&bars[B_KSTART], 0, abort);
-    bool first_of_cta = true;
     for (int jj = 0; w.valid && !stop;) {
       // descriptors of the next tiles, one per lane (their block-table reads overlap); a short first round, so that
       // the first copies start early
       const int round = jj == 0 ? 4 : 32;
-      int g = 0, j = 0, flags = 0, np = 0, Lp = 0, qrow = 0, nt = 0, b = 0, rel = 0, u = 0, cnt = 0;
+      int g = 0, j = 0, flags = 0, np = 0, Lp = 0, qrow = 0, nt = 0, b = 0, rel = 0, phase = 0, cnt = 0;
       for (; cnt < round && w.valid; ++cnt) {
-        const bool first = first_of_cta || w.j == 0;
+        const bool first = w.fresh || w.j == 0;
         const bool seg_end = w.j == w.nt - 1;
         if (lane == cnt) {
           g = w.g * p.head_set + member;
@@ -482,11 +569,11 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
           b = w.b;
           qrow = w.q0 + w.piece * p.max_n;
           rel = w.rel;
-          u = w.u;
+          phase = w.phase;
         }
-        first_of_cta = false;
         w.next_tile(p);
-        if (lane == cnt) flags = (first ? 1 : 0) | (seg_end || !w.valid ? 2 : 0) | (!w.valid ? 4 : 0);
+        // 1: first, 2: last tile of this CTA's part of a segment, 4: of the CTA
+        if (lane == cnt) flags = (first ? 1 : 0) | (seg_end || !w.valid || w.fresh ? 2 : 0) | (!w.valid ? 4 : 0);
       }
       int page = -1, off = 0;
       if (lane < cnt) {
@@ -501,7 +588,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       for (int i = 0; i < cnt; ++i, ++jj) {
         const int st = jj % stages;
         const int gi = __shfl_sync(kFull, g, i), pi = __shfl_sync(kFull, page, i), oi = __shfl_sync(kFull, off, i);
-        int ji = 0, fi = 0, ni = 0, Li = 0, qi = 0, ti = 0, ri = 0, ui = 0;
+        int ji = 0, fi = 0, ni = 0, Li = 0, qi = 0, ti = 0, ri = 0, hi = 0;
         if (is_k) {
           ji = __shfl_sync(kFull, j, i);
           fi = __shfl_sync(kFull, flags, i);
@@ -510,7 +597,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
           qi = __shfl_sync(kFull, qrow, i);
           ti = __shfl_sync(kFull, nt, i);
           ri = __shfl_sync(kFull, rel, i);
-          ui = __shfl_sync(kFull, u, i);
+          hi = __shfl_sync(kFull, phase, i);
         }
         if (!mbar_wait_warp(&empty[st], ((jj / stages) & 1) ^ 1, abort)) {
           stop = true;
@@ -521,7 +608,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             const int e = jj % kInfoRing;
             info[3 * e] = make_int4(ji * 128, pi, oi, gi);
             info[3 * e + 1] = make_int4(ni, Li, qi, ti);
-            info[3 * e + 2] = make_int4(fi, ri, ui, 0);
+            info[3 * e + 2] = make_int4(fi, ri, hi, 0);
             mbar_arrive(&bars[B_INFO + e]);
           }
           mbar_arrive_expect_tx(&full[st], kTile);
@@ -667,22 +754,26 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     float ks_next = 0.f, vs_next = 1.f;   // the next tile's scales of this thread's token
 
     // A piece of a cut segment is done (its rows written): take a ticket.  The CTA that brings
-    // it to the number of pieces puts the counter back to zero and merges them all; a CTA has at most two cut segments,
+    // it to the number of pieces puts the counter back to zero and merges them all; a CTA has at most two cut segments a phase,
     // so it notes them and merges after its last tile, out of the loop's registers.
-    auto arrive_piece = [&](int p_first, int p_last, int R, int64_t out_base) {
+    constexpr int kSlots = 2 * kPhases<kMixed>;   // pieces a CTA may leave: two per phase
+    auto arrive_piece = [&](int phase, int p_first, int p_last, int R, int64_t out_base) {
       named_bar_sync(bar_id, 128);
       if (ct == 0) {
         // the CTAs of the segment's first and last tile
-        const int c0 = member * teams + static_cast<int>((start->x0 + p_first) / start->per);
-        const int c1 = member * teams + static_cast<int>((start->x0 + p_last) / start->per);
-        int32_t* ticket = p.counters + kTicketStride * c0;
+        const Start& st = start[phase];
+        const int c0 = member * teams + static_cast<int>((st.x0 + p_first) / st.per);
+        const int c1 = member * teams + static_cast<int>((st.x0 + p_last) / st.per);
+        int32_t* ticket = p.counters + kTicketStride * c0 + phase;
         __threadfence();   // release: the group's partial rows before the ticket
         if (atomicAdd(ticket, 1) == c1 - c0) {
           *ticket = 0;
-          Pending* d = pending + (pending[0].c1 >= 0 ? 1 : 0);
+          Pending* d = pending;
+          while (d->c1 >= 0) ++d;   // (at most one for each of the CTA's cut segments)
           d->c0 = c0;
           d->c1 = c1;
           d->rows = R;
+          d->phase = phase;
           d->out_base = out_base;
         }
       }
@@ -909,10 +1000,11 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       const int R = ib.x * G;
       // positions of the segment's first and last tile relative to this CTA's share: a segment inside it is finished
       // here, one that is cut leaves a piece
-      const int span = static_cast<int>(start->x1 - start->x0);
-      const int p_first = ic.y + ic.z * kSegCost, p_last = p_first + ic.z * (ib.w - 1);
+      const int phase = ic.z;
+      const int span = static_cast<int>(start[phase].x1 - start[phase].x0);
+      const int p_first = ic.y + kSegCost, p_last = p_first + ib.w - 1;
       const bool complete = p_first >= 0 && p_last < span;
-      const int slot = 2 * vcta + (p_first < 0 ? 0 : 1);   // (of a piece)
+      const int slot = kSlots * vcta + 2 * phase + (p_first < 0 ? 0 : 1);   // (of a piece)
       const int64_t out_base = ib.z * p.out_row_stride + static_cast<int64_t>(seg_g) * G * kHeadDim;
       if (ct < R) {
         const float lt = red[ct] + red[NP + ct] + red[2 * NP + ct] + red[3 * NP + ct];
@@ -955,7 +1047,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         }
       }
       tc_fence_before();
-      if (!complete) arrive_piece(p_first, p_last, R, out_base);
+      if (!complete) arrive_piece(phase, p_first, p_last, R, out_base);
       done = ic.x & 4;
       ++jj;
     }
@@ -963,13 +1055,15 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     const bool gave_up = named_bar_any(bar_id, 128, !alive);
     __threadfence();   // acquire: the other pieces' rows
 #pragma unroll 1
-    for (int i = 0; i < 2 && !gave_up; ++i) {
+    for (int i = 0; i < kSlots && !gave_up; ++i) {
       const Pending d = pending[i];
       if (d.c1 < 0) continue;
       // the piece of CTA c lies in its second slot where the segment begins (c0), in its first slot behind that
       const int pieces = d.c1 - d.c0 + 1;
       float* table = reinterpret_cast<float*>(smem + C::kK);   // [rows][pieces] weights; the rings are idle
-      auto piece_row = [&](int c, int r) { return static_cast<int64_t>(2 * (d.c0 + c) + (c == 0 ? 1 : 0)) * NP + r; };
+      auto piece_row = [&](int c, int r) {
+        return static_cast<int64_t>(kSlots * (d.c0 + c) + 2 * d.phase + (c == 0 ? 1 : 0)) * NP + r;
+      };
       // weights 2^(lse - max) / sum of pieces that saw a key; partials come from other CTAs: past L1
       if (pieces <= 16) {   // (a thread per row)
         if (ct < d.rows) {
@@ -1089,9 +1183,13 @@ int tile_rows(int64_t rows) {
   return rows <= 8 ? 8 : rows >= kMaxRows8 ? kMaxRows8 : static_cast<int>((rows + 7) / 8 * 8);
 }
 
-size_t workspace8(int sms, int nr) {
-  const int np = (nr + 15) / 16 * 16;
-  return decode_ticket_bytes(sms) + static_cast<size_t>(2) * (2 * sms) * np * (kHeadDim + 1) * sizeof(float);
+// Whether a varlen call of that row count takes the kernel for mixed lengths (pieces of 32 rows, 8-row runs apart).
+bool mixed_lengths(int nr, int group) { return nr > 16 && group <= 32; }
+
+size_t workspace8(int sms, int nr, int group) {
+  // two pieces per CTA of two per SM, or four of 32 rows
+  const size_t rows = std::max<size_t>(2 * static_cast<size_t>((nr + 15) / 16 * 16), mixed_lengths(nr, group) ? 4 * 32 : 0);
+  return decode_ticket_bytes(sms) + (2 * static_cast<size_t>(sms)) * rows * (kHeadDim + 1) * sizeof(float);
 }
 
 // The part of both calls after their own checks.
@@ -1101,15 +1199,16 @@ int run_attention(Fp8DecodeParams p, const void* k_cache, const void* v_cache, c
   const int64_t rows = static_cast<int64_t>(p.num_blocks) * p.block_size;
   const int sms = sm_count();
   if (sms == 0) return cuda_fail(cudaGetLastError());
-  if (workspace == nullptr || workspace_bytes < workspace8(sms, nr) ||
+  if (workspace == nullptr || workspace_bytes < workspace8(sms, nr, p.group) ||
       (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
     return NVA_ERR_WORKSPACE;
   CUtensorMap tm_k, tm_v;
   int rc;
   if ((rc = encode_rows8(&tm_k, k_cache, p.num_kv_heads, rows)) != NVA_OK) return rc;
   if ((rc = encode_rows8(&tm_v, v_cache, p.num_kv_heads, rows)) != NVA_OK) return rc;
-  const int grid = 2 * sms, np = (nr + 15) / 16 * 16;
-  const bool mixed = p.cu_q != nullptr && nr > 16;
+  const int grid = 2 * sms;
+  const bool mixed = p.cu_q != nullptr && mixed_lengths(nr, p.group);
+  const int rows_per_cta = mixed ? 4 * 32 : 2 * ((nr + 15) / 16 * 16);
   // (merge weights of a segment cut into as many pieces as there are CTAs fit the idle K and V rings)
   if (static_cast<size_t>(nr) * grid * sizeof(float) > 4 * kTile) return NVA_ERR_UNSUPPORTED;
   p.k_scale = k_scale;
@@ -1126,7 +1225,7 @@ int run_attention(Fp8DecodeParams p, const void* k_cache, const void* v_cache, c
   p.max_n = (mixed ? 32 : nr) / p.group;
   p.counters = static_cast<int32_t*>(workspace);
   p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + decode_ticket_bytes(sms));
-  p.part_lse = p.part_o + static_cast<size_t>(2) * grid * np * kHeadDim;
+  p.part_lse = p.part_o + static_cast<size_t>(grid) * rows_per_cta * kHeadDim;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   switch (mixed ? 0 : nr) {
@@ -1175,7 +1274,8 @@ NVA_API size_t nva_paged_attention_fp8_workspace_bytes(int32_t max_q, int32_t nu
       head_dim != nva::kHeadDim || num_heads / num_kv_heads > nva::kMaxRows8)
     return 0;
   const int sms = nva::sm_count();
-  return sms == 0 ? 0 : nva::workspace8(sms, nva::tile_rows(static_cast<int64_t>(max_q) * (num_heads / num_kv_heads)));
+  const int group = num_heads / num_kv_heads;
+  return sms == 0 ? 0 : nva::workspace8(sms, nva::tile_rows(static_cast<int64_t>(max_q) * group), group);
 }
 
 NVA_API int nva_paged_decode_fp8(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,

@@ -140,12 +140,14 @@ def test_rows_without_a_key(cuda):
 
 @pytest.mark.parametrize("qlens,lens", [([1], [1]), ([200, 1, 300], [456, 90, 300]), ([0, 5, 0, 1], [40, 5, 0, 700]),
                                         ([13, 1, 1, 64, 2], [13, 500, 1, 900, 131]), ([1000], [1000]),
-                                        ([7, 50], [3, 20]), ([4, 4, 4], [0, 4, 0])])
+                                        ([7, 50], [3, 20]), ([4, 4, 4], [0, 4, 0]), ([40, 1, 8, 16, 9], [40, 1, 8, 16, 9]),
+                                        ([33] * 5 + [1] * 70, [900] * 5 + list(range(1, 1400, 20))),
+                                        ([2500], [5000])])
 def test_varlen(cuda, qlens, lens):
     check(make(lens, qlens=qlens, seed=sum(qlens)))
 
 
-@pytest.mark.parametrize("H,KVH", [(8, 1), (16, 8), (20, 4)])
+@pytest.mark.parametrize("H,KVH", [(8, 1), (16, 8), (20, 4), (40, 1), (33, 1), (32, 1), (4, 4), (14, 2)])
 def test_varlen_head_layouts(cuda, H, KVH):
     check(make([300, 77, 520, 33], H=H, KVH=KVH, qlens=[100, 1, 9, 33], seed=H, G=64))
 
