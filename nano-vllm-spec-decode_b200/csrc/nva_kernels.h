@@ -91,6 +91,7 @@ struct Fp8DecodeParams {
   int32_t num_kv_heads;
   int32_t group;
   int32_t max_n;        // queries per piece: tile rows / group
+  int32_t longest;      // varlen: sequences with longer query runs are left to the prefill kernel
   int32_t head_set;     // kv heads that as many CTAs walk side by side (divides num_kv_heads and the grid)
   int32_t block_size;
   int32_t num_blocks;
@@ -126,6 +127,12 @@ struct PrefillParams {
   int32_t o_tma;                // 1: full output tiles are written by TMA stores through the output tensor map
   int32_t wait_primary;         // 1: the preceding kernel (the plan kernel) produced data this grid reads
   float scale_log2;
+  // 8-bit cache (prefill_kernel only; nullptr: bf16 K/V): scales [num_blocks, num_kv_heads, page_blocks]
+  const float* k_scale;
+  const float* v_scale;
+  int32_t page_blocks;
+  int32_t lg_block;
+  int32_t bt_width;
   int32_t* plan;                // workspace: [0] = number of items, [1..] = (seq << 12 | item of the sequence),
                                 // heaviest first, [1 + q_tiles_bound] = work counter (items taken after the first
                                 // wave)

@@ -133,6 +133,7 @@ __device__ __forceinline__ Shape8 shape_of(const Fp8DecodeParams& p, int b) {
   if (p.cu_q != nullptr) {
     const int a = __ldg(p.cu_q + b);
     s.n = max(__ldg(p.cu_q + b + 1) - a, 0);
+    if (s.n > p.longest) s.n = 0;   // (the prefill kernel's)
     s.q0 = a;
     s.L = max(__ldg(p.cu_k + b + 1) - __ldg(p.cu_k + b), 0);
   } else {
@@ -1186,10 +1187,16 @@ int tile_rows(int64_t rows) {
 // Whether a varlen call of that row count takes the kernel for mixed lengths (pieces of 32 rows, 8-row runs apart).
 bool mixed_lengths(int nr, int group) { return nr > 16 && group <= 32; }
 
-size_t workspace8(int sms, int nr, int group) {
+size_t pieces_bytes(int sms, int nr, int group) {
   // two pieces per CTA of two per SM, or four of 32 rows
   const size_t rows = std::max<size_t>(2 * static_cast<size_t>((nr + 15) / 16 * 16), mixed_lengths(nr, group) ? 4 * 32 : 0);
-  return decode_ticket_bytes(sms) + (2 * static_cast<size_t>(sms)) * rows * (kHeadDim + 1) * sizeof(float);
+  return (decode_ticket_bytes(sms) + (2 * static_cast<size_t>(sms)) * rows * (kHeadDim + 1) * sizeof(float) + 255) &
+         ~size_t(255);
+}
+
+// Tickets and pieces, then the prefill kernel's plan.
+size_t workspace8(int sms, int nr, int group) {
+  return pieces_bytes(sms, nr, group) + sizeof(int32_t) * (2 + static_cast<size_t>(kMaxPrefillTiles));
 }
 
 // The part of both calls after their own checks.
@@ -1228,6 +1235,7 @@ int run_attention(Fp8DecodeParams p, const void* k_cache, const void* v_cache, c
   p.part_lse = p.part_o + static_cast<size_t>(grid) * rows_per_cta * kHeadDim;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
+  if (p.longest == 0) p.longest = 0x7FFFFFFF;
   switch (mixed ? 0 : nr) {
     case 8: e = launch8<8, false>(tm_k, tm_v, p, grid, s); break;
     case 16: e = launch8<16, false>(tm_k, tm_v, p, grid, s); break;
@@ -1259,6 +1267,11 @@ int check_common(const void* q, int64_t q_row_stride, const void* k_cache, const
     return NVA_ERR_ALIGNMENT;
   return NVA_OK;
 }
+
+// Query runs of at least this many tokens take the prefill kernel, which gives each q head 128 rows of its own: its tile
+// of 128 keys takes about 2.5 us for the group's heads one after another, the pieces of 32 packed rows here 2 us each,
+// two at a time, so that runs of 80 cost about the same either way.
+constexpr int kMinPrefillRun = 81;
 
 bool positive_finite(float s) { return s > 0.f && s < 3.0e38f; }
 
@@ -1353,9 +1366,58 @@ NVA_API int nva_varlen_attention_fp8(const void* q, int64_t q_row_stride, const 
   p.block_size = block_size;
   p.num_blocks = num_blocks;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  return nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block,
-                            nva::tile_rows(static_cast<int64_t>(max_seqlen_q) * p.group), workspace, workspace_bytes,
-                            stream);
+  const int nr = nva::tile_rows(static_cast<int64_t>(max_seqlen_q) * p.group);
+  // Long runs: the prefill kernel, as far as its plan holds the call (1024 sequences, 4096 query tiles).
+  const int64_t tiles = static_cast<int64_t>(total_q) / 128 + num_seqs + 1;
+  const bool prefill = max_seqlen_q >= nva::kMinPrefillRun && num_seqs <= nva::kMaxDecodeSeqs &&
+                       tiles <= nva::kMaxPrefillTiles;
+  if (prefill) {
+    const int sms = nva::sm_count();
+    if (sms == 0) return nva::cuda_fail(cudaGetLastError());
+    if (workspace == nullptr || workspace_bytes < nva::workspace8(sms, nr, p.group) ||
+        (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
+      return NVA_ERR_WORKSPACE;
+    CUtensorMap tm_q, tm_k, tm_v, tm_o;
+    const int64_t rows = static_cast<int64_t>(num_blocks) * block_size;
+    if ((rc = nva::encode_rows8(&tm_k, k_cache, num_kv_heads, rows)) != NVA_OK) return rc;
+    if ((rc = nva::encode_rows8(&tm_v, v_cache, num_kv_heads, rows)) != NVA_OK) return rc;
+    if ((rc = nva::encode_rows(&tm_q, q, num_heads, total_q, q_row_stride * 2)) != NVA_OK) return rc;
+    if ((rc = nva::encode_rows(&tm_o, out, num_heads, total_q, out_row_stride * 2)) != NVA_OK) return rc;
+    nva::PrefillParams pp{};
+    pp.q = p.q;
+    pp.q_row_stride = q_row_stride;
+    pp.out = p.out;
+    pp.out_row_stride = out_row_stride;
+    pp.cu_q = cu_seqlens_q;
+    pp.cu_k = cu_seqlens_k;
+    pp.block_tables = block_tables;
+    pp.bt_stride = bt_row_stride;
+    pp.bt_width = bt_width;
+    pp.num_seqs = num_seqs;
+    pp.num_heads = num_heads;
+    pp.num_kv_heads = num_kv_heads;
+    pp.group = p.group;
+    pp.min_q = nva::kMinPrefillRun;
+    pp.block_size = block_size;
+    pp.num_blocks = num_blocks;
+    pp.q_tiles_bound = static_cast<int32_t>(tiles);
+    pp.tiles_per_item = 1;
+    pp.o_tma = 1;
+    pp.wait_primary = 1;
+    pp.scale_log2 = p.scale_log2;
+    pp.k_scale = k_scale;
+    pp.v_scale = v_scale;
+    pp.page_blocks = block_size / scale_block;
+    pp.lg_block = __builtin_ctz(static_cast<unsigned>(scale_block));
+    pp.plan = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + nva::pieces_bytes(sms, nr, p.group));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int grid = static_cast<int>(std::min<int64_t>(sms, tiles * num_heads));
+    cudaError_t e = nva::launch_prefill_plan(pp, s);
+    if (e == cudaSuccess) e = nva::launch_prefill(tm_q, tm_k, tm_v, tm_o, pp, grid, s);
+    if (e != cudaSuccess) return nva::cuda_fail(e);
+    p.longest = nva::kMinPrefillRun - 1;
+  }
+  return nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, nr, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -23,6 +23,12 @@
 // and redo the weights.  The row sums meet in spare TMEM columns.  The softmax warps stage
 // the normalised O tile in the item's Q buffer (TMA's 128-byte-swizzled two-slab layout) and move on; the writer
 // warp stores it (TMA for full 128-row tiles, plain stores for a sequence's last partial tile) and frees the buffer.
+//
+// From an 8-bit cache (kF8) K and V tiles arrive as raw e4m3 bytes and four more warps (12..15) widen them into the rings
+// while the tile before is worked on; everything behind the rings is the same.
+#include <cuda_fp8.h>
+#include <type_traits>
+
 #include "nva_ptx.cuh"
 #include "nva_kernels.h"
 
@@ -30,7 +36,6 @@ namespace nva {
 
 namespace {
 
-constexpr int kThreads = 384;           // 4 service warps + 2 softmax warpgroups
 constexpr int kSlab = 128 * 128;       // 128 rows x 128 bytes
 constexpr int kTile = 2 * kSlab;       // 128 rows x 256 bytes (all 128 dims, or 128 keys of P)
 constexpr int kItemRing = 8;           // item descriptors: producer is at most ~5 items ahead of the softmax warps
@@ -38,24 +43,31 @@ constexpr float kNegInf = -__builtin_huge_valf();
 constexpr uint32_t kFull = 0xffffffffu;
 constexpr float kRescaleLog2 = 8.0f;   // rescale O only when a row maximum grows by more than this (log2 units)
 
-// shared memory map (offsets from a 1024-aligned base)
-constexpr int kKStages = 2;
-constexpr int kVStages = 3;
-constexpr int kOffQ = 0;                              // 2 x Q tile
-constexpr int kOffK = kOffQ + 2 * kTile;              // K ring
-constexpr int kOffV = kOffK + kKStages * kTile;       // V ring
-constexpr int kOffBars = kOffV + kVStages * kTile;    // 32 x u64
-constexpr int kOffItems = kOffBars + 32 * 8;      // kItemRing x 2 x int4
-constexpr int kOffRed = kOffItems + kItemRing * 32;   // [2 tiles][2 groups][128 rows] half-row maxima
-constexpr int kOffTmem = kOffRed + 2 * 2 * 128 * 4;
-constexpr int kOffAbort = kOffTmem + 4;
-constexpr int kSmemBytes = kOffAbort + 4;             // the dynamic shared memory base is 1024-aligned (checked)
-static_assert(kSmemBytes <= 232448, "prefill shared memory budget");
+// Threads and shared memory map (offsets from a 1024-aligned base).  kF8: K and V come from an 8-bit cache, raw tiles of
+// 16 KB that four more warps widen into the rings (the V ring gives up a stage for the two raw buffers).
+template <bool kF8>
+struct Map {
+  static constexpr int kThreads = kF8 ? 512 : 384;   // 4 service warps + 2 softmax warpgroups (+ 4 widening warps)
+  static constexpr int kKStages = 2;
+  static constexpr int kVStages = kF8 ? 2 : 3;
+  static constexpr int kOffQ = 0;                              // 2 x Q tile
+  static constexpr int kOffK = kOffQ + 2 * kTile;              // K ring
+  static constexpr int kOffV = kOffK + kKStages * kTile;       // V ring
+  static constexpr int kOffRaw = kOffV + kVStages * kTile;     // (kF8) raw K tile, raw V tile
+  static constexpr int kOffBars = kOffRaw + (kF8 ? 2 * kSlab : 0);   // 32 x u64
+  static constexpr int kOffItems = kOffBars + 32 * 8;          // kItemRing x 2 x int4
+  static constexpr int kOffRed = kOffItems + kItemRing * 32;   // [2 tiles][2 groups][128 rows] half-row maxima
+  static constexpr int kOffTmem = kOffRed + 2 * 2 * 128 * 4;
+  static constexpr int kOffAbort = kOffTmem + 4;
+  static constexpr int kSmemBytes = kOffAbort + 4;             // the dynamic shared memory base is 1024-aligned (checked)
+  static_assert(kSmemBytes <= 232448, "prefill shared memory budget");
+};
 
 enum {
   B_QFULL = 0, B_QEMPTY = 2, B_KFULL = 4, B_KEMPTY = 6, B_VFULL = 8, B_VEMPTY = 11, B_SFULL = 14, B_PFULL = 16,
   B_ODONE = 17, B_ITEM = 18,  // B_ITEM + kItemRing <= B_OSTAGED
-  B_OSTAGED = 26              // 2: normalised O of the item staged in Q buffer 0 / 1
+  B_OSTAGED = 26,             // 2: normalised O of the item staged in Q buffer 0 / 1
+  B_RAWFULL = 28, B_RAWEMPTY = 30   // (kF8) raw K, raw V
 };
 
 struct Item {
@@ -148,21 +160,23 @@ __global__ void __launch_bounds__(1024) prefill_plan_kernel(const PrefillParams 
 }
 
 // ------------------------------------------------------------------------------------------------ main kernel
-__global__ void __launch_bounds__(kThreads, 1)
+template <bool kF8>
+__global__ void __launch_bounds__(Map<kF8>::kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
                const PrefillParams p) {
+  using C = Map<kF8>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
   if ((smem_u32(smem_raw) & 1023u) != 0) {   // the swizzled layouts need a 1024-byte aligned base
     if (threadIdx.x == 0) atomicOr(&g_error_word, kErrTimeout);
     return;
   }
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
-  int4* items = reinterpret_cast<int4*>(smem + kOffItems);
-  float* red = reinterpret_cast<float*>(smem + kOffRed);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOffTmem);
-  volatile int* abort = reinterpret_cast<volatile int*>(smem + kOffAbort);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
+  int4* items = reinterpret_cast<int4*>(smem + C::kOffItems);
+  float* red = reinterpret_cast<float*>(smem + C::kOffRed);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffTmem);
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + C::kOffAbort);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const bool paged = p.block_tables != nullptr;
 
@@ -171,13 +185,19 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       mbar_init(&bars[B_QFULL + i], 1);
       mbar_init(&bars[B_QEMPTY + i], 1);     // released by the writer warp once the staged O has been read
       mbar_init(&bars[B_OSTAGED + i], 256);  // the softmax threads' halves of O staged
-      mbar_init(&bars[B_KFULL + i], 1);
+      mbar_init(&bars[B_KFULL + i], kF8 ? 128 : 1);   // (kF8) the widening threads
       mbar_init(&bars[B_KEMPTY + i], 1);
       mbar_init(&bars[B_SFULL + i], 1);
     }
-    for (int i = 0; i < kVStages; ++i) {
-      mbar_init(&bars[B_VFULL + i], 1);
+    for (int i = 0; i < C::kVStages; ++i) {
+      mbar_init(&bars[B_VFULL + i], kF8 ? 128 : 1);
       mbar_init(&bars[B_VEMPTY + i], 1);
+    }
+    if constexpr (kF8) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&bars[B_RAWFULL + i], 1);
+        mbar_init(&bars[B_RAWEMPTY + i], 128);
+      }
     }
     mbar_init(&bars[B_PFULL], 256);
     mbar_init(&bars[B_ODONE], 1);
@@ -208,10 +228,11 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     // ------------------------------------------------------------ Q+K (warp 0) and V (warp 3) producers
     const bool is_k = warp == 0;
     const CUtensorMap* tm = is_k ? &tm_k : &tm_v;
-    uint8_t* ring = smem + (is_k ? kOffK : kOffV);
-    uint64_t* full = bars + (is_k ? B_KFULL : B_VFULL);
-    uint64_t* empty = bars + (is_k ? B_KEMPTY : B_VEMPTY);
-    const int stages = is_k ? kKStages : kVStages;
+    // (kF8) into the one raw tile of the operand
+    uint8_t* ring = kF8 ? smem + C::kOffRaw + (is_k ? 0 : kSlab) : smem + (is_k ? C::kOffK : C::kOffV);
+    uint64_t* full = bars + (kF8 ? B_RAWFULL + (is_k ? 0 : 1) : is_k ? B_KFULL : B_VFULL);
+    uint64_t* empty = bars + (kF8 ? B_RAWEMPTY + (is_k ? 0 : 1) : is_k ? B_KEMPTY : B_VEMPTY);
+    const int stages = kF8 ? 1 : is_k ? C::kKStages : C::kVStages;
     int g = 0;
     bool stop = false;
     int* counter = p.plan + 1 + p.q_tiles_bound;
@@ -251,7 +272,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         if (!mbar_wait_warp(&bars[B_QEMPTY + qb], ((it_count >> 1) & 1) ^ 1, abort)) break;
         if (elect_one()) {
           mbar_arrive_expect_tx(&bars[B_QFULL + qb], kTile);
-          uint8_t* dst = smem + kOffQ + qb * kTile;
+          uint8_t* dst = smem + C::kOffQ + qb * kTile;
           tma_load_3d(dst, &tm_q, 0, it.h, it.q0 + it.qt * 128, &bars[B_QFULL + qb]);
           tma_load_3d(dst + kSlab, &tm_q, 64, it.h, it.q0 + it.qt * 128, &bars[B_QFULL + qb]);
         }
@@ -263,9 +284,10 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         if (base + lane < it.nkv) {
           const int tok0 = (base + lane) * 128;
           if (paged) {
-            int page = __ldg(p.block_tables + (int64_t)it.b * p.bt_stride + tok0 / p.block_size);
+            const int col = tok0 / p.block_size;
+            int page = kF8 && col >= p.bt_width ? -1 : __ldg(p.block_tables + (int64_t)it.b * p.bt_stride + col);
             if (page < 0 || page >= p.num_blocks) {
-              if (is_k) atomicOr(&g_error_word, kErrBlockRange);
+              if (is_k && (!kF8 || tok0 < it.L)) atomicOr(&g_error_word, kErrBlockRange);
               page = -1;   // rows filled with zeros by TMA; nothing outside the pool is read
             }
             row0 = page * p.block_size + tok0 % p.block_size;
@@ -282,9 +304,14 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             break;
           }
           if (elect_one()) {
-            mbar_arrive_expect_tx(&full[st], kTile);
-            tma_load_3d(ring + st * kTile, tm, 0, kvh, r0, &full[st]);
-            tma_load_3d(ring + st * kTile + kSlab, tm, 64, kvh, r0, &full[st]);
+            if constexpr (kF8) {
+              mbar_arrive_expect_tx(&full[st], kSlab);
+              tma_load_3d(ring, tm, 0, kvh, r0 < 0 ? -128 : r0, &full[st]);
+            } else {
+              mbar_arrive_expect_tx(&full[st], kTile);
+              tma_load_3d(ring + st * kTile, tm, 0, kvh, r0, &full[st]);
+              tma_load_3d(ring + st * kTile + kSlab, tm, 64, kvh, r0, &full[st]);
+            }
           }
           __syncwarp();
         }
@@ -294,9 +321,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     // ------------------------------------------------------------ UMMA issuer
     constexpr uint32_t idesc_qk = umma_idesc_bf16(128, 128, false, false);
     constexpr uint32_t idesc_pv = umma_idesc_bf16(128, 128, false, true);
-    const uint32_t v_base = smem_u32(smem + kOffV);
-    const uint64_t q_desc0 = umma_desc_sw128(smem_u32(smem + kOffQ), 16, 1024);
-    const uint64_t k_desc0 = umma_desc_sw128(smem_u32(smem + kOffK), 16, 1024);
+    const uint32_t v_base = smem_u32(smem + C::kOffV);
+    const uint64_t q_desc0 = umma_desc_sw128(smem_u32(smem + C::kOffQ), 16, 1024);
+    const uint64_t k_desc0 = umma_desc_sw128(smem_u32(smem + C::kOffK), 16, 1024);
     const uint64_t v_desc0 = umma_desc_sw128(v_base, kSlab, 1024);
     // Issue order: QK(0), QK(1), then PV(g), QK(g+2), ...  QK(g+2) overwrites the S buffer that holds P(g), so it
     // must follow PV(g) (the tensor pipe runs one thread's products in issue order); every wait is a blocking,
@@ -340,9 +367,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     // S runs two tiles ahead of PV, so the end marker is read before PV reaches the last item
     while (ok && (!q_done || it_p < it_q)) {
       const int nkv_p = items[2 * (it_p % kItemRing)].w;   // published (and awaited) before this item's first QK
-      const int st = gp % kVStages;
+      const int st = gp % C::kVStages;
       if (!mbar_wait_warp(&bars[B_PFULL], gp & 1, abort)) break;
-      if (!mbar_wait_warp(&bars[B_VFULL + st], (gp / kVStages) & 1, abort)) break;
+      if (!mbar_wait_warp(&bars[B_VFULL + st], (gp / C::kVStages) & 1, abort)) break;
       tc_fence_after();
       if (elect_one()) {
         const uint64_t vd = v_desc0 + ((st * kTile) >> 4);
@@ -372,7 +399,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const int qb = it_count & 1;
       if (!mbar_wait_warp(&bars[B_OSTAGED + qb], (it_count >> 1) & 1, abort)) break;
       const int h = i0.z, row0 = i1.z + i0.y * 128, rows = i1.w;
-      const uint8_t* stage = smem + kOffQ + qb * kTile;
+      const uint8_t* stage = smem + C::kOffQ + qb * kTile;
       if (p.o_tma && rows == 128) {
         if (elect_one()) {
           tma_store_3d(&tm_o, stage, 0, h, row0);
@@ -407,6 +434,78 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       }
     }
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // every TMA store of this warp complete
+  } else if (kF8 && warp >= 12) {
+    // ------------------------------------------------------------ (kF8) widening warps: thread t owns token t of a tile
+    // Raw e4m3 rows (128-byte swizzle) times their scale, as bf16 in the layout the bf16 cache's TMA loads give: exact
+    // when the scale is a power of two, one rounding to bf16 else.  Tokens past the keys become zeros.
+    if constexpr (kF8) {
+      const int t = tid - 384;
+      int g = 0;
+      bool ok = true;
+      for (int it_count = 0; ok; ++it_count) {
+        const int e = it_count % kItemRing;
+        if (!mbar_wait_warp(&bars[B_ITEM + e], (it_count / kItemRing) & 1, abort)) break;
+        const int4 i0 = items[2 * e];
+        const int L = items[2 * e + 1].y;
+        if (i0.w == 0) break;
+        const int64_t kvh = i0.z / p.group;
+        const int32_t* table = p.block_tables + static_cast<int64_t>(i0.x) * p.bt_stride;
+        auto page_of = [&](int j) {
+          const int col = j * 128 / p.block_size;
+          return j < i0.w && col < p.bt_width ? __ldg(table + col) : -1;
+        };
+        float ks = 0.f, vs = 0.f;
+        auto load_scales = [&](int j, int page) {
+          ks = vs = 0.f;
+          if (page >= 0 && page < p.num_blocks && j * 128 + t < L) {
+            const int64_t at = (page * static_cast<int64_t>(p.num_kv_heads) + kvh) * p.page_blocks +
+                               ((j * 128 % p.block_size + t) >> p.lg_block);
+            ks = __ldg(p.k_scale + at);
+            vs = __ldg(p.v_scale + at);
+          }
+        };
+        load_scales(0, page_of(0));
+        for (int j = 0; j < i0.w && ok; ++j, ++g) {
+          const int next_page = page_of(j + 1);
+          const float scale[2] = {ks, vs};
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const int st = g & 1;
+            uint64_t* empty = &bars[(kv ? B_VEMPTY : B_KEMPTY) + st];
+            if (!mbar_wait_warp(&bars[B_RAWFULL + kv], g & 1, abort) ||
+                !mbar_wait_warp(empty, ((g >> 1) & 1) ^ 1, abort)) {
+              ok = false;
+              break;
+            }
+            const uint8_t* src = smem + C::kOffRaw + kv * kSlab;
+            uint8_t* dst = smem + (kv ? C::kOffV : C::kOffK) + st * kTile;
+            const bool live = j * 128 + t < L;
+            const float2 f2 = make_float2(scale[kv], scale[kv]);
+#pragma unroll 2
+            for (int c = 0; c < 8; ++c) {   // 16 dims
+              const uint4 raw = *reinterpret_cast<const uint4*>(src + sw128_offset(t, c));
+              const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+              uint32_t o[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
+                    static_cast<__nv_fp8x2_storage_t>(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
+                const float2 x = fmul2(__half22float2(*reinterpret_cast<const __half2*>(&h)), f2);
+                o[i] = live ? pack_bf16x2(x.x, x.y) : 0u;
+              }
+              uint8_t* slab = dst + (c >> 2) * kSlab;
+              const int chunk = 2 * (c & 3);
+              *reinterpret_cast<uint4*>(slab + sw128_offset(t, chunk)) = make_uint4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<uint4*>(slab + sw128_offset(t, chunk + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+            fence_proxy_async_smem();   // the widened rows before the products, the raw reads before the next copy
+            mbar_arrive(&bars[(kv ? B_VFULL : B_KFULL) + st]);
+            mbar_arrive(&bars[B_RAWEMPTY + kv]);
+            if (kv == 0) load_scales(j + 1, next_page);
+          }
+        }
+      }
+    }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ softmax + epilogue: two warpgroups
     // All eight softmax warps run the same sequence of named barriers (bar.red.or of "gave up"), one per tile and
@@ -432,14 +531,14 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       float m_used = kNegInf, l = 0.f;       // l: this thread's half of the row sum
       for (int j = 0; j < nkv; ++j, ++g) {
         const int st = g & 1;              // S / P buffer
-        const int vs = g % kVStages;       // V ring slot
+        const int vs = g % C::kVStages;       // V ring slot
         float s[64];
         float mpart = kNegInf;
         // paged keys past the sequence end may be stale or uninitialised: zero V there (P is 0 there anyway)
-        if (alive && wg == 0 && paged && j * 128 + 127 >= L) {
-          alive = mbar_wait_warp(&bars[B_VFULL + vs], (g / kVStages) & 1, abort);
+        if (!kF8 && alive && wg == 0 && paged && j * 128 + 127 >= L) {
+          alive = mbar_wait_warp(&bars[B_VFULL + vs], (g / C::kVStages) & 1, abort);
           if (alive && j * 128 + t >= L) {
-            uint8_t* vrow = smem + kOffV + vs * kTile + t * 128;
+            uint8_t* vrow = smem + C::kOffV + vs * kTile + t * 128;
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
               *reinterpret_cast<uint4*>(vrow + c * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -575,7 +674,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const float lt = lp[0] + lp[1];
       const float inv = lt > 0.f ? 1.f / lt : 0.f;
       const int qb = it_count & 1;
-      uint8_t* stage = smem + kOffQ + qb * kTile;
+      uint8_t* stage = smem + C::kOffQ + qb * kTile;
 #pragma unroll 1
       for (int c = 0; c < 64; c += 32) {
         float ot[32];
@@ -621,10 +720,15 @@ cudaError_t launch_prefill_plan(const PrefillParams& p, cudaStream_t stream) {
 cudaError_t launch_prefill(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                            const CUtensorMap& tm_o, const PrefillParams& p, int grid, cudaStream_t stream) {
   if (p.num_seqs > kMaxDecodeSeqs || p.q_tiles_bound > kMaxPrefillTiles) return cudaErrorInvalidValue;
-  const cudaError_t e = cudaFuncSetAttribute(prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  if (e != cudaSuccess) return e;
-  return launch_kernel(prefill_kernel, dim3(grid), dim3(kThreads), kSmemBytes, stream, true, tm_q, tm_k, tm_v, tm_o,
-                       p);
+  auto launch = [&](auto f8) {
+    constexpr bool kF8 = decltype(f8)::value;
+    constexpr int smem = Map<kF8>::kSmemBytes;
+    const cudaError_t e = cudaFuncSetAttribute(prefill_kernel<kF8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    return launch_kernel(prefill_kernel<kF8>, dim3(grid), dim3(Map<kF8>::kThreads), smem, stream, true, tm_q, tm_k, tm_v,
+                         tm_o, p);
+  };
+  return p.k_scale != nullptr ? launch(std::true_type{}) : launch(std::false_type{});
 }
 
 }  // namespace nva

@@ -131,6 +131,36 @@ def test_padding_sequences_and_poison_behind_the_context(cuda):
     assert (got[1] == 0).all() and (got[4] == 0).all() and _lib.device_error() == 0
 
 
+@pytest.mark.parametrize("qlens", [[81, 200, 300, 1], [80, 129, 17, 82]])
+def test_long_runs_with_poison_behind_the_context(cuda, qlens):
+    """Runs on either side of the length from which a kernel of their own takes them, pages full of NaN past the keys."""
+    from nvattn import _lib
+    lens = [81, 456, 300, 90]
+    b = make(lens, qlens=qlens, seed=23, spread=6, size=0.1)
+    want, bound = ref(b)
+    for c, s in zip(b["c"], b["s"]):
+        raw = c.view(torch.uint8)
+        for i, L in enumerate(lens):
+            for col in range((L + 255) // 256):
+                page = int(b["table"][i, col])
+                raw[page, max(0, L - col * 256):] = 0xFF
+                last = max(0, min(16, (L - col * 256 + 15) // 16))
+                s[page, :, last:] = float("inf")
+    got = run(b)
+    assert torch.isfinite(got).all() and ((got.double() - want).abs() <= bound).all() and _lib.device_error() == 0
+
+
+def test_long_run_without_keys_and_bad_pages(cuda):
+    from nvattn import _lib
+    b = make([0, 50, 700], qlens=[130, 200, 90], seed=24)
+    got = check(b)
+    assert (got[:130] == 0).all() and (got[130:280] == 0).all()
+    b["table"][2, 1] = -7
+    got = run(b)
+    assert torch.isfinite(got).all() and _lib.device_error() & 4
+    _lib.clear_device_error()
+
+
 def test_rows_without_a_key(cuda):
     """More queries than keys: the first rows see nothing and are zero, in pieces with and without keys."""
     b = make([3, 30, 12], n=20, seed=8)
