@@ -103,6 +103,7 @@ struct Fp8DecodeParams {
   float* part_o;        // [slots * grid, NP, 128], [slots * grid, NP] as in DecodeParams; two slots a CTA and phase
   float* part_lse;
   int32_t* counters;    // [grid][4] merge tickets (one a phase): zero on entry and on exit
+  int32_t pdl;          // 1: launched with a programmatic dependency on the prefill plan, before the prefill kernel
 };
 
 // Varlen prefill kernel (long query runs) — q rows tiled by 128 per (sequence, q head).

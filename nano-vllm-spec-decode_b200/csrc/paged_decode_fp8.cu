@@ -433,6 +433,12 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
+  // With a programmatic dependency on the prefill plan: wait for it (and what came before it), then let the call's
+  // prefill kernel start its blocks where this grid's leave.
+  if (p.pdl) {
+    griddep_wait();
+    if (tid == 0) griddep_launch_dependents();
+  }
   // ------------------------------------------------------------ the work split
   // Two scans over the sequences' costs: the total (hence each CTA's share), then the sequence that holds this CTA's
   // first position.  Batches of up to kThreads sequences keep the first scan's values in registers.
@@ -1168,7 +1174,7 @@ cudaError_t launch8(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const Fp8D
                                        Cfg8<NR>::kBytes);
   if (e != cudaSuccess) return e;
   return launch_kernel(paged_decode_fp8_kernel<NR, kMixed>, dim3(grid), dim3(Cfg8<NR>::kThreads), Cfg8<NR>::kBytes, stream,
-                       false, tm_k, tm_v, p);
+                       p.pdl != 0, tm_k, tm_v, p);
 }
 
 // 8-bit view {128 bytes, heads, rows} of a cache, 128 x 1 x 128 boxes, 128-byte swizzle.
@@ -1403,7 +1409,7 @@ NVA_API int nva_varlen_attention_fp8(const void* q, int64_t q_row_stride, const 
     pp.q_tiles_bound = static_cast<int32_t>(tiles);
     pp.tiles_per_item = 1;
     pp.o_tma = 1;
-    pp.wait_primary = 1;
+    pp.wait_primary = 0;
     pp.scale_log2 = p.scale_log2;
     pp.k_scale = k_scale;
     pp.v_scale = v_scale;
@@ -1412,10 +1418,15 @@ NVA_API int nva_varlen_attention_fp8(const void* q, int64_t q_row_stride, const 
     pp.plan = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + nva::pieces_bytes(sms, nr, p.group));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int grid = static_cast<int>(std::min<int64_t>(sms, tiles * num_heads));
+    // plan, short runs, long runs: the prefill kernel's blocks take their items from a counter as SMs come free
     cudaError_t e = nva::launch_prefill_plan(pp, s);
-    if (e == cudaSuccess) e = nva::launch_prefill(tm_q, tm_k, tm_v, tm_o, pp, grid, s);
     if (e != cudaSuccess) return nva::cuda_fail(e);
     p.longest = nva::kMinPrefillRun - 1;
+    p.pdl = 1;
+    rc = nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, nr, workspace, workspace_bytes, stream);
+    if (rc != NVA_OK) return rc;
+    e = nva::launch_prefill(tm_q, tm_k, tm_v, tm_o, pp, grid, s);
+    return e == cudaSuccess ? NVA_OK : nva::cuda_fail(e);
   }
   return nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, nr, workspace, workspace_bytes, stream);
 }
