@@ -14,9 +14,9 @@
 //
 // A token id is a whole number: two programs agree on it only if the running sums they compare agree far below the gap
 // between neighbouring sums, and a vocabulary has 150,000 of those.  So weights are fixed-point integers, w * 2^44
-// rounded from a double-precision exponential (relative error 1e-16: a table of 2^(j/256) and four terms of the
-// exponential series), and every sum is an exact 64-bit integer sum: no order of additions, atomics included, can change
-// a result.  Weights below 2^-45 are 0.
+// rounded from a double-precision exponential (a table of 2^(j/16) and five terms of the exponential series, off by
+// 1.5e-13 at most), and sums are exact 64-bit integer sums: no order of additions, atomics included, can change a result.
+// Weights below 2^-45 are 0.
 //
 // One pass over HBM: a cluster of CTAs keeps a row in its shared memory (V = 151,936 in bf16: four CTAs of 76 KB) as
 // order-preserving integer keys.  Thresholds of top-k and top-p come from histograms (counts, or fixed-point weights)
@@ -45,7 +45,7 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 1024;
-constexpr int kTable = 256;
+constexpr int kTable = 16;            // 128 bytes: whatever entries a warp's lanes ask for, no two meet in a bank
 constexpr int kList = 1024;            // tokens of a crossing bin kept aside per CTA
 constexpr int kMaxCluster = 8;
 constexpr float kReach = 31.5f;        // exp(-31.5) < 2^-45: weight 0
@@ -141,26 +141,35 @@ __device__ __forceinline__ int64_t read_id(const void* p, int64_t at, int bytes)
   return bytes == 8 ? static_cast<const int64_t*>(p)[at] : static_cast<const int32_t*>(p)[at];
 }
 
-// w * 2^44 of a logit within reach of the maximum, rounded, as the low 52 bits of a double in [2^52, 2^53):
-// 2^(u / 256) with u = 256 log2(e) (l - m) / T = 256 e + j + r, |r| <= 1/2, from a table of 2^(j / 256 + 44), e added to
-// its exponent, and three terms of the exponential series in r ln 2 / 256 (the fourth is below 1.5e-13: a running sum is
-// off by as little, against gaps of 1e-6 between a vocabulary's sums).
+// w * 2^44 of a logit within reach of the maximum: 2^(u / 16) with u = 16 log2(e) (l - m) / T = 16 e + j + r, |r| <= 1/2,
+// from a table of 2^(j / 16 + 44), e added to its exponent, and five terms of the exponential series in r ln 2 / 16 (the
+// sixth is below 1.5e-13: a running sum is off by as little, against gaps of 1e-6 between a vocabulary's sums).
 struct Weight {
-  double m, c;           // row maximum, 256 log2(e) / T
+  double m, c;           // row maximum, 16 log2(e) / T
   float low;             // logits above it have a weight
   const double* table;
-  __device__ __forceinline__ u64 bits(float l) const {   // (only for l > low)
+  __device__ __forceinline__ double2 factors(float l) const {   // their product is the weight (only for l > low)
     const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the nearest whole number
     const double d = static_cast<double>(l) - m;
     const double n = fma(d, c, magic);
     const double r = fma(d, c, magic - n);
     const int k = __double2loint(n);
-    double s = fma(r, 3.308302680541371e-09, 3.665565596910106e-06);   // (ln 2 / 256)^3 / 6, (ln 2 / 256)^2 / 2
-    s = fma(s, r, 0.0027076061740622863);                                // ln 2 / 256
+    double s = fma(r, 1.271587195055813e-09, 1.467610032291943e-07);   // (ln 2 / 16)^5 / 120, ^4 / 24
+    s = fma(s, r, 1.3550807779497455e-05);                            // ^3 / 6
+    s = fma(s, r, 0.0009383847928089871);                             // ^2 / 2
+    s = fma(s, r, 0.04332169878499658);                              // ln 2 / 16
     s = fma(s, r, 1.0);
-    const double t = table[k & 255];
-    const double scaled = __hiloint2double(__double2hiint(t) + ((k & ~255) << 12), __double2loint(t));   // + e << 20
-    return __double_as_longlong(fma(s, scaled, 4503599627370496.0));
+    const double t = table[k & 15];
+    return make_double2(s, __hiloint2double(__double2hiint(t) + ((k & ~15) << 16), __double2loint(t)));   // + e << 20
+  }
+  // as a double, and as the whole number in the low 52 bits of one in [2^52, 2^53)
+  __device__ __forceinline__ double value(float l) const {
+    const double2 f = factors(l);
+    return f.x * f.y;
+  }
+  __device__ __forceinline__ u64 bits(float l) const {
+    const double2 f = factors(l);
+    return __double_as_longlong(fma(f.x, f.y, 4503599627370496.0));
   }
   static constexpr u64 kZero = 0x4330000000000000ull;   // the bits of 2^52
   __device__ __forceinline__ u64 operator()(float l) const { return l > low ? bits(l) - kZero : 0ull; }
@@ -360,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   // ---------------------------------------------------------------- thresholds
   Weight weight;
   weight.m = top;
-  weight.c = 369.3299304675746 / static_cast<double>(temp);   // 256 log2(e)
+  weight.c = 23.083120654223414 / static_cast<double>(temp);   // 16 log2(e)
   // (below the maximum however large that is; at an infinite temperature everything but -inf)
   weight.low = fminf(fmaxf(top - kReach * temp, -FLT_MAX), nextafterf(top, -kInf));
   weight.table = table;
@@ -630,21 +639,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   u64 mine = 0;
   uint32_t ties = 0;
   {
-    if (cut <= weight.low) {
-      // nothing cut off: (nearly) every token has a weight, so all lanes take one and the few without drop theirs
-      const float low = weight.low;
+    const float dust = top - 1.3f * (top - weight.low);   // about 41 T below: 2^-59
+    if (cut <= weight.low && top - dust > 36.f * temp && dust > -FLT_MAX) {
+      // Nothing cut off: (nearly) every token has a weight.  All are taken, those without (and padding) as dust; the run's
+      // sum is one double, rounded to a whole number at its end (the order inside a run is fixed).
+      double sum = 0.0;
 #pragma unroll 4
       for (int w = run0; w < run0 + p.run_words; ++w)
-        R::each(data[w], [&](float l, int) {
-          const bool on = l > low;
-          const u64 b = weight.bits(on ? l : top);
-          mine += on ? b : Weight::kZero;
-        });
-      mine -= static_cast<u64>(p.run_words * kPer) * Weight::kZero;
+        R::each(data[w], [&](float l, int) { sum += weight.value(fmaxf(l, dust)); });
+      mine = static_cast<u64>(__double2ll_rn(sum));
     } else {
       for (int w = run0; w < run0 + p.run_words; ++w)
         R::each(data[w], [&](float l, int) {
-          if (l > cut) mine += weight.bits(l) - Weight::kZero;
+          if (l > cut) mine += weight(l);
         });
     }
     if (cut_ties > 0)
@@ -735,6 +742,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     const int count = p.run_words * kPer;
     u64 rest = found_rest;
     uint32_t seen = found_ties;
+    int last = 0;          // the last token with a weight: the tokens' rounded weights may end just short of the run's sum
     for (int base = 0; base < count; base += 32) {
       const int e = base + lane;
       float l = __int_as_float(0x7FFFFFFF);
@@ -752,19 +760,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         const u64 y = __shfl_up_sync(kAll, x, o);
         if (lane >= o) x += y;
       }
-      const uint32_t hit = __ballot_sync(kAll, x > rest);
-      if (hit != 0) {
-        if (lane == __ffs(hit) - 1) {
-          if constexpr (kVerify) {
-            p.row_result[row] = make_int2(token, accepted ? 1 : 0);
-          } else {
-            p.ids[row] = token;
-          }
-        }
-        break;
-      }
+      const uint32_t some = __ballot_sync(kAll, v != 0), hit = __ballot_sync(kAll, x > rest);
+      if (some != 0) last = __shfl_sync(kAll, token, 31 - __clz(hit != 0 ? hit & -hit : some));
+      if (hit != 0) break;
       rest -= __shfl_sync(kAll, x, 31);
       seen += __popc(tie_vote);
+    }
+    if (lane == 0) {
+      if constexpr (kVerify) {
+        p.row_result[row] = make_int2(last, accepted ? 1 : 0);
+      } else {
+        p.ids[row] = last;
+      }
     }
   }
   cluster.sync();   // nobody's shared memory goes while another CTA reads it
