@@ -640,7 +640,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   uint32_t ties = 0;
   {
     const float dust = top - 1.3f * (top - weight.low);   // about 41 T below: 2^-59
-    if (cut <= weight.low && top - dust > 36.f * temp && dust > -FLT_MAX) {
+    // (from 2^23 T on the logits' steps grow past T: there `dust` lies too near or beyond the exponential's range)
+    if (cut <= weight.low && top - dust > 36.f * temp && top - dust < 60.f * temp && dust > -FLT_MAX) {
       // Nothing cut off: (nearly) every token has a weight.  All are taken, those without (and padding) as dust; the run's
       // sum is one double, rounded to a whole number at its end (the order inside a run is fixed).
       double sum = 0.0;

@@ -120,6 +120,28 @@ def test_infinities_nan_and_masks(cuda, dtype):
     assert got.tolist() == x.float().argmax(-1).tolist()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t", [1e-3, 1e-6, 1e-9, 1e-20, 1e-38, 1.0])
+@pytest.mark.parametrize("scale", [1.0, 1e4, 1e10, 1e37])
+def test_steps_of_the_type_against_the_temperature(cuda, dtype, t, scale):
+    """Logits whose neighbours in the type lie many temperatures apart: the largest alone has a weight."""
+    V = 9001
+    x, g = rows(6, V, dtype, 8)
+    x = (x.double() * scale).to(dtype)
+    x[1, ::3] = float("-inf")
+    x[2, 5:] = float("-inf")
+    x[3] = x[3, 0]
+    x[3, 17] = float("-inf")
+    x[4] = -x[4].abs()
+    x[4, 4000:] = float("-inf")
+    x[5, 1::2] = torch.finfo(dtype).min
+    u = torch.rand(6, generator=g)
+    temp = torch.full((6,), t)
+    check(x, temp, u)
+    check(x, temp, u, top_k=torch.full((6,), 50).int(), top_p=torch.full((6,), 0.9))
+    check(x, temp, u, min_p=torch.full((6,), 1e-30))
+
+
 def test_extreme_settings(cuda):
     x, g = rows(10, 5000, torch.float32, 6)
     one = torch.ones(10)
