@@ -261,13 +261,15 @@ NVA_API size_t nva_paged_attention_fp8_workspace_bytes(int32_t max_q, int32_t nu
  * num_accepted = unbroken run of accepts; next_token = the draw from row num_accepted without the draft that was turned
  * down there, or, behind the last draft, the plain draw.  Drafts outside the vocabulary are never accepted.  This is
  * speculative sampling for proposals that are fixed tokens (n-gram matches, a greedy draft model): the tokens are
- * distributed as if drawn one by one.  Ids int32 (id_bytes 4) or int64 (8).  workspace needs no initial value.
+ * distributed as if drawn one by one.  Ids int32 (id_bytes 4) or int64 (8).  The workspace needs no initial
+ * value; calls that may overlap need one each.
  */
 #define NVA_MAX_SAMPLE_VOCAB 393216
 #define NVA_MAX_SAMPLE_ROWS (1 << 20)
 NVA_API int nva_sample_tokens(const void* logits, int64_t row_stride, int32_t rows, int32_t vocab, int32_t elem_bytes,
                               const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
-                              const void* uniform, int32_t uniform_bytes, int64_t* ids, void* stream);
+                              const void* uniform, int32_t uniform_bytes, int64_t* ids, void* workspace,
+                              size_t workspace_bytes, void* stream);
 NVA_API int nva_verify_sampled(const void* logits, int64_t row_stride, int32_t num_seqs, int32_t k, int32_t vocab,
                                int32_t elem_bytes, const void* draft_ids, int64_t draft_row_stride,
                                const void* num_drafts, int32_t id_bytes, const float* temperature,
@@ -275,7 +277,8 @@ NVA_API int nva_verify_sampled(const void* logits, int64_t row_stride, int32_t n
                                const void* accept_uniform, int64_t accept_row_stride, const void* uniform,
                                int32_t uniform_bytes, void* num_accepted, void* next_tokens, void* workspace,
                                size_t workspace_bytes, void* stream);
-NVA_API size_t nva_verify_sampled_workspace_bytes(int32_t num_seqs, int32_t k);
+/* Workspace of both calls (16-byte aligned); rows: the rows of logits. */
+NVA_API size_t nva_sample_workspace_bytes(int32_t rows, int32_t vocab, int32_t elem_bytes);
 
 /*
  * Device error word.  Kernels never trap: a slot or block id out of range, or a pipeline wait that ran past its

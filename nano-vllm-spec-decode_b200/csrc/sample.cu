@@ -24,6 +24,10 @@
 // bin's keys until one key is left; at that key the first m equal tokens stay, in index order.  CTAs exchange maxima,
 // histograms and sums through distributed shared memory.  For the draw every thread owns a run of consecutive tokens, a
 // prefix sum over threads and CTAs names the run that holds u * W, and one warp walks it.
+// Calls without top-k, top-p and min-p need no threshold, so no row has to stay on the chip: one kernel gives a warp each
+// a segment of 4 KB, straight from registers (its maximum, then its weights' sum against that), a second one brings a
+// row's segments to one maximum, draws a segment and walks it (510 rows of 151,936: 140 us with the row in shared memory,
+// where loads, exchanges and sums of a CTA follow one another).
 // Bound: the double-precision exponentials, one per token that no threshold removes (a row with top-k only takes them
 // for the k kept ones), next to the one read of the logits.
 #include <cooperative_groups.h>
@@ -97,6 +101,10 @@ template <>
 struct Row<__nv_bfloat16> {
   static constexpr int kPerWord = 2;
   static constexpr uint32_t kPad = 0xFFFFu;
+  static __device__ __forceinline__ uint32_t both(float l) {   // in every place of a word, rounded to the type
+    const __nv_bfloat162 v = __float2bfloat162_rn(l);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {   // the number where one is NaN
     const __nv_bfloat162 v =
         __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
@@ -119,6 +127,7 @@ template <>
 struct Row<float> {
   static constexpr int kPerWord = 1;
   static constexpr uint32_t kPad = 0xFFFFFFFFu;
+  static __device__ __forceinline__ uint32_t both(float l) { return __float_as_uint(l); }
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
     return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
   }
@@ -175,7 +184,19 @@ struct Weight {
   __device__ __forceinline__ u64 operator()(float l) const { return l > low ? bits(l) - kZero : 0ull; }
 };
 
-// Block-wide exclusive prefix sums of a weight and a count; `tot` receives the block's sums.
+// Weights of logits up to `top` > -inf, finite, at temperature `temp`.
+__device__ __forceinline__ Weight make_weight(float top, float temp, const double* table) {
+  Weight w;
+  w.m = top;
+  w.c = 23.083120654223414 / static_cast<double>(temp);   // 16 log2(e)
+  // (below the maximum however large that is; at an infinite temperature everything but -inf)
+  w.low = fminf(fmaxf(top - kReach * temp, -FLT_MAX), nextafterf(top, -__int_as_float(0x7F800000)));
+  w.table = table;
+  return w;
+}
+
+// Exclusive prefix sums of a weight and a count over a block of kCount warps; `tot` receives the block's sums.
+template <int kCount>
 __device__ __forceinline__ void block_scan(u64& mass, uint32_t& count, u64* wm, uint32_t* wc, u64* tot_m,
                                            uint32_t* tot_c, int lane, int warp) {
   u64 x = mass;
@@ -197,7 +218,7 @@ __device__ __forceinline__ void block_scan(u64& mass, uint32_t& count, u64* wm, 
   u64 bm = 0, tm = 0;
   uint32_t bc = 0, tc = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < kCount; ++w) {
     if (w < warp) {
       bm += wm[w];
       bc += wc[w];
@@ -367,12 +388,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   }
 
   // ---------------------------------------------------------------- thresholds
-  Weight weight;
-  weight.m = top;
-  weight.c = 23.083120654223414 / static_cast<double>(temp);   // 16 log2(e)
-  // (below the maximum however large that is; at an infinite temperature everything but -inf)
-  weight.low = fminf(fmaxf(top - kReach * temp, -FLT_MAX), nextafterf(top, -kInf));
-  weight.table = table;
+  const Weight weight = make_weight(top, temp, table);
   // kept: logits above `cut`, and the first `cut_ties` tokens at it
   float cut = -kInf;
   uint32_t cut_ties = 0;
@@ -431,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         }
         u64 pre = v[0] + v[1], tot;
         uint32_t none = 0, none_t;
-        block_scan(pre, none, scan_m, scan_c, &tot, &none_t, lane, warp);
+        block_scan<kWarps>(pre, none, scan_m, scan_c, &tot, &none_t, lane, warp);
         // (the first token always stays: a target of 0 would find no crossing)
         const double target = !linear ? ctrl.target : kMass ? fmax(share * static_cast<double>(tot), 1.0) : k;
         auto tell = [&](uint32_t bin, u64 above) {
@@ -664,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   {
     u64 tm;
     uint32_t tc;
-    block_scan(pre_m, pre_c, scan_m, scan_c, &tm, &tc, lane, warp);
+    block_scan<kWarps>(pre_m, pre_c, scan_m, scan_c, &tm, &tc, lane, warp);
     if (tid == 0) {
       ctrl.sum = tm;
       ctrl.ties = tc;
@@ -778,6 +794,432 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   cluster.sync();   // nobody's shared memory goes while another CTA reads it
 }
 
+// ------------------------------------------------------------------------------------------------ temperature alone
+constexpr int kVectors = 8;            // 16-byte vectors of a segment per lane
+template <typename T>
+constexpr int kSegment = 32 * kVectors * 4 * Row<T>::kPerWord;   // tokens
+
+struct Segment {
+  double sum;                          // weights against `top` (equals of an infinite one count 1)
+  float top;
+  uint32_t first;                      // greedy: first index of the segment's largest logit (or of its first NaN)
+};
+static_assert(sizeof(Segment) == 16, "Segment");
+
+// The same weights, two at a time, for sums that start at a segment's maximum: the argument 16 log2(e) l / T is reduced in
+// single precision with its rounding error carried along (u = n + q, |q| <= 1/2, from the constant's two parts), the
+// maximum's own n and q taken off, so that its weight is 1.  Rounding q and the series leaves 2e-9 of a token's weight,
+// either way and different from token to token; the products with the table, and the sums, are in double precision.
+// Needs |16 log2(e) l / T| < 2^20.  One double-precision multiply-add and one sum per token instead of eleven operations
+// (510 rows of 151,936: 112 -> 83 us together with the smaller draw blocks).
+struct PairWeight {
+  float c, lo, q0, zero;
+  double one;                    // 1 / the maximum's weight as `sum` has it
+  const double* table;           // 2^(j / 16), less j << 16 in its high word
+  static constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: the sum's low bits are the nearest whole number
+  __device__ __forceinline__ PairWeight(float top, const Weight& w, const double* shifted) {
+    c = static_cast<float>(w.c);
+    lo = static_cast<float>(w.c - static_cast<double>(c));
+    const float n = fmaf(top, c, kMagic) - kMagic;
+    const float n16 = floorf(n * 0.0625f) * 16.f;      // taken off n, the rest of it stays in the table's index
+    zero = kMagic - n16;
+    q0 = fmaf(top, lo, fmaf(top, c, -n));
+    table = shifted;
+    one = 1.0 / w.table[static_cast<int>(n - n16) & 15];
+  }
+  __device__ __forceinline__ double scaled(float s, int n) const {   // n = 16 e + j: e << 20 with j << 16 below it
+    const double t = table[n & 15];
+    const double e = __hiloint2double(__double2hiint(t) + (n << 16), __double2loint(t));
+    return fma(static_cast<double>(s), e, e);
+  }
+  __device__ __forceinline__ double sum(float2 l) const {
+    const float2 y = ffma2(l, make_float2(c, c), make_float2(zero, zero));
+    const float2 n = fsub2(make_float2(zero, zero), y);
+    float2 r = ffma2(l, make_float2(lo, lo), ffma2(l, make_float2(c, c), n));
+    r = fsub2(r, make_float2(q0, q0));
+    float2 s = ffma2(r, make_float2(1.271587195055813e-09f, 1.271587195055813e-09f),
+                     make_float2(1.467610032291943e-07f, 1.467610032291943e-07f));
+    s = ffma2(s, r, make_float2(1.3550807779497455e-05f, 1.3550807779497455e-05f));
+    s = ffma2(s, r, make_float2(0.0009383847928089871f, 0.0009383847928089871f));
+    s = ffma2(s, r, make_float2(0.04332169878499658f, 0.04332169878499658f));
+    s = fmul2(s, r);
+    return scaled(s.x, __float_as_int(y.x)) + scaled(s.y, __float_as_int(y.y));
+  }
+};
+
+// This lane's words of kCount vectors from token e0 of the row: vector v, lane l are the tokens from
+// e0 + ((v * 32 + l) * 4) * kPer.  Tokens past the row are -inf.
+template <typename T, int kCount>
+__device__ __forceinline__ void load_vectors(const T* row, int vocab, int e0, int lane, uint4 (&x)[kCount]) {
+  constexpr int kPer = Row<T>::kPerWord;
+  const uint32_t low = kPer == 2 ? 0xFF80FF80u : 0xFF800000u;
+  const T* src = row + e0;
+  if ((reinterpret_cast<uintptr_t>(src) & 15u) == 0 && e0 + kCount * 128 * kPer <= vocab) {
+#pragma unroll
+    for (int v = 0; v < kCount; ++v) x[v] = __ldg(reinterpret_cast<const uint4*>(src) + v * 32 + lane);
+    return;
+  }
+#pragma unroll
+  for (int v = 0; v < kCount; ++v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = low;
+#pragma unroll
+      for (int h = 0; h < kPer; ++h) {
+        const int e = ((v * 32 + lane) * 4 + i) * kPer + h;
+        if (e0 + e < vocab) {
+          const uint32_t b = kPer == 2 ? static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(src) + e))
+                                       : __ldg(reinterpret_cast<const uint32_t*>(src) + e);
+          w[i] = kPer == 2 ? (w[i] & ~(0xFFFFu << (16 * h))) | (b << (16 * h)) : b;
+        }
+      }
+    }
+    x[v] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256, 4) segment_kernel(const SampleParams p, Segment* __restrict__ segments,
+                                                         int per_row) {
+  using R = Row<T>;
+  constexpr int kPer = R::kPerWord;
+  const float kInf = __int_as_float(0x7F800000);
+  __shared__ double table[kTable], shifted[kTable];
+  if (threadIdx.x < kTable) {
+    const double t = exp2(static_cast<double>(threadIdx.x) / kTable);
+    table[threadIdx.x] = t;
+    shifted[threadIdx.x] = __hiloint2double(__double2hiint(t) - static_cast<int>(threadIdx.x << 16), __double2loint(t));
+  }
+  const int lane = threadIdx.x & 31;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int row = static_cast<int>(id / per_row), seg = static_cast<int>(id - static_cast<int64_t>(row) * per_row);
+  const bool any = row < p.rows;
+  uint4 x[kVectors];
+  float temp = 0.f;
+  const int e0 = seg * kSegment<T>;
+  if (any) {
+    temp = __ldg(p.temperature + row / p.group);
+    load_vectors<T>(static_cast<const T*>(p.logits) + row * p.row_stride, p.vocab, e0, lane, x);
+  }
+  __syncthreads();
+  if (!any) return;
+  const bool greedy = !(temp > 0.f);
+  const uint32_t low = kPer == 2 ? 0xFF80FF80u : 0xFF800000u;   // -inf
+  uint32_t best = low;    // (never NaN)
+  bool nan = false;
+#pragma unroll
+  for (int v = 0; v < kVectors; ++v)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) best = R::larger(best, word_of(x[v], i));
+  if (greedy) {
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) R::each(word_of(x[v], i), [&](float l, int) { nan |= l != l; });
+  }
+  float top = -kInf;
+  R::each(best, [&](float l, int) { top = fmaxf(top, l); });
+  uint32_t k = __float_as_uint(top + 0.f);
+  k = __reduce_max_sync(kAll, (k & 0x80000000u) ? ~k : (k | 0x80000000u));
+  top = __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+  Segment out;
+  out.top = top;
+  out.first = 0;
+  out.sum = 0.0;
+  if (greedy) {
+    nan = __any_sync(kAll, nan);
+    uint32_t first = kNone;
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        R::each(word_of(x[v], i), [&](float l, int h) {
+          const int e = e0 + ((v * 32 + lane) * 4 + i) * kPer + h;
+          if (first == kNone && e < p.vocab && (nan ? l != l : l == top)) first = static_cast<uint32_t>(e);
+        });
+    out.first = __reduce_min_sync(kAll, first);
+    if (nan) out.top = __int_as_float(0x7FFFFFFF);
+  } else {
+    double sum = 0.0;
+    if (top - top != 0.f) {
+      // an infinite maximum: its equals weigh 1 (segments of nothing but -inf count where the whole row is so)
+      int count = 0;
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          R::each(word_of(x[v], i), [&](float l, int h) {
+            count += fmaxf(l, -kInf) == top && e0 + ((v * 32 + lane) * 4 + i) * kPer + h < p.vocab ? 1 : 0;
+          });
+      sum = count;
+    } else {
+      const Weight weight = make_weight(top, temp, table);
+      // about 41 T below, 2^-59; (nearly) every token has a weight, and those that have not (padding and NaN too) count
+      // as dust
+      const uint32_t dusts = R::both(top - 1.3f * (top - weight.low));
+      float dust = 0.f;
+      R::each(dusts, [&](float l, int) { dust = l; });
+      const PairWeight pair(top, weight, shifted);
+      if (top - dust > 36.f * temp && top - dust < 60.f * temp && dust > -FLT_MAX &&
+          fmaxf(fabsf(top), fabsf(dust)) * pair.c < 1048576.f) {
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+          float l[4 * kPer];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            R::each(R::larger(word_of(x[v], i), dusts), [&](float y, int h) { l[i * kPer + h] = y; });
+#pragma unroll
+          for (int i = 0; i < 4 * kPer; i += 2) sum += pair.sum(make_float2(l[i], l[i + 1]));
+        }
+        sum *= pair.one;
+      } else {
+        for (int v = 0; v < kVectors; ++v) {
+          const uint4 w = v == 0 ? x[0] : v == 1 ? x[1] : v == 2 ? x[2] : v == 3 ? x[3] : v == 4 ? x[4]
+                          : v == 5 ? x[5] : v == 6 ? x[6] : x[7];
+          for (int i = 0; i < 4; ++i)
+            R::each(word_of(w, i), [&](float l, int) {
+              if (l > weight.low) sum += weight.value(l);
+            });
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+    out.sum = sum;
+  }
+  if (lane == 0) segments[id] = out;
+}
+
+// One block per row; a thread holds up to four neighbouring segments (blocks of one segment a thread, 512 threads, took one
+// SM each: 30 us for 510 rows instead of 12).
+constexpr int kDrawThreads = 128;
+constexpr int kDrawWarps = kDrawThreads / 32;
+constexpr int kDrawSegments = 4;
+
+template <typename T, bool kVerify>
+__global__ void __launch_bounds__(kDrawThreads, 4) draw_kernel(const SampleParams p, const Segment* __restrict__ segments,
+                                                            int per_row) {
+  using R = Row<T>;
+  constexpr int kPer = R::kPerWord;
+  const float kInf = __int_as_float(0x7F800000);
+  static_assert(NVA_MAX_SAMPLE_VOCAB <= kDrawThreads * kDrawSegments * kSegment<float>, "segments of a row");
+  __shared__ double table[kTable];
+  __shared__ u64 scan_m[kDrawWarps];
+  __shared__ uint32_t scan_c[kDrawWarps];
+  __shared__ u64 draft_part;             // the draft's weight, as far as its segment's sum has it
+  __shared__ u64 found_rest;
+  __shared__ int found;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x;
+  const int set = row / p.group;
+  const float temp = __ldg(p.temperature + set);
+  const T* src = static_cast<const T*>(p.logits) + row * p.row_stride;
+  if (tid < kTable) table[tid] = exp2(static_cast<double>(tid) / kTable + 44.0);
+  if (tid == 0) {
+    found = 0;
+    found_rest = 0;
+    draft_part = 0;
+  }
+  int draft = -1;
+  if constexpr (kVerify) {
+    const int k = p.group - 1, j = row - set * p.group;
+    if (j < k && j < read_id(p.num_drafts, set, p.id_bytes)) {
+      const int64_t d = read_id(p.drafts, set * p.draft_stride + j, p.id_bytes);
+      draft = d >= 0 && d < p.vocab ? static_cast<int>(d) : p.vocab;
+    }
+  }
+  const int s0 = tid * kDrawSegments;
+  Segment seg[kDrawSegments];
+#pragma unroll
+  for (int i = 0; i < kDrawSegments; ++i) {
+    seg[i].top = -kInf;
+    seg[i].sum = 0.0;
+    seg[i].first = kNone;
+    if (s0 + i < per_row) seg[i] = segments[static_cast<int64_t>(row) * per_row + s0 + i];
+  }
+  auto tell = [&](int token, bool accepted) {
+    if constexpr (kVerify) {
+      p.row_result[row] = make_int2(token, accepted ? 1 : 0);
+    } else {
+      p.ids[row] = token;
+    }
+  };
+  // the row's maximum
+  auto key = [](float l) {
+    const uint32_t k = __float_as_uint(l + 0.f);
+    return l != l ? kNone : (k & 0x80000000u) ? ~k : (k | 0x80000000u);
+  };
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < kDrawSegments; ++i) most = max(most, key(seg[i].top));
+  most = __reduce_max_sync(kAll, most);
+  if (lane == 0) scan_c[warp] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kDrawWarps; ++w) most = max(most, scan_c[w]);
+  __syncthreads();
+  if (!(temp > 0.f)) {   // argmax: the first segment with the row's largest holds it
+    uint32_t first = kNone;
+#pragma unroll
+    for (int i = 0; i < kDrawSegments; ++i)
+      if (key(seg[i].top) == most) first = min(first, seg[i].first);
+    first = __reduce_min_sync(kAll, first);
+    if (lane == 0) scan_c[warp] = first;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < kDrawWarps; ++w) first = min(first, scan_c[w]);
+      tell(static_cast<int>(first), draft == static_cast<int>(first));
+    }
+    return;
+  }
+  const float top = __uint_as_float((most & 0x80000000u) ? (most & 0x7FFFFFFFu) : ~most);
+  const bool flat = top - top != 0.f;      // infinite: its equals weigh 1
+  const Weight weight = make_weight(flat ? 0.f : top, temp, table);
+  auto weigh = [&](float l) -> u64 { return flat ? (l == top ? 1ull << 44 : 0ull) : weight(l); };
+  u64 draft_w = 0;
+  if (kVerify && draft >= 0 && draft < p.vocab) {
+    // the draft's weight (every thread: one address)
+    const uint32_t b = kPer == 2 ? static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(src) + draft)) << 16
+                                 : __ldg(reinterpret_cast<const uint32_t*>(src) + draft);
+    const float l = __uint_as_float(b);
+    draft_w = weigh(l != l ? -kInf : l);
+  }
+  // segments against the row's maximum, as whole numbers
+  u64 kept[kDrawSegments];
+  u64 mine = 0;
+#pragma unroll
+  for (int i = 0; i < kDrawSegments; ++i) {
+    double f = seg[i].top == top ? 1.0 : 0.0;
+    if (!flat && seg[i].top != top && seg[i].top > -kInf)
+      f = exp((static_cast<double>(seg[i].top) - static_cast<double>(top)) / static_cast<double>(temp));
+    kept[i] = static_cast<u64>(__double2ll_rn(seg[i].sum * f * 17592186044416.0));   // 2^44
+    if (kVerify && draft >= 0 && s0 + i == draft / kSegment<T>) draft_part = min(draft_w, kept[i]);
+    mine += kept[i];
+  }
+  u64 at = mine, total;
+  uint32_t none = 0, none_t;
+  block_scan<kDrawWarps>(at, none, scan_m, scan_c, &total, &none_t, lane, warp);
+  bool accepted = false;
+  if constexpr (kVerify) {
+    if (draft >= 0) {
+      const double ua = read_uniform(p.accept_uniform, set * p.accept_stride + (row - set * p.group), p.uniform_bytes);
+      accepted = ua * static_cast<double>(total) < static_cast<double>(draft_w);
+      // without the draft
+      const int there = draft / kSegment<T>;
+      const u64 less = draft_part;
+#pragma unroll
+      for (int i = 0; i < kDrawSegments; ++i)
+        if (s0 + i == there) kept[i] -= less;
+      if (s0 > there) at -= less;
+      total -= less;
+    }
+  }
+  const double un = read_uniform(p.uniform, set, p.uniform_bytes);
+  u64 want = static_cast<u64>(un * static_cast<double>(total));
+  if (total > 0 && want >= total) want = total - 1;
+#pragma unroll
+  for (int i = 0; i < kDrawSegments; ++i) {
+    if (want >= at && want - at < kept[i]) {
+      found = s0 + i;
+      found_rest = want - at;
+    }
+    at += kept[i];
+  }
+  __syncthreads();
+  if (total == 0) {         // nothing but the (then accepted) draft
+    if (tid == 0) tell(draft, accepted);
+    return;
+  }
+  // the block walks the segment: a share of its vectors each warp, in index order
+  constexpr int kShare = kVectors / kDrawWarps;
+  const int e0 = found * kSegment<T>, e1 = e0 + warp * kShare * 128 * kPer;
+  u64 rest = found_rest;
+  u64 w[kShare][4 * kPer], sum[kShare], up_to[kShare], share = 0;
+  {
+    uint4 x[kShare];
+    load_vectors<T>(src, p.vocab, e1, lane, x);
+#pragma unroll
+    for (int v = 0; v < kShare; ++v) {
+      sum[v] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        R::each(word_of(x[v], i), [&](float l, int h) {
+          const int e = e1 + ((v * 32 + lane) * 4 + i) * kPer + h;
+          u64 y = e < p.vocab ? weigh(l != l ? -kInf : l) : 0ull;
+          if (kVerify && e == draft) y = 0;
+          w[v][i * kPer + h] = y;
+          sum[v] += y;
+        });
+      up_to[v] = sum[v];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(kAll, up_to[v], o);
+        if (lane >= o) up_to[v] += y;
+      }
+      up_to[v] += share;
+      share = __shfl_sync(kAll, up_to[v], 31);
+    }
+  }
+  if (lane == 0) scan_m[warp] = share;
+  __syncthreads();
+  u64 before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kDrawWarps; ++i) {
+    if (i < warp) before += scan_m[i];
+    all += scan_m[i];
+  }
+  if (all != 0) {
+    // (the segment's own sum is rounded differently: a number past the last weight draws the last token with one)
+    rest = min(rest, all - 1);
+#pragma unroll
+    for (int v = 0; v < kShare; ++v) {
+      u64 run = before + up_to[v] - sum[v];
+      if (rest < run || rest - run >= sum[v]) continue;
+      int token = -1;
+#pragma unroll
+      for (int i = 0; i < 4 * kPer; ++i) {
+        run += w[v][i];
+        if (token < 0 && run > rest) token = e1 + (v * 32 + lane) * 4 * kPer + i;
+      }
+      tell(token, accepted);
+    }
+    return;
+  }
+  // a sum of parts below 2^-44 each: its largest
+  if (warp != 0) return;
+  uint4 x[kVectors];
+  load_vectors<T>(src, p.vocab, e0, lane, x);
+  int last;
+  {
+    uint32_t best = 0;
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        R::each(word_of(x[v], i), [&](float l, int h) {
+          const int e = e0 + ((v * 32 + lane) * 4 + i) * kPer + h;
+          if (l > -kInf && !(kVerify && e == draft)) best = max(best, key(l));
+        });
+    best = __reduce_max_sync(kAll, best);
+    uint32_t first = kNone;
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        R::each(word_of(x[v], i), [&](float l, int h) {
+          const int e = e0 + ((v * 32 + lane) * 4 + i) * kPer + h;
+          if (l > -kInf && !(kVerify && e == draft) && key(l) == best) first = min(first, static_cast<uint32_t>(e));
+        });
+    first = __reduce_min_sync(kAll, first);
+    last = first != kNone ? static_cast<int>(first) : draft;
+  }
+  if (lane == 0) tell(last, accepted);
+}
+
 // Accepted drafts of each sequence and the token behind them.
 template <typename I>
 __global__ void __launch_bounds__(128) verify_merge_kernel(const int2* __restrict__ rows, int32_t sets, int32_t k,
@@ -823,12 +1265,34 @@ cudaError_t launch_rows(SampleParams p, int sms, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+template <typename T, bool kVerify>
+cudaError_t launch_plain(const SampleParams& p, Segment* segments, cudaStream_t stream) {
+  const int per_row = (p.vocab + kSegment<T> - 1) / kSegment<T>;
+  const int64_t blocks = (static_cast<int64_t>(p.rows) * per_row + 7) / 8;
+  segment_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, segments, per_row);
+  draw_kernel<T, kVerify><<<static_cast<unsigned>(p.rows), kDrawThreads, 0, stream>>>(p, segments, per_row);
+  return cudaGetLastError();
+}
+
+size_t segments_bytes(int64_t rows, int32_t vocab, int32_t elem_bytes) {
+  const int tokens = elem_bytes == 2 ? kSegment<__nv_bfloat16> : kSegment<float>;
+  return static_cast<size_t>(rows) * static_cast<size_t>((vocab + tokens - 1) / tokens) * sizeof(Segment);
+}
+
+// `scratch`: segments_bytes, used without any of top-k, top-p and min-p.
 template <bool kVerify>
-int launch_sample(const SampleParams& p, int elem_bytes, cudaStream_t stream) {
-  const int sms = sm_count();
-  if (sms == 0) return cuda_fail(cudaGetLastError());
-  const cudaError_t e = elem_bytes == 2 ? launch_rows<__nv_bfloat16, kVerify>(p, sms, stream)
-                                        : launch_rows<float, kVerify>(p, sms, stream);
+int launch_sample(const SampleParams& p, int elem_bytes, void* scratch, cudaStream_t stream) {
+  cudaError_t e;
+  if (p.top_k == nullptr && p.top_p == nullptr && p.min_p == nullptr) {
+    Segment* segments = static_cast<Segment*>(scratch);
+    e = elem_bytes == 2 ? launch_plain<__nv_bfloat16, kVerify>(p, segments, stream)
+                        : launch_plain<float, kVerify>(p, segments, stream);
+  } else {
+    const int sms = sm_count();
+    if (sms == 0) return cuda_fail(cudaGetLastError());
+    e = elem_bytes == 2 ? launch_rows<__nv_bfloat16, kVerify>(p, sms, stream)
+                        : launch_rows<float, kVerify>(p, sms, stream);
+  }
   return e == cudaSuccess ? NVA_OK : cuda_fail(e);
 }
 
@@ -842,7 +1306,8 @@ extern "C" {
 
 NVA_API int nva_sample_tokens(const void* logits, int64_t row_stride, int32_t rows, int32_t vocab, int32_t elem_bytes,
                               const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
-                              const void* uniform, int32_t uniform_bytes, int64_t* ids, void* stream) {
+                              const void* uniform, int32_t uniform_bytes, int64_t* ids, void* workspace,
+                              size_t workspace_bytes, void* stream) {
   if (rows < 0 || vocab < 0) return NVA_ERR_INVALID_ARGUMENT;
   if ((elem_bytes != 2 && elem_bytes != 4) || (uniform_bytes != 4 && uniform_bytes != 8)) return NVA_ERR_UNSUPPORTED;
   if (rows == 0) return NVA_OK;
@@ -853,6 +1318,9 @@ NVA_API int nva_sample_tokens(const void* logits, int64_t row_stride, int32_t ro
   if (nva::misaligned(logits, static_cast<uintptr_t>(elem_bytes)) ||
       nva::misaligned(uniform, static_cast<uintptr_t>(uniform_bytes)) || nva::misaligned(ids, 8))
     return NVA_ERR_ALIGNMENT;
+  if (workspace == nullptr || workspace_bytes < nva_sample_workspace_bytes(rows, vocab, elem_bytes) ||
+      nva::misaligned(workspace, 16))
+    return NVA_ERR_WORKSPACE;
   nva::SampleParams p{};
   p.logits = logits;
   p.row_stride = row_stride;
@@ -866,11 +1334,12 @@ NVA_API int nva_sample_tokens(const void* logits, int64_t row_stride, int32_t ro
   p.uniform = uniform;
   p.uniform_bytes = uniform_bytes;
   p.ids = ids;
-  return nva::launch_sample<false>(p, elem_bytes, static_cast<cudaStream_t>(stream));
+  return nva::launch_sample<false>(p, elem_bytes, workspace, static_cast<cudaStream_t>(stream));
 }
 
-NVA_API size_t nva_verify_sampled_workspace_bytes(int32_t num_seqs, int32_t k) {
-  return num_seqs < 0 || k < 0 ? 0 : static_cast<size_t>(num_seqs) * (static_cast<size_t>(k) + 1) * sizeof(int2);
+NVA_API size_t nva_sample_workspace_bytes(int32_t rows, int32_t vocab, int32_t elem_bytes) {
+  if (rows < 0 || vocab < 0 || (elem_bytes != 2 && elem_bytes != 4)) return 0;
+  return static_cast<size_t>(rows) * sizeof(int4) + nva::segments_bytes(rows, vocab, elem_bytes);
 }
 
 NVA_API int nva_verify_sampled(const void* logits, int64_t row_stride, int32_t num_seqs, int32_t k, int32_t vocab,
@@ -897,8 +1366,8 @@ NVA_API int nva_verify_sampled(const void* logits, int64_t row_stride, int32_t n
       (k > 0 && (nva::misaligned(accept_uniform, ub) || nva::misaligned(draft_ids, ib))) ||
       nva::misaligned(num_drafts, ib) || nva::misaligned(num_accepted, ib) || nva::misaligned(next_tokens, ib))
     return NVA_ERR_ALIGNMENT;
-  if (workspace == nullptr || workspace_bytes < nva_verify_sampled_workspace_bytes(num_seqs, k) ||
-      nva::misaligned(workspace, 8))
+  if (workspace == nullptr || workspace_bytes < nva_sample_workspace_bytes(static_cast<int32_t>(rows), vocab, elem_bytes) ||
+      nva::misaligned(workspace, 16))
     return NVA_ERR_WORKSPACE;
   nva::SampleParams p{};
   p.logits = logits;
@@ -918,9 +1387,11 @@ NVA_API int nva_verify_sampled(const void* logits, int64_t row_stride, int32_t n
   p.id_bytes = id_bytes;
   p.accept_uniform = accept_uniform;
   p.accept_stride = accept_row_stride;
+  // the rows' results, then the segments (16 bytes a row: the segments stay aligned)
   p.row_result = static_cast<int2*>(workspace);
+  void* scratch = static_cast<uint8_t*>(workspace) + static_cast<size_t>(rows) * sizeof(int4);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int rc = nva::launch_sample<true>(p, elem_bytes, s);
+  const int rc = nva::launch_sample<true>(p, elem_bytes, scratch, s);
   if (rc != NVA_OK) return rc;
   const unsigned blocks = static_cast<unsigned>((num_seqs + 127) / 128);
   if (id_bytes == 4)

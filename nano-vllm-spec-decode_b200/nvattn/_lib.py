@@ -37,10 +37,10 @@ SIGNATURES = {
     "nva_varlen_attention_fp8": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _I32, _I32, _I32, _P, _P, _I32, _I32, _I32,
                                                 _P, _I32, _I32, _I32, _I32, _I32, _F, _P, _I64, _P, _SZ, _P]),
     "nva_paged_attention_fp8_workspace_bytes": (ctypes.c_size_t, [_I32, _I32, _I32, _I32]),
-    "nva_sample_tokens": (ctypes.c_int, [_P, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _I32, _P, _P]),
+    "nva_sample_tokens": (ctypes.c_int, [_P, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _I32, _P, _P, _SZ, _P]),
     "nva_verify_sampled": (ctypes.c_int, [_P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _P, _I32, _P, _P, _P, _P, _P,
                                           _I64, _P, _I32, _P, _P, _P, _SZ, _P]),
-    "nva_verify_sampled_workspace_bytes": (ctypes.c_size_t, [_I32, _I32]),
+    "nva_sample_workspace_bytes": (ctypes.c_size_t, [_I32, _I32, _I32]),
     "nva_get_device_error": (ctypes.c_int, [ctypes.POINTER(ctypes.c_uint32)]),
     "nva_clear_device_error": (ctypes.c_int, []),
 }

@@ -400,10 +400,14 @@ def sample_tokens(logits: torch.Tensor, temperatures: torch.Tensor, uniforms: to
     assert temperatures is not None and uniforms.device == logits.device
     t, k, p, m = _settings(R, logits.device, temperatures, top_k, top_p, min_p)
     ids = torch.empty(R, dtype=torch.int64, device=logits.device)
+    lib = _lib.load()
+    ws = torch.empty(lib.nva_sample_workspace_bytes(R, V, logits.element_size()), dtype=torch.uint8,
+                     device=logits.device)
     with _on(logits.device):
-        _lib.check(_lib.load().nva_sample_tokens(
+        _lib.check(lib.nva_sample_tokens(
             logits.data_ptr(), logits.stride(0) if R > 1 else max(logits.stride(0), V), R, V, logits.element_size(), t,
-            k, p, m, uniforms.data_ptr(), uniforms.element_size(), ids.data_ptr(), _stream()), "sample tokens")
+            k, p, m, uniforms.data_ptr(), uniforms.element_size(), ids.data_ptr(), ws.data_ptr(), ws.numel(),
+            _stream()), "sample tokens")
     return ids
 
 
@@ -431,14 +435,15 @@ def verify_sampled(logits: torch.Tensor, draft_ids: torch.Tensor, num_drafts: to
     acc = torch.empty(S, dtype=dt, device=logits.device)
     nxt = torch.empty(S, dtype=dt, device=logits.device)
     lib = _lib.load()
-    ws = torch.empty(S * (K + 1), 2, dtype=torch.int32, device=logits.device)
+    ws = torch.empty(lib.nva_sample_workspace_bytes(S * (K + 1), V, logits.element_size()), dtype=torch.uint8,
+                     device=logits.device)
     with _on(logits.device):
         _lib.check(lib.nva_verify_sampled(
             logits.data_ptr(), max(logits.stride(0), V), S, K, V, logits.element_size(),
             draft_ids.data_ptr() if K else 0, max(draft_ids.stride(0), K) if K else 0, num_drafts.data_ptr(),
             draft_ids.element_size(), t, k, p, m, accept_uniforms.data_ptr() if K else 0,
             max(accept_uniforms.stride(0), K) if K else 0, uniforms.data_ptr(), uniforms.element_size(),
-            acc.data_ptr(), nxt.data_ptr(), ws.data_ptr(), ws.numel() * 4, _stream()), "verify sampled")
+            acc.data_ptr(), nxt.data_ptr(), ws.data_ptr(), ws.numel(), _stream()), "verify sampled")
     return acc, nxt
 
 

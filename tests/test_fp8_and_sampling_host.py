@@ -17,6 +17,10 @@ class _Recorder:
     def nva_paged_attention_fp8_workspace_bytes(n, H, KVH, D):
         return 0 if D != 128 or H // KVH > 40 else 1 << 16
 
+    @staticmethod
+    def nva_sample_workspace_bytes(rows, vocab, elem_bytes):
+        return 32 * rows
+
     def __getattr__(self, name):
         def call(*args):
             self.calls.append((name, args))
@@ -188,19 +192,20 @@ def test_entry_points_refuse_on_the_host():
     f = lib.nva_varlen_attention_fp8
     assert f(*with_(var, a12=0)) == 0 and f(*with_(var, a13=-1)) == 1 and f(*with_(var, a9=0)) == 1
     assert f(*with_(var, a20=math.nan)) == 1 and f(*with_(var, a19=64)) == 2
-    smp = [16, 100, 3, 100, 4, 16, 0, 0, 0, 16, 4, 16, 0]
+    smp = [16, 100, 3, 100, 4, 16, 0, 0, 0, 16, 4, 16, 16, 1 << 20, 0]
     f = lib.nva_sample_tokens
     assert f(*with_(smp, a2=0)) == 0
     assert f(*with_(smp, a1=99)) == 1 and f(*with_(smp, a5=0)) == 1 and f(*with_(smp, a3=0)) == 1
     assert f(*with_(smp, a4=8)) == 2 and f(*with_(smp, a10=2)) == 2
     assert f(*with_(smp, a3=400000, a1=400000)) == 2 and f(*with_(smp, a2=(1 << 20) + 1)) == 2
     assert f(*with_(smp, a0=18)) == 3 and f(*with_(smp, a11=4)) == 3
-    ver = [16, 100, 3, 2, 100, 4, 16, 2, 16, 8, 16, 0, 0, 0, 16, 2, 16, 4, 16, 16, 16, 72, 0]
+    assert f(*with_(smp, a12=0)) == 4 and f(*with_(smp, a13=3 * 32 - 1)) == 4 and f(*with_(smp, a12=8)) == 4
+    ver = [16, 100, 3, 2, 100, 4, 16, 2, 16, 8, 16, 0, 0, 0, 16, 2, 16, 4, 16, 16, 16, 9 * 32, 0]
     f = lib.nva_verify_sampled
     assert f(*with_(ver, a2=0)) == 0
     assert f(*with_(ver, a3=-1)) == 1 and f(*with_(ver, a7=1)) == 1 and f(*with_(ver, a14=0)) == 1
-    assert f(*with_(ver, a9=2)) == 2 and f(*with_(ver, a21=71)) == 4 and f(*with_(ver, a20=0)) == 4
-    assert lib.nva_verify_sampled_workspace_bytes(3, 2) == 72
+    assert f(*with_(ver, a9=2)) == 2 and f(*with_(ver, a21=9 * 32 - 1)) == 4 and f(*with_(ver, a20=0)) == 4
+    assert lib.nva_sample_workspace_bytes(9, 100, 4) == 9 * 32 and lib.nva_sample_workspace_bytes(1, 2049, 2) == 48
 
 
 # ---------------------------------------------------------------------------------------------- restatements
