@@ -18,18 +18,22 @@
 // 1.5e-13 at most), and sums are exact 64-bit integer sums: no order of additions, atomics included, can change a result.
 // Weights below 2^-45 are 0.
 //
-// One pass over HBM: a cluster of CTAs keeps a row in its shared memory (V = 151,936 in bf16: four CTAs of 76 KB) as
-// order-preserving integer keys.  Thresholds of top-k and top-p come from histograms (counts, or fixed-point weights)
-// over 1024 bins, first of equal width in l (so that neighbouring logits rarely meet in one bin), then of the crossing
-// bin's keys until one key is left; at that key the first m equal tokens stay, in index order.  CTAs exchange maxima,
-// histograms and sums through distributed shared memory.  For the draw every thread owns a run of consecutive tokens, a
-// prefix sum over threads and CTAs names the run that holds u * W, and one warp walks it.
-// Calls without top-k, top-p and min-p need no threshold, so no row has to stay on the chip: one kernel gives a warp each
-// a segment of 4 KB, straight from registers (its maximum, then its weights' sum against that), a second one brings a
-// row's segments to one maximum, draws a segment and walks it (510 rows of 151,936: 140 us with the row in shared memory,
-// where loads, exchanges and sums of a CTA follow one another).
-// Bound: the double-precision exponentials, one per token that no threshold removes (a row with top-k only takes them
-// for the k kept ones), next to the one read of the logits.
+// Three ways, by the settings of a row (the arguments that are given, and their values on the device):
+//   * none of top-k, top-p and min-p given: no threshold, so no row has to stay on the chip.  One kernel gives a warp each
+//     a segment of 4 KB, straight from registers (its maximum, then its weights' sum against that), a second one brings a
+//     row's segments to one maximum, draws a segment and walks it.  510 rows of 151,936 in bf16: 71 us, a third of the
+//     copy bandwidth (140 us with the row in shared memory); the issue slots of the exponentials bound it.
+//   * else a cluster of CTAs keeps a row in its shared memory (V = 151,936 in bf16: four CTAs of 78 KB) -- one pass over
+//     HBM.  Where top-k or min-p leaves few tokens, the CTAs list what passes a bound, and the first of them sorts the
+//     lists and finishes alone: one row 14 us (20 with the histograms), of which loads take 1.5, the list 2.5, an
+//     exchange across the cluster 2.5, the sort and the draw 5: latency.
+//   * other rows: thresholds from histograms (counts, or fixed-point weights) over 1024 bins, first of equal width in l
+//     (so that neighbouring logits rarely meet in one bin), then of the crossing bin's keys until one key is left; at
+//     that key the first m equal tokens stay, in index order.  CTAs exchange maxima, histograms and sums through
+//     distributed shared memory.  For the draw every thread owns a run of consecutive tokens, a prefix sum over threads
+//     and CTAs names the run that holds u * W, and one warp walks it.  A row takes 30 to 45 us next to others.
+// A batch of 64 rows in fp32 with all kinds of settings takes 60 us: its rows do not fit the chip at once, and rows that
+// start second wait for shared memory.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -51,6 +55,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 1024;
 constexpr int kTable = 16;            // 128 bytes: whatever entries a warp's lanes ask for, no two meet in a bank
 constexpr int kList = 1024;            // tokens of a crossing bin kept aside per CTA
+constexpr int kRowsPerThread = 4;      // rows that the order by work goes up to, per thread
+constexpr int kShort = 2048;           // tokens that rank 0 sorts and finishes by itself
 constexpr int kMaxCluster = 8;
 constexpr float kReach = 31.5f;        // exp(-31.5) < 2^-45: weight 0
 constexpr uint32_t kAll = 0xffffffffu;
@@ -63,6 +69,7 @@ struct SampleParams {
   int32_t rows, vocab;
   int32_t run_words;                   // 32-bit words of a row per thread (odd: neighbouring threads, other banks)
   int32_t group;                       // rows that share one set of settings: 1, or k + 1 (verify)
+  int32_t by_work;                     // 1: rows start in the order of their work
   const float* temperature;
   const int32_t* top_k;
   const float* top_p;
@@ -242,14 +249,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const int rank = static_cast<int>(cluster.block_rank());
   const int ranks = static_cast<int>(cluster.num_blocks());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x / ranks;
+  int row = blockIdx.x / ranks;
 
   extern __shared__ __align__(16) uint8_t smem[];
   const int words = p.run_words * kThreads;
   uint32_t* data = reinterpret_cast<uint32_t*>(smem);
-  __shared__ __align__(16) uint32_t hist[2][kBins];          // counts, or weights: low and high words
+  // histograms (counts, or weights: low and high words); rank 0's sorted tokens of a short list
+  __shared__ __align__(16) union {
+    uint32_t hist[2][kBins];
+    u64 sorted[kShort];
+  } bins;
+  auto& hist = bins.hist;
   __shared__ double table[kTable];
-  __shared__ uint32_t list[kList];
+  __shared__ __align__(16) union {
+    uint32_t keys[kList];
+    u64 tokens[kShort];
+  } lists;
+  auto& list = lists.keys;
   __shared__ uint32_t list_count;
   __shared__ u64 scan_m[kWarps];
   __shared__ uint32_t scan_c[kWarps];
@@ -258,14 +274,46 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   __shared__ u64 found_rest;
   __shared__ uint32_t found_ties;
 
+  if (p.by_work) {
+    // Rows that no small list finishes (30 to 45 us, the others 15) first, so that none of them starts last (160 rows of
+    // verify in bf16: 77 us in their own order, 72 in this).
+    uint32_t mine = 0, long_rows;
+    u64 none = 0, none_t;
+    const int first = tid * kRowsPerThread;
+    auto is_long = [&](int r) {
+      const int s = r / p.group;
+      const int k = p.top_k != nullptr ? __ldg(p.top_k + s) : 0;
+      return r < p.rows && __ldg(p.temperature + s) > 0.f && !(k > 0 && k <= kThreads / 2) &&
+             !(p.min_p != nullptr && __ldg(p.min_p + s) > 0.f);
+    };
+    bool is[kRowsPerThread];
+#pragma unroll
+    for (int i = 0; i < kRowsPerThread; ++i) {
+      is[i] = first + i < p.rows && is_long(first + i);
+      mine += is[i] ? 1 : 0;
+    }
+    block_scan<kWarps>(none, mine, scan_m, scan_c, &none_t, &long_rows, lane, warp);
+#pragma unroll
+    for (int i = 0; i < kRowsPerThread; ++i) {
+      const int place = is[i] ? static_cast<int>(mine) : static_cast<int>(long_rows) + first + i - static_cast<int>(mine);
+      if (first + i < p.rows && place == row) found_thread = first + i;
+      mine += is[i] ? 1 : 0;
+    }
+    __syncthreads();
+    row = found_thread;
+    __syncthreads();
+  }
   const int set = row / p.group;
   const float temp = __ldg(p.temperature + set);
   const bool greedy = !(temp > 0.f);
+  int k = p.top_k != nullptr ? __ldg(p.top_k + set) : 0;
+  if (k >= p.vocab) k = 0;
+  const float bin_scale = (kBins / 32.0f) / temp;
 
   // ---------------------------------------------------------------- the row
   const int e0 = rank * words * kPer;          // first token of this CTA
   const int n = max(0, min(p.vocab - e0, words * kPer));
-  float top = -kInf;
+  float top = -kInf, cta_top, own_top = -kInf;  // the largest logit of the row, the CTA and this thread's loads
   {
     const T* src = static_cast<const T*>(p.logits) + row * p.row_stride + e0;
     const uint32_t* src32 = reinterpret_cast<const uint32_t*>(src);
@@ -314,16 +362,66 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       data[w] = keep(x) | pad;   // (-inf's bits are among the padding's NaN's)
     }
     if (tid < kTable) table[tid] = exp2(static_cast<double>(tid) / kTable + 44.0);
-    R::each(best, [&](float l, int) { top = fmaxf(top, l); });
+    R::each(best, [&](float l, int) { own_top = fmaxf(own_top, l); });
+    top = own_top;
     // as a key (NaN, which only a greedy row looks for, above +inf)
     uint32_t k = __float_as_uint(top + 0.f);
     k = nan ? kNone : (k & 0x80000000u) ? ~k : (k | 0x80000000u);
     k = __reduce_max_sync(kAll, k);
     if (lane == 0) scan_c[warp] = k;
     __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < kWarps; ++w) k = max(k, scan_c[w]);
-      ctrl.first = k;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) k = max(k, scan_c[w]);
+    if (tid == 0) ctrl.first = k;
+    cta_top = __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+  }
+  // Appends the CTA's tokens above a logit to its list (key complemented and index: ascending from the largest).
+  auto list_above = [&](float above) {
+    for (int v = tid; v < words / 4; v += kThreads) {   // (whole warps: words are a multiple of 512)
+      const uint4 x = reinterpret_cast<const uint4*>(data)[v];
+      bool any = false;
+      R::each(R::larger(R::larger(x.x, x.y), R::larger(x.z, x.w)), [&](float l, int) { any |= l > above; });
+      if (__ballot_sync(kAll, any) == 0) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        R::each(i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w, [&](float l, int h) {
+          const bool in = l > above;
+          const uint32_t vote = __ballot_sync(kAll, in);
+          if (vote == 0) return;
+          uint32_t at = 0;
+          if (lane == 0) at = atomicAdd(&list_count, static_cast<uint32_t>(__popc(vote)));
+          at = __shfl_sync(kAll, at, 0) + __popc(vote & ((1u << lane) - 1u));
+          if (in && at < kShort)
+            lists.tokens[at] = static_cast<u64>(~R::key(l)) << 32 | static_cast<uint32_t>(e0 + (v * 4 + i) * kPer + h);
+        });
+    }
+  };
+  // a little below every logit that lies in bins up to `bin` of a maximum
+  auto below_bin = [&](float max, int bin) {
+    return nextafterf(nextafterf(max - (static_cast<float>(bin) + 1.01f) / bin_scale, -kInf), -kInf);
+  };
+  // A small top-k: every CTA lists its own k largest, and whatever its bound lets through, before it knows the others'
+  // (one exchange in all instead of four).  The bound: the k-th largest of its threads' maxima, to a bin, so that 512
+  // numbers are counted and not its share of the row; about k + k^2 / 1024 tokens pass it.
+  bool listed = !greedy && k > 0 && k <= kThreads / 2 && k * ranks <= kShort / 2;
+  if (listed) {
+    for (int i = tid; i < kBins; i += kThreads) hist[0][i] = 0;
+    if (tid == 0) list_count = 0;
+    __syncthreads();
+    if (cta_top - cta_top == 0.f) {
+      if (own_top > -kInf) atomicAdd(&hist[0][min(kBins - 1, __float2int_rz((cta_top - own_top) * bin_scale))], 1u);
+      __syncthreads();
+      const uint2 c = reinterpret_cast<const uint2*>(&hist[0][0])[tid];
+      u64 none = 0, none_t;
+      uint32_t pre = c.x + c.y, tot;
+      if (tid == 0) found_ties = kBins - 1;      // (fewer maxima than k: no bound)
+      block_scan<kWarps>(none, pre, scan_m, scan_c, &none_t, &tot, lane, warp);
+      const uint32_t want = static_cast<uint32_t>(k);
+      if (pre < want && pre + c.x >= want) found_ties = 2 * tid;
+      if (pre + c.x < want && pre + c.x + c.y >= want) found_ties = 2 * tid + 1;
+      __syncthreads();
+      const int bin = static_cast<int>(found_ties);
+      list_above(bin < kBins - 1 ? below_bin(cta_top, bin) : -kInf);
     }
   }
   cluster.sync();
@@ -383,7 +481,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       });
       data[w] = x;
     }
+    own_top = own_top == top ? 0.f : -kInf;
     top = 0.f;
+    listed = false;
     __syncthreads();
   }
 
@@ -401,9 +501,65 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       if (f == f) cut = nextafterf(f, -kInf);
     }
   }
-  const float bin_scale = (kBins / 32.0f) / temp;
   auto linear_bin = [&](float l) {             // rises as the logit falls; bins of T / 32, the last takes the rest
     return min(kBins - 1, __float2int_rz((top - l) * bin_scale));
+  };
+  auto clear = [&]() {
+    for (int i = tid; i < 2 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
+    if (tid == 0) list_count = 0;
+    __syncthreads();
+  };
+  // (rank 0) the CTAs' bins together, two per thread: the first at which the target is reached, to everyone
+  auto cross = [&](auto by_weight, u64 before, bool linear, uint32_t k, double share) {
+    constexpr bool kMass = decltype(by_weight)::value;
+    if (rank == 0) {
+      u64 v[2] = {0, 0};
+      constexpr int kAtOnce = kMass ? 4 : kMaxCluster;   // CTAs' bins on their way at once
+#pragma unroll 1
+      for (int r0 = 0; r0 < ranks; r0 += kAtOnce) {
+        uint2 low[kAtOnce], high[kAtOnce];
+#pragma unroll
+        for (int r = 0; r < kAtOnce; ++r) {
+          low[r] = high[r] = make_uint2(0u, 0u);
+          if (r0 + r < ranks) {
+            const uint2* h = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[0][0], r0 + r));
+            low[r] = h[tid];
+            if constexpr (kMass) high[r] = h[kBins / 2 + tid];
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < kAtOnce; ++r) {
+          v[0] += low[r].x + (static_cast<u64>(high[r].x) << 32);
+          v[1] += low[r].y + (static_cast<u64>(high[r].y) << 32);
+        }
+      }
+      uint32_t last = 0;
+      if (!kMass && linear && warp == 0)
+        last = __reduce_add_sync(kAll, lane < ranks ? cluster.map_shared_rank(&ctrl, lane)->last : 0u);
+      u64 pre = v[0] + v[1], tot;
+      uint32_t none = 0, none_t;
+      block_scan<kWarps>(pre, none, scan_m, scan_c, &tot, &none_t, lane, warp);
+      // (the first token always stays: a target of 0 would find no crossing)
+      const double target = !linear ? ctrl.target : kMass ? fmax(share * static_cast<double>(tot), 1.0) : k;
+      auto tell = [&](uint32_t bin, u64 above) {
+        for (int r = 0; r < ranks; ++r) {
+          Control* c = cluster.map_shared_rank(&ctrl, r);
+          c->bin = bin;
+          c->before = above;
+          c->target = target;
+        }
+      };
+      pre += before;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (v[i] != 0 && static_cast<double>(pre) < target && static_cast<double>(pre + v[i]) >= target)
+          tell(static_cast<uint32_t>(2 * tid + i), pre);
+        pre += v[i];
+      }
+      if (!kMass && linear && tid == 0 && tot < k)   // not within the bins counted
+        tell(tot + last > k ? static_cast<uint32_t>(kBins - 1) : kNone, tot);
+    }
+    cluster.sync();
   };
   uint32_t kept_tokens = 0x7FFFFFFFu;          // an upper bound on the tokens kept
   // Sets the threshold to the logit at which the running count from the top reaches `k`, or the running weight `share`
@@ -417,58 +573,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       const uint32_t old = atomicAdd(&hist[0][b], x);
       const uint32_t up = static_cast<uint32_t>(v >> 32) + (old + x < old ? 1u : 0u);
       if (up != 0) atomicAdd(&hist[1][b], up);
-    };
-    auto clear = [&]() {
-      for (int i = tid; i < 2 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
-      if (tid == 0) list_count = 0;
-      __syncthreads();
-    };
-    // (rank 0) the CTAs' bins together, two per thread: the first at which the target is reached, to everyone
-    auto cross = [&](u64 before, bool linear) {
-      if (rank == 0) {
-        u64 v[2] = {0, 0};
-        uint2 low[kMaxCluster], high[kMaxCluster];   // (every CTA's bins on their way at once)
-#pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) {
-          low[r] = high[r] = make_uint2(0u, 0u);
-          if (r < ranks) {
-            const uint2* h = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[0][0], r));
-            low[r] = h[tid];
-            if constexpr (kMass) high[r] = h[kBins / 2 + tid];
-          }
-        }
-        uint32_t last = 0;
-        if (!kMass && linear && warp == 0)
-          last = __reduce_add_sync(kAll, lane < ranks ? cluster.map_shared_rank(&ctrl, lane)->last : 0u);
-#pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) {
-          v[0] += low[r].x + (static_cast<u64>(high[r].x) << 32);
-          v[1] += low[r].y + (static_cast<u64>(high[r].y) << 32);
-        }
-        u64 pre = v[0] + v[1], tot;
-        uint32_t none = 0, none_t;
-        block_scan<kWarps>(pre, none, scan_m, scan_c, &tot, &none_t, lane, warp);
-        // (the first token always stays: a target of 0 would find no crossing)
-        const double target = !linear ? ctrl.target : kMass ? fmax(share * static_cast<double>(tot), 1.0) : k;
-        auto tell = [&](uint32_t bin, u64 above) {
-          for (int r = 0; r < ranks; ++r) {
-            Control* c = cluster.map_shared_rank(&ctrl, r);
-            c->bin = bin;
-            c->before = above;
-            c->target = target;
-          }
-        };
-        pre += before;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (v[i] != 0 && static_cast<double>(pre) < target && static_cast<double>(pre + v[i]) >= target)
-            tell(static_cast<uint32_t>(2 * tid + i), pre);
-          pre += v[i];
-        }
-        if (!kMass && linear && tid == 0 && tot < k)   // not within the bins counted
-          tell(tot + last > k ? static_cast<uint32_t>(kBins - 1) : kNone, tot);
-      }
-      cluster.sync();
     };
     clear();
     uint32_t lo = R::key(floor), hi = R::key(top);   // (the threshold itself may be no bf16 number: a bound)
@@ -501,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         }
       }
       cluster.sync();
-      cross(0, true);
+      cross(by_weight, 0, true, k, share);
       if (ctrl.bin == kNone) return;
       // the crossing bin's keys: from the least with linear_bin <= bin to the last before linear_bin < bin, by 32-way
       // searches
@@ -619,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       if (kMass && rank == 0 && tid == 0 && w_floor != 0 && R::key(floor) >= lo && R::key(floor) <= hi)
         add_mass(static_cast<int>((hi - R::key(floor)) >> shift), w_floor);
       cluster.sync();
-      cross(before, false);
+      cross(by_weight, before, false, k, share);
       const uint32_t bin = ctrl.bin;
       before = ctrl.before;
       const uint32_t nhi = hi - (bin << shift);
@@ -640,14 +744,178 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     __syncthreads();   // (ctrl is read)
   };
 
-  if (p.top_k != nullptr) {
-    const int k = __ldg(p.top_k + set);
-    if (k > 0 && k < p.vocab) select(std::false_type{}, static_cast<uint32_t>(k), 0.0);
+  const float share = p.top_p != nullptr ? __ldg(p.top_p + set) : 1.f;
+
+  // (rank 0) the rest for the `count` tokens of a short list, in bins.sorted: sorts them, applies top-k and top-p, draws.
+  // Nothing is held in registers from one loop to the next: next to rows that fill the shared memory there is no L1 to
+  // spill to.
+  auto finish = [&](int count) {
+    // Ascending, n different numbers in v: every warp sorts 32 in its registers, then runs are merged in pairs into the
+    // other buffer, each number's place from a binary search of the other run (180 numbers: 1.5 us; a bitonic network in
+    // shared memory: 5).  Returns the buffer they end in.
+    auto sort = [&](u64* v, u64* other, int n) -> u64* {
+      for (int at = tid; at - lane < n; at += kThreads) {   // (whole warps)
+        u64 own = at < n ? v[at] : ~0ull;
+#pragma unroll
+        for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+          for (int j = size >> 1; j > 0; j >>= 1) {
+            const u64 y = __shfl_xor_sync(kAll, own, j);
+            const bool keep_less = ((lane & j) == 0) == ((lane & size) == 0);
+            if ((y < own) == keep_less) own = y;
+          }
+        if (at < n) v[at] = own;
+      }
+      __syncthreads();
+      for (int run = 32; run < n; run <<= 1) {
+        for (int at = tid; at < n; at += kThreads) {
+          const u64 own = v[at];
+          const int start = (at & -run) ^ run, length = min(run, n - start);
+          int less = 0;
+          if (length > 0) {
+            for (int step = run; step > 0; step >>= 1) {
+              const int to = less + step;
+              const u64 x = v[start + min(to, length) - 1];
+              less = to <= length && x < own ? to : less;
+            }
+          }
+          other[(at & -(2 * run)) + (at & (run - 1)) + less] = own;
+        }
+        u64* const t = v;
+        v = other;
+        other = t;
+        __syncthreads();
+      }
+      return v;
+    };
+    u64* const weights = reinterpret_cast<u64*>(data);   // (this CTA's share of the row has been searched)
+    u64* a = sort(bins.sorted, lists.tokens, count);
+    const int kept_k = k > 0 ? min(k, count) : count;
+    const int per_thread = (count + kThreads - 1) / kThreads;   // positions of a thread, side by side
+    const int first = min(tid * per_thread, count), last = min(first + per_thread, count);
+    u64 sum = 0, total, none64;
+    uint32_t none = 0, none_t;
+    for (int at = first; at < last; ++at) {
+      const float l = R::value(static_cast<uint32_t>(~(a[at] >> 32)));
+      const u64 w = at < kept_k && l > cut ? weight(l) : 0ull;
+      weights[at] = w;
+      sum += w;
+    }
+    u64 before = sum;
+    block_scan<kWarps>(before, none, scan_m, scan_c, &total, &none_t, lane, warp);
+    int kept = kept_k;
+    if (share < 1.f) {
+      const double target = fmax(static_cast<double>(fmaxf(share, 0.f)) * static_cast<double>(total), 1.0);
+      uint32_t n = 0;
+      sum = 0;
+      for (int at = first; at < last; ++at) {
+        if (at >= kept_k || !(static_cast<double>(before) < target)) break;
+        before += weights[at];
+        sum += weights[at];
+        ++n;
+      }
+      block_scan<kWarps>(sum, n, scan_m, scan_c, &total, &none_t, lane, warp);
+      kept = static_cast<int>(none_t);
+    }
+    // the kept ones in the order of their indices
+    if (tid == 0) found_rest = 0;
+    __syncthreads();
+    for (int at = tid; at < kept; at += kThreads) {
+      const uint32_t token = static_cast<uint32_t>(a[at]);
+      a[at] = static_cast<u64>(token) << 32 | static_cast<uint32_t>(at);
+      if (kVerify && static_cast<int>(token) == draft) found_rest = weights[at];
+    }
+    __syncthreads();
+    bool accepted = false;
+    if constexpr (kVerify) {
+      const u64 draft_w = found_rest;
+      if (draft >= 0) {
+        const double ua = read_uniform(p.accept_uniform, set * p.accept_stride + (row - set * p.group), p.uniform_bytes);
+        accepted = ua * static_cast<double>(total) < static_cast<double>(draft_w);
+      }
+      total -= draft_w;
+    }
+    a = sort(a, a == bins.sorted ? lists.tokens : bins.sorted, kept);
+    auto weight_at = [&](int at) {
+      const u64 x = a[at];
+      return kVerify && static_cast<int>(x >> 32) == draft ? 0ull : weights[x & 0xFFFFFFFFull];
+    };
+    const int begin = min(first, kept), end = min(last, kept);
+    sum = 0;
+    for (int at = begin; at < end; ++at) sum += weight_at(at);
+    u64 run = sum;
+    block_scan<kWarps>(run, none, scan_m, scan_c, &none64, &none_t, lane, warp);
+    const double un = read_uniform(p.uniform, set, p.uniform_bytes);
+    u64 want = static_cast<u64>(un * static_cast<double>(total));
+    if (total > 0 && want >= total) want = total - 1;
+    if (want >= run && want - run < sum) {
+      int at = begin;
+      for (u64 rest = want - run; at < end - 1; ++at) {
+        const u64 w = weight_at(at);
+        if (rest < w) break;
+        rest -= w;
+      }
+      const int token = static_cast<int>(a[at] >> 32);
+      if constexpr (kVerify) {
+        p.row_result[row] = make_int2(token, accepted ? 1 : 0);
+      } else {
+        p.ids[row] = token;
+      }
+    }
+    if (kVerify && total == 0 && tid == 0)   // nothing but the (then accepted) draft
+      p.row_result[row] = make_int2(draft, accepted ? 1 : 0);
+  };
+
+  // Few tokens left by min-p or a top-k: rank 0 takes them all, sorts them (by logit, then index) and finishes alone.  A
+  // bound that a larger top-k keeps: as above, over all the CTAs' threads.  (64 rows of 151,936 in fp32, mixed settings:
+  // 76 us with the histograms below for every row, 60 with the lists.)
+  if ((k > 0 && k <= kShort) || cut > -kInf) {
+    for (;;) {
+      if (!listed) {
+        float above = cut;
+        clear();
+        if (k > 0 && k <= kShort) {
+          if (own_top > cut) atomicAdd(&hist[0][linear_bin(own_top)], 1u);
+          if (tid == 0) ctrl.last = 0;
+          cluster.sync();
+          cross(std::false_type{}, 0, true, static_cast<uint32_t>(k), 0.0);
+          const uint32_t bin = ctrl.bin;
+          if (bin < kBins - 1) above = fmaxf(cut, below_bin(top, static_cast<int>(bin)));   // (else too few maxima)
+        }
+        list_above(above);
+        cluster.sync();
+      }
+      const uint32_t mine = lane < ranks ? *cluster.map_shared_rank(&list_count, lane) : 0u;
+      const uint32_t count = __reduce_add_sync(kAll, mine);
+      const uint32_t longest = __reduce_max_sync(kAll, mine);
+      if (longest <= kShort && count <= kShort) {
+        if (rank == 0) {
+          for (int i = tid; i - lane < static_cast<int>(count); i += kThreads) {
+            int from = -1, place = 0;
+            uint32_t first = 0;
+            for (int r = 0; r < ranks; ++r) {
+              const uint32_t c = __shfl_sync(kAll, mine, r);
+              if (static_cast<uint32_t>(i) >= first && static_cast<uint32_t>(i) < first + c) {
+                from = r;
+                place = i - static_cast<int>(first);
+              }
+              first += c;
+            }
+            if (from >= 0) bins.sorted[i] = cluster.map_shared_rank(&lists.tokens[0], from)[place];
+          }
+        }
+        cluster.sync();   // the lists are read: the other CTAs are done
+        if (rank == 0) finish(static_cast<int>(count));
+        return;
+      }
+      cluster.sync();     // (list_count is read)
+      if (!listed) break;
+      listed = false;     // too many tokens near a CTA's k-th: once more with a bound from all of them
+    }
   }
-  if (p.top_p != nullptr) {
-    const double tp = __ldg(p.top_p + set);
-    if (tp < 1.0) select(std::true_type{}, 0, fmax(tp, 0.0));
-  }
+
+  if (k > 0) select(std::false_type{}, static_cast<uint32_t>(k), 0.0);
+  if (share < 1.f) select(std::true_type{}, 0, static_cast<double>(fmaxf(share, 0.f)));
 
   // ---------------------------------------------------------------- the draw
   // kept weight of this thread's run, of the runs and CTAs before it, and of all
@@ -759,7 +1027,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     const int count = p.run_words * kPer;
     u64 rest = found_rest;
     uint32_t seen = found_ties;
-    int last = 0;          // the last token with a weight: the tokens' rounded weights may end just short of the run's sum
+    int last = -1;         // the last token with a weight: the tokens' rounded weights may end just short of the run's sum
+    uint32_t best = 0;     // (a run of parts below 2^-44 each: its largest)
+    int best_token = 0;
     for (int base = 0; base < count; base += 32) {
       const int e = base + lane;
       float l = __int_as_float(0x7FFFFFFF);
@@ -771,6 +1041,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       u64 v = l > cut ? weight(l) : tie_kept ? w_cut : 0ull;
       const int token = e0 + first_word * kPer + e;
       if (kVerify && token == draft) v = 0;
+      const uint32_t key = l > -kInf && !(kVerify && token == draft) ? R::key(l) : 0u;
+      const uint32_t most = __reduce_max_sync(kAll, key);
+      if (most > best) {
+        best = most;
+        best_token = __shfl_sync(kAll, token, __ffs(__ballot_sync(kAll, key == most)) - 1);
+      }
       u64 x = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -783,6 +1059,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       rest -= __shfl_sync(kAll, x, 31);
       seen += __popc(tie_vote);
     }
+    if (last < 0) last = best != 0 ? best_token : draft;
     if (lane == 0) {
       if constexpr (kVerify) {
         p.row_result[row] = make_int2(last, accepted ? 1 : 0);
@@ -808,10 +1085,10 @@ static_assert(sizeof(Segment) == 16, "Segment");
 
 // The same weights, two at a time, for sums that start at a segment's maximum: the argument 16 log2(e) l / T is reduced in
 // single precision with its rounding error carried along (u = n + q, |q| <= 1/2, from the constant's two parts), the
-// maximum's own n and q taken off, so that its weight is 1.  Rounding q and the series leaves 2e-9 of a token's weight,
-// either way and different from token to token; the products with the table, and the sums, are in double precision.
+// maximum's own q taken off, so that its weight is 1.  Rounding q and the series leaves 2e-9 of a token's weight, either
+// way and different from token to token; the products with the table, and the sums, are in double precision.
 // Needs |16 log2(e) l / T| < 2^20.  One double-precision multiply-add and one sum per token instead of eleven operations
-// (510 rows of 151,936: 112 -> 83 us together with the smaller draw blocks).
+// (the segments of 510 rows of 151,936: 86 -> 63 us).
 struct PairWeight {
   float c, lo, q0, zero;
   double one;                    // 1 / the maximum's weight as `sum` has it
@@ -996,7 +1273,7 @@ __global__ void __launch_bounds__(256, 4) segment_kernel(const SampleParams p, S
 }
 
 // One block per row; a thread holds up to four neighbouring segments (blocks of one segment a thread, 512 threads, took one
-// SM each: 30 us for 510 rows instead of 12).
+// SM each: 30 us for 510 rows instead of 9).
 constexpr int kDrawThreads = 128;
 constexpr int kDrawWarps = kDrawThreads / 32;
 constexpr int kDrawSegments = 4;
@@ -1239,15 +1516,16 @@ template <typename T, bool kVerify>
 cudaError_t launch_rows(SampleParams p, int sms, cudaStream_t stream) {
   constexpr int kPer = Row<T>::kPerWord;
   const int words = (p.vocab + kPer - 1) / kPer;
-  // CTAs per row: a share of at most 80 KB, so that two CTAs fit an SM and one row's exchange runs beside another's
+  // CTAs per row: a share of at most 78 KB, so that two CTAs fit an SM and one row's exchange runs beside another's
   // loads; more of them when there are few rows (but at least 4 KB each)
   int cluster = 1;
   while (cluster < kMaxCluster &&
-         (words > cluster * 20480 || (static_cast<int64_t>(p.rows) * cluster * 2 <= 2 * sms && words >= cluster * 2048)))
+         (words > cluster * 38 * kThreads || (static_cast<int64_t>(p.rows) * cluster * 2 <= 2 * sms && words >= cluster * 2048)))
     cluster *= 2;
   const int per_cta = (words + cluster - 1) / cluster;
   p.run_words = ((per_cta + kThreads - 1) / kThreads) | 1;
-  const size_t smem = static_cast<size_t>(p.run_words) * kThreads * 4;
+  p.by_work = static_cast<int64_t>(p.rows) * cluster > 2 * sms && p.rows <= kRowsPerThread * kThreads ? 1 : 0;
+  const size_t smem = std::max(static_cast<size_t>(p.run_words) * kThreads * 4, kShort * sizeof(u64));
   auto kernel = sample_kernel<T, kVerify>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;

@@ -121,6 +121,37 @@ def test_infinities_nan_and_masks(cuda, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("k", [1, 2, 31, 33, 127, 129, 256, 257, 513, 1000, 1900, 2047, 2049, 5000])
+@pytest.mark.parametrize("V", [700, 2500, 40001])
+def test_short_lists(cuda, V, k, dtype):
+    """Around the sizes at which a top-k goes from one list to the next, with equal logits that overflow them."""
+    R = 8
+    x, g = rows(R, V, dtype, V + k)
+    x[1] = x[1].round()                                    # some tens of values
+    x[2] = (x[2] > 2).to(dtype)                            # two values
+    x[3] = 1.5
+    x[4, V // 2:] = float("-inf")
+    x[5, : V - 20] = x[5, : V - 20].sort(descending=True)[0]   # every large one in one place
+    x[6, ::7] = 30.0
+    u = torch.rand(R, generator=g)
+    t = torch.rand(R, generator=g) + 0.3
+    top_k = torch.full((R,), k).int()
+    check(x, t, u, top_k=top_k)
+    check(x, t, u, top_k=top_k, top_p=torch.rand(R, generator=g), min_p=torch.rand(R, generator=g) * 1e-3)
+    check(x, t, u, top_p=torch.rand(R, generator=g), min_p=torch.rand(R, generator=g) * 1e-6)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_more_rows_than_start_at_once(cuda, dtype):
+    """Rows begin in the order of their work there, each with its own settings."""
+    R, V = 700, 5001
+    x, g = rows(R, V, dtype, 12)
+    pick = lambda xs: torch.tensor(xs)[torch.randint(len(xs), (R,), generator=g)]  # noqa: E731
+    check(x, pick([0.0, 0.7, 1.0]), torch.rand(R, generator=g), top_k=pick([0, 0, 20, 400]).int(),
+          top_p=pick([0.5, 0.9, 1.0]), min_p=pick([0.0, 0.0, 0.05]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("t", [1e-3, 1e-6, 1e-9, 1e-20, 1e-38, 1.0])
 @pytest.mark.parametrize("scale", [1.0, 1e4, 1e10, 1e37])
 def test_steps_of_the_type_against_the_temperature(cuda, dtype, t, scale):
