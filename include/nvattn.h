@@ -277,7 +277,8 @@ NVA_API int nva_verify_sampled(const void* logits, int64_t row_stride, int32_t n
                                const void* accept_uniform, int64_t accept_row_stride, const void* uniform,
                                int32_t uniform_bytes, void* num_accepted, void* next_tokens, void* workspace,
                                size_t workspace_bytes, void* stream);
-/* Workspace of both calls (16-byte aligned); rows: the rows of logits. */
+/* Workspace of both calls (16-byte aligned); rows: the rows of logits.  Where any of top_k, top_p and min_p is given,
+ * nva_sample_tokens needs none and nva_verify_sampled 16 bytes a row. */
 NVA_API size_t nva_sample_workspace_bytes(int32_t rows, int32_t vocab, int32_t elem_bytes);
 
 /*

@@ -1596,8 +1596,9 @@ NVA_API int nva_sample_tokens(const void* logits, int64_t row_stride, int32_t ro
   if (nva::misaligned(logits, static_cast<uintptr_t>(elem_bytes)) ||
       nva::misaligned(uniform, static_cast<uintptr_t>(uniform_bytes)) || nva::misaligned(ids, 8))
     return NVA_ERR_ALIGNMENT;
-  if (workspace == nullptr || workspace_bytes < nva_sample_workspace_bytes(rows, vocab, elem_bytes) ||
-      nva::misaligned(workspace, 16))
+  if (top_k == nullptr && top_p == nullptr && min_p == nullptr &&
+      (workspace == nullptr || workspace_bytes < nva_sample_workspace_bytes(rows, vocab, elem_bytes) ||
+       nva::misaligned(workspace, 16)))
     return NVA_ERR_WORKSPACE;
   nva::SampleParams p{};
   p.logits = logits;
@@ -1644,7 +1645,9 @@ NVA_API int nva_verify_sampled(const void* logits, int64_t row_stride, int32_t n
       (k > 0 && (nva::misaligned(accept_uniform, ub) || nva::misaligned(draft_ids, ib))) ||
       nva::misaligned(num_drafts, ib) || nva::misaligned(num_accepted, ib) || nva::misaligned(next_tokens, ib))
     return NVA_ERR_ALIGNMENT;
-  if (workspace == nullptr || workspace_bytes < nva_sample_workspace_bytes(static_cast<int32_t>(rows), vocab, elem_bytes) ||
+  if (workspace == nullptr || workspace_bytes < (top_k != nullptr || top_p != nullptr || min_p != nullptr
+                             ? static_cast<size_t>(rows) * sizeof(int4)
+                             : nva_sample_workspace_bytes(static_cast<int32_t>(rows), vocab, elem_bytes)) ||
       nva::misaligned(workspace, 16))
     return NVA_ERR_WORKSPACE;
   nva::SampleParams p{};

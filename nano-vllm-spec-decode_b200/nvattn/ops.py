@@ -22,13 +22,18 @@ from . import _lib
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current device's current stream (its number alone: a Stream object costs 3 us more a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _on(device: torch.device):
     """The context in which `device` is the current one (nothing to do when it already is)."""
-    if device.type != "cuda" or device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        return _HERE
     return torch.cuda.device(device)
 
 
@@ -376,12 +381,12 @@ def shard_accept(keys: torch.Tensor, draft_ids: torch.Tensor, num_drafts: torch.
 
 def _settings(rows: int, device, temperatures, top_k, top_p, min_p):
     """Checks the per-row sampling settings; returns their pointers (0: off)."""
-    out = []
+    shape, out = (rows,), []
     for x, dt in ((temperatures, torch.float32), (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32)):
         if x is None:
             out.append(0)
             continue
-        assert x.dtype == dt and x.shape == (rows,) and x.is_contiguous() and x.device == device
+        assert x.dtype is dt and x.shape == shape and x.is_contiguous() and x.device == device
         out.append(x.data_ptr())
     return out
 
@@ -401,13 +406,15 @@ def sample_tokens(logits: torch.Tensor, temperatures: torch.Tensor, uniforms: to
     t, k, p, m = _settings(R, logits.device, temperatures, top_k, top_p, min_p)
     ids = torch.empty(R, dtype=torch.int64, device=logits.device)
     lib = _lib.load()
-    ws = torch.empty(lib.nva_sample_workspace_bytes(R, V, logits.element_size()), dtype=torch.uint8,
-                     device=logits.device)
+    ws, ws_bytes = None, 0
+    if not (k or p or m):
+        ws_bytes = lib.nva_sample_workspace_bytes(R, V, logits.element_size())
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device)
     with _on(logits.device):
         _lib.check(lib.nva_sample_tokens(
             logits.data_ptr(), logits.stride(0) if R > 1 else max(logits.stride(0), V), R, V, logits.element_size(), t,
-            k, p, m, uniforms.data_ptr(), uniforms.element_size(), ids.data_ptr(), ws.data_ptr(), ws.numel(),
-            _stream()), "sample tokens")
+            k, p, m, uniforms.data_ptr(), uniforms.element_size(), ids.data_ptr(), ws.data_ptr() if ws_bytes else 0,
+            ws_bytes, _stream()), "sample tokens")
     return ids
 
 
@@ -432,18 +439,18 @@ def verify_sampled(logits: torch.Tensor, draft_ids: torch.Tensor, num_drafts: to
     assert temperatures is not None
     assert logits.device == draft_ids.device == num_drafts.device == accept_uniforms.device == uniforms.device
     t, k, p, m = _settings(S, logits.device, temperatures, top_k, top_p, min_p)
-    acc = torch.empty(S, dtype=dt, device=logits.device)
-    nxt = torch.empty(S, dtype=dt, device=logits.device)
+    acc, nxt = torch.empty_like(num_drafts), torch.empty_like(num_drafts)
     lib = _lib.load()
-    ws = torch.empty(lib.nva_sample_workspace_bytes(S * (K + 1), V, logits.element_size()), dtype=torch.uint8,
-                     device=logits.device)
+    ws_bytes = (16 * logits.shape[0] if k or p or m
+                else lib.nva_sample_workspace_bytes(logits.shape[0], V, logits.element_size()))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device)
     with _on(logits.device):
         _lib.check(lib.nva_verify_sampled(
             logits.data_ptr(), max(logits.stride(0), V), S, K, V, logits.element_size(),
             draft_ids.data_ptr() if K else 0, max(draft_ids.stride(0), K) if K else 0, num_drafts.data_ptr(),
             draft_ids.element_size(), t, k, p, m, accept_uniforms.data_ptr() if K else 0,
             max(accept_uniforms.stride(0), K) if K else 0, uniforms.data_ptr(), uniforms.element_size(),
-            acc.data_ptr(), nxt.data_ptr(), ws.data_ptr(), ws.numel(), _stream()), "verify sampled")
+            acc.data_ptr(), nxt.data_ptr(), ws.data_ptr(), ws_bytes, _stream()), "verify sampled")
     return acc, nxt
 
 
