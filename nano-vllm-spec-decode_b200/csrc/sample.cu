@@ -504,6 +504,44 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   auto linear_bin = [&](float l) {             // rises as the logit falls; bins of T / 32, the last takes the rest
     return min(kBins - 1, __float2int_rz((top - l) * bin_scale));
   };
+  // Ascending, n different numbers in v: every warp sorts 32 in its registers, then runs are merged in pairs into the
+  // other buffer, each number's place from a binary search of the other run (180 numbers: 1.5 us; a bitonic network in
+  // shared memory: 5).  Returns the buffer they end in.
+  auto sort = [&](u64* v, u64* other, int n) -> u64* {
+    for (int at = tid; at - lane < n; at += kThreads) {   // (whole warps)
+      u64 own = at < n ? v[at] : ~0ull;
+#pragma unroll
+      for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int j = size >> 1; j > 0; j >>= 1) {
+          const u64 y = __shfl_xor_sync(kAll, own, j);
+          const bool keep_less = ((lane & j) == 0) == ((lane & size) == 0);
+          if ((y < own) == keep_less) own = y;
+        }
+      if (at < n) v[at] = own;
+    }
+    __syncthreads();
+    for (int run = 32; run < n; run <<= 1) {
+      for (int at = tid; at < n; at += kThreads) {
+        const u64 own = v[at];
+        const int start = (at & -run) ^ run, length = min(run, n - start);
+        int less = 0;
+        if (length > 0) {
+          for (int step = run; step > 0; step >>= 1) {
+            const int to = less + step;
+            const u64 x = v[start + min(to, length) - 1];
+            less = to <= length && x < own ? to : less;
+          }
+        }
+        other[(at & -(2 * run)) + (at & (run - 1)) + less] = own;
+      }
+      u64* const t = v;
+      v = other;
+      other = t;
+      __syncthreads();
+    }
+    return v;
+  };
   auto clear = [&]() {
     for (int i = tid; i < 2 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
     if (tid == 0) list_count = 0;
@@ -642,54 +680,70 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         });
     }
     if (lo < hi) {
-      // Few tokens in all: rank 0 takes everyone's, one per thread, and each thread adds up what lies above its token
-      // and what equals it.
+      // Few tokens in all: rank 0 takes everyone's, sorts them and runs along them to the target.
       cluster.sync();
       const uint32_t mine = lane < ranks ? *cluster.map_shared_rank(&list_count, lane) : 0u;
       const uint32_t all = __reduce_add_sync(kAll, mine);
       const uint32_t longest = __reduce_max_sync(kAll, mine);
-      if (all + 1 <= kThreads && longest <= kList) {
+      if (all + 1 <= kShort && longest <= kList) {
         if (rank == 0) {
-          uint32_t* keys = &hist[0][0];                                     // (the histogram has been read)
-          u64* masses = reinterpret_cast<u64*>(&hist[1][0]);
-          uint32_t first = 0, key = 0;
-          u64 v = 0;
-          int from = -1, place = 0;           // the CTA whose list holds this thread's token, and where
-          for (int r = 0; r < ranks; ++r) {
-            const uint32_t c = __shfl_sync(kAll, mine, r);
-            if (static_cast<uint32_t>(tid) >= first && static_cast<uint32_t>(tid) < first + c) {
-              from = r;
-              place = tid - static_cast<int>(first);
+          int count = static_cast<int>(all);
+          for (int i = tid; i - lane < count; i += kThreads) {   // (bins.sorted: the histogram has been read)
+            int from = -1, place = 0;         // the CTA whose list holds token i, and where
+            uint32_t first = 0;
+            for (int r = 0; r < ranks; ++r) {
+              const uint32_t c = __shfl_sync(kAll, mine, r);
+              if (static_cast<uint32_t>(i) >= first && static_cast<uint32_t>(i) < first + c) {
+                from = r;
+                place = i - static_cast<int>(first);
+              }
+              first += c;
             }
-            first += c;
+            if (from >= 0)
+              bins.sorted[i] = static_cast<u64>(~cluster.map_shared_rank(&list[0], from)[place]) << 32 |
+                               static_cast<uint32_t>(i);
           }
-          if (from >= 0) key = cluster.map_shared_rank(&list[0], from)[place];
-          if (key != 0) v = kMass ? weight(R::value(key)) : 1ull;
-          if (kMass && static_cast<uint32_t>(tid) == all && w_floor != 0 && R::key(floor) >= lo && R::key(floor) <= hi) {
-            key = R::key(floor);
-            v = w_floor;
+          if (kMass && w_floor != 0 && R::key(floor) >= lo && R::key(floor) <= hi) {   // the equals of the floor, as one
+            if (tid == 0) bins.sorted[count] = static_cast<u64>(~R::key(floor)) << 32 | kNone;
+            ++count;
           }
-          keys[tid] = key;
-          if constexpr (kMass) masses[tid] = v;
+          if (tid == 0) found_thread = -1;
           __syncthreads();
-          u64 above = before, same = 0, sum = 0;
-          const int count = static_cast<int>(all) + (kMass ? 1 : 0);
-          if (v != 0)
-            for (int i = 0; i < count; ++i) {
-              const uint32_t k = keys[i];
-              const u64 x = kMass ? masses[i] : 1ull;
-              above += k > key ? x : 0ull;
-              same += k == key ? x : 0ull;
-              sum += x;
+          const u64* a = sort(bins.sorted, lists.tokens, count);
+          const int per_thread = (count + kThreads - 1) / kThreads;
+          const int begin = min(tid * per_thread, count), end = min(begin + per_thread, count);
+          auto mass = [&](u64 x) -> u64 {
+            if constexpr (!kMass) return 1ull;
+            return static_cast<uint32_t>(x) == kNone ? w_floor : weight(R::value(static_cast<uint32_t>(~(x >> 32))));
+          };
+          u64 sum = 0, tot;
+          for (int i = begin; i < end; ++i) sum += mass(a[i]);
+          u64 above = sum;
+          uint32_t none = 0, none_t;
+          block_scan<kWarps>(above, none, scan_m, scan_c, &tot, &none_t, lane, warp);
+          above += before;
+          const double target = direct ? fmax(share * static_cast<double>(tot), 1.0) : ctrl.target;
+          u64 run = above;
+          for (int i = begin; i < end; ++i) {
+            const u64 to = run + mass(a[i]);
+            if (static_cast<double>(run) < target && static_cast<double>(to) >= target) found_thread = i;
+            run = to;
+          }
+          __syncthreads();
+          if (found_thread >= 0) {
+            const uint32_t key = static_cast<uint32_t>(a[found_thread] >> 32);   // (complemented)
+            run = above;
+            for (int i = begin; i < end; ++i) {
+              if (static_cast<uint32_t>(a[i] >> 32) == key && (i == 0 || static_cast<uint32_t>(a[i - 1] >> 32) != key))
+                for (int r = 0; r < ranks; ++r) {   // the first of the equals: what lies above them
+                  Control* c = cluster.map_shared_rank(&ctrl, r);
+                  c->bin = ~key;
+                  c->before = run;
+                  c->target = target;
+                }
+              run += mass(a[i]);
             }
-          const double target = direct ? fmax(share * static_cast<double>(sum), 1.0) : ctrl.target;
-          if (v != 0 && static_cast<double>(above) < target && static_cast<double>(above + same) >= target)
-            for (int r = 0; r < ranks; ++r) {   // (equal tokens say the same)
-              Control* c = cluster.map_shared_rank(&ctrl, r);
-              c->bin = key;
-              c->before = above;
-              c->target = target;
-            }
+          }
         }
         cluster.sync();
         lo = hi = ctrl.bin;
@@ -750,44 +804,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   // Nothing is held in registers from one loop to the next: next to rows that fill the shared memory there is no L1 to
   // spill to.
   auto finish = [&](int count) {
-    // Ascending, n different numbers in v: every warp sorts 32 in its registers, then runs are merged in pairs into the
-    // other buffer, each number's place from a binary search of the other run (180 numbers: 1.5 us; a bitonic network in
-    // shared memory: 5).  Returns the buffer they end in.
-    auto sort = [&](u64* v, u64* other, int n) -> u64* {
-      for (int at = tid; at - lane < n; at += kThreads) {   // (whole warps)
-        u64 own = at < n ? v[at] : ~0ull;
-#pragma unroll
-        for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-          for (int j = size >> 1; j > 0; j >>= 1) {
-            const u64 y = __shfl_xor_sync(kAll, own, j);
-            const bool keep_less = ((lane & j) == 0) == ((lane & size) == 0);
-            if ((y < own) == keep_less) own = y;
-          }
-        if (at < n) v[at] = own;
-      }
-      __syncthreads();
-      for (int run = 32; run < n; run <<= 1) {
-        for (int at = tid; at < n; at += kThreads) {
-          const u64 own = v[at];
-          const int start = (at & -run) ^ run, length = min(run, n - start);
-          int less = 0;
-          if (length > 0) {
-            for (int step = run; step > 0; step >>= 1) {
-              const int to = less + step;
-              const u64 x = v[start + min(to, length) - 1];
-              less = to <= length && x < own ? to : less;
-            }
-          }
-          other[(at & -(2 * run)) + (at & (run - 1)) + less] = own;
-        }
-        u64* const t = v;
-        v = other;
-        other = t;
-        __syncthreads();
-      }
-      return v;
-    };
     u64* const weights = reinterpret_cast<u64*>(data);   // (this CTA's share of the row has been searched)
     u64* a = sort(bins.sorted, lists.tokens, count);
     const int kept_k = k > 0 ? min(k, count) : count;
