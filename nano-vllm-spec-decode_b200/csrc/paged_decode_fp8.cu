@@ -16,8 +16,7 @@
 //        (0.12% rms, bf16's rounding is 0.16%) and never below 2^-17 where the row's largest is 2^8 to 2^11, so tokens
 //        down to 2^-25 of the largest weight still count.  Sums of weights stay in float32, unrounded.
 //
-// Bound: HBM, one byte per cached value (decode of 64 sequences, contexts 512 to 4096: 303 MB, 46 us at the measured
-// copy rate).  A 128-token tile then takes 0.74 us of an SM's share of the bandwidth, half of the bf16 cache's, which is
+// Bound: HBM, one byte per cached value (decode of 64 sequences, contexts 512 to 4096: 303 MB, 46 us at the copy rate).  A 128-token tile then takes 0.74 us of an SM's share of the bandwidth, half of the bf16 cache's, which is
 // less than one tile's chain S -> weights -> PV takes; so two CTAs share an SM and their chains overlap.
 //
 // Orientation, roles and the merge of split segments are those of paged_decode.cu: tokens on the TMEM lanes (UMMA M),
@@ -25,10 +24,17 @@
 // K tile: K-major, 128-byte swizzle, 128 dims = one swizzle row.  V tile: the same bytes read MN-major.  P^T: MN-major
 // without swizzle, 16 rows of a token per 16 bytes.
 //
-// Work split: every CTA owns an equal share of cost positions (tiles + 3 per segment) in (sequence, piece, kv head,
-// tile) order, where a piece is a run of at most max_n queries of a sequence: a prefill chunk is walked piece by piece,
-// each over the keys its last query sees.  A CTA finds its start with one scan over the lengths and walks on from there,
-// so there is no table of sequences on the chip and no bound on their number.
+// Work split: heads go in sets of 8 (or 4, 2, 1) that as many CTAs walk side by side, tile for tile, so that the rows of
+// a token, 128 bytes a head, are fetched as the 1 KB that lies together (contexts of 50,000 of 8 sequences: 201 us a head
+// alone, 135 in sets; short ones 28.0 and 28.8).  Every set owns an equal share of cost positions (tiles + 3 per segment)
+// in (sequence, piece, set, tile) order, where a piece is a run of at most max_n queries of a sequence: a longer run is
+// walked piece by piece, each over the keys its last query sees, up to where the prefill kernel takes it (kMinPrefillRun).
+// A set finds its start with one scan over the lengths and walks on from there, so there is no table of sequences on the
+// chip and no bound on their number.
+//
+// Measured (32 q heads over 8, copy rate 6.57 TB/s): decode of 64 sequences of 512 to 4096 62 us (75%), of 8192 168 us
+// (97%), 8 of 40,000 to 65,536 139 us (95%); verify of 32 sequences of 256 to 2048, k = 4, 40 us; 4 sequences of 37 to
+// 1000 18 us, of which the start takes 6, the tiles 5 and the ends 5; 256 single queries with three prefill chunks 265 us.
 #include <algorithm>
 #include <cuda_fp8.h>
 
@@ -52,8 +58,8 @@ constexpr float kSlack = 3.0f;          // ... and may pass it by this much (log
 constexpr float kWeightMax = 2048.0f;   // 2^(kBase + kSlack): lo <= 2^-3 w stays inside e4m3's range
 
 // NR: the most query rows a softmax thread carries.  One softmax group of 128 threads at 128 registers each: at 40 rows
-// (weights and sums of 40 rows, 80 registers) nothing spills; at 48, or with two groups of 80-register threads, rows
-// spill past an L1 that two CTAs' shared memory leaves next to nothing, and a tile took four times as long.
+// (weights and sums of 40 rows, 80 registers) nothing spills; with more rows they spill past an L1 that two CTAs' shared
+// memory leaves next to nothing, and a tile takes four times as long.
 template <int NR>
 struct Cfg8 {
   static constexpr int kThreads = kConsumerBase + 128;
@@ -1190,12 +1196,33 @@ int tile_rows(int64_t rows) {
   return rows <= 8 ? 8 : rows >= kMaxRows8 ? kMaxRows8 : static_cast<int>((rows + 7) / 8 * 8);
 }
 
-// Whether a varlen call of that row count takes the kernel for mixed lengths (pieces of 32 rows, 8-row runs apart).
-bool mixed_lengths(int nr, int group) { return nr > 16 && group <= 32; }
+// Query runs of at least this many tokens take the prefill kernel, which gives each q head 128 rows of its own and costs
+// the same for 33 queries as for 128, while here every 32 packed rows are walked anew.  32 q heads over 8, here and there:
+// 4 runs of 64 over 1000 keys 45 and 35 us, 32 such runs 219 and 152, 8 over 8000 keys 239 and 277; runs of 48: 40 and 35,
+// 164 and 150, 184 and 276; runs of 80: 49 and 36, 267 and 153, 293 and 281.
+constexpr int kMinPrefillRun = 64;
+
+// Whether a varlen call of that row count may take the kernel for mixed lengths (pieces of 32 rows, 8-row runs apart).
+bool may_mix(int nr, int group) { return nr > 16 && group <= 32; }
+
+// Whether it does.  The other kernels give every run the rows of the longest, this one splits its work twice and merges
+// more; it pays where single queries outnumber the long runs' pieces, as the totals tell if all long runs are alike (runs
+// for the prefill kernel count as none).  Single queries + long runs over 2000 keys, 32 q heads over 8, mixed and not:
+// 32 + 2 x 60 93 and 81 us, 48 + 2 x 60 102 and 100, 64 + 2 x 60 112 and 122, 96 + 2 x 60 133 and 158, 256 + 16 x 20 299
+// and 378, 128 + 16 x 9 164 and 205; with the narrower rows of k = 4, 128 + 16 x 5 152 and 146, 256 + 2 x 5 212 and 233.
+bool mixed_lengths(int nr, int group, int64_t total_q, int64_t num_seqs, int64_t longest,
+                   bool prefill) {
+  if (!may_mix(nr, group)) return false;
+  if (prefill) return true;
+  if (longest <= 1) return false;
+  const int64_t runs = std::max<int64_t>((total_q - num_seqs + longest - 2) / (longest - 1), 0);
+  const int64_t pieces = runs * ((longest * group + 31) / 32);
+  return num_seqs - runs >= (nr <= 24 ? 16 : 4) * pieces;
+}
 
 size_t pieces_bytes(int sms, int nr, int group) {
   // two pieces per CTA of two per SM, or four of 32 rows
-  const size_t rows = std::max<size_t>(2 * static_cast<size_t>((nr + 15) / 16 * 16), mixed_lengths(nr, group) ? 4 * 32 : 0);
+  const size_t rows = std::max<size_t>(2 * static_cast<size_t>((nr + 15) / 16 * 16), may_mix(nr, group) ? 4 * 32 : 0);
   return (decode_ticket_bytes(sms) + (2 * static_cast<size_t>(sms)) * rows * (kHeadDim + 1) * sizeof(float) + 255) &
          ~size_t(255);
 }
@@ -1207,8 +1234,8 @@ size_t workspace8(int sms, int nr, int group) {
 
 // The part of both calls after their own checks.
 int run_attention(Fp8DecodeParams p, const void* k_cache, const void* v_cache, const float* k_scale,
-                  const float* v_scale, int32_t scale_block, int nr, void* workspace, size_t workspace_bytes,
-                  void* stream) {
+                  const float* v_scale, int32_t scale_block, int nr, bool mixed, void* workspace,
+                  size_t workspace_bytes, void* stream) {
   const int64_t rows = static_cast<int64_t>(p.num_blocks) * p.block_size;
   const int sms = sm_count();
   if (sms == 0) return cuda_fail(cudaGetLastError());
@@ -1220,7 +1247,6 @@ int run_attention(Fp8DecodeParams p, const void* k_cache, const void* v_cache, c
   if ((rc = encode_rows8(&tm_k, k_cache, p.num_kv_heads, rows)) != NVA_OK) return rc;
   if ((rc = encode_rows8(&tm_v, v_cache, p.num_kv_heads, rows)) != NVA_OK) return rc;
   const int grid = 2 * sms;
-  const bool mixed = p.cu_q != nullptr && mixed_lengths(nr, p.group);
   const int rows_per_cta = mixed ? 4 * 32 : 2 * ((nr + 15) / 16 * 16);
   // (merge weights of a segment cut into as many pieces as there are CTAs fit the idle K and V rings)
   if (static_cast<size_t>(nr) * grid * sizeof(float) > 4 * kTile) return NVA_ERR_UNSUPPORTED;
@@ -1228,7 +1254,7 @@ int run_attention(Fp8DecodeParams p, const void* k_cache, const void* v_cache, c
   p.v_scale = v_scale;
   p.page_blocks = p.block_size / scale_block;
   p.lg_block = __builtin_ctz(static_cast<unsigned>(scale_block));
-  // heads that walk side by side: see the head of this file
+  // heads that walk side by side (the work split, above)
   p.head_set = 1;
   for (int h = 8; h > 1; h /= 2)
     if (p.num_kv_heads % h == 0 && grid % h == 0) {
@@ -1274,10 +1300,6 @@ int check_common(const void* q, int64_t q_row_stride, const void* k_cache, const
   return NVA_OK;
 }
 
-// Query runs of at least this many tokens take the prefill kernel, which gives each q head 128 rows of its own: its tile
-// of 128 keys takes about 2.5 us for the group's heads one after another, the pieces of 32 packed rows here 2 us each,
-// two at a time, so that runs of 80 cost about the same either way.
-constexpr int kMinPrefillRun = 81;
 
 bool positive_finite(float s) { return s > 0.f && s < 3.0e38f; }
 
@@ -1333,7 +1355,8 @@ NVA_API int nva_paged_decode_fp8(const void* q, int64_t q_row_stride, const void
   p.block_size = block_size;
   p.num_blocks = num_blocks;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  return nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, nr, workspace, workspace_bytes, stream);
+  return nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, nr, false, workspace, workspace_bytes,
+                            stream);
 }
 
 NVA_API int nva_varlen_attention_fp8(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
@@ -1377,6 +1400,7 @@ NVA_API int nva_varlen_attention_fp8(const void* q, int64_t q_row_stride, const 
   const int64_t tiles = static_cast<int64_t>(total_q) / 128 + num_seqs + 1;
   const bool prefill = max_seqlen_q >= nva::kMinPrefillRun && num_seqs <= nva::kMaxDecodeSeqs &&
                        tiles <= nva::kMaxPrefillTiles;
+  const bool mixed = nva::mixed_lengths(nr, p.group, total_q, num_seqs, max_seqlen_q, prefill);
   if (prefill) {
     const int sms = nva::sm_count();
     if (sms == 0) return nva::cuda_fail(cudaGetLastError());
@@ -1423,12 +1447,14 @@ NVA_API int nva_varlen_attention_fp8(const void* q, int64_t q_row_stride, const 
     if (e != cudaSuccess) return nva::cuda_fail(e);
     p.longest = nva::kMinPrefillRun - 1;
     p.pdl = 1;
-    rc = nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, nr, workspace, workspace_bytes, stream);
+    rc = nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, nr, mixed, workspace, workspace_bytes,
+                            stream);
     if (rc != NVA_OK) return rc;
     e = nva::launch_prefill(tm_q, tm_k, tm_v, tm_o, pp, grid, s);
     return e == cudaSuccess ? NVA_OK : nva::cuda_fail(e);
   }
-  return nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, nr, workspace, workspace_bytes, stream);
+  return nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, nr, mixed, workspace, workspace_bytes,
+                            stream);
 }
 
 }  // extern "C"

@@ -182,6 +182,16 @@ def test_varlen_head_layouts(cuda, H, KVH):
     check(make([300, 77, 520, 33], H=H, KVH=KVH, qlens=[100, 1, 9, 33], seed=H, G=64))
 
 
+@pytest.mark.parametrize("qlens", [[1] * 8 + [60] * 2, [60] * 2 + [1] * 96, [20] * 16, [5] * 64, [63] * 3, [64] * 3,
+                                   [9] * 16 + [1] * 130, [1, 63, 1, 5, 64, 1, 17], [33] * 5, [7] * 2 + [1] * 200])
+@pytest.mark.parametrize("H", [32, 8])
+def test_varlen_kernel_choice(cuda, qlens, H):
+    """Both sides of the bounds at which runs go to another kernel."""
+    lens = [n + (37 * i) % 300 for i, n in enumerate(qlens)]
+    lens[1] = max(qlens[1] - 3, 0)                         # keys for some of its queries only
+    check(make(lens, H=H, qlens=qlens, seed=len(qlens) + H))
+
+
 def test_varlen_rows_behind_the_last_sequence_stay(cuda):
     b = make([300, 50], qlens=[100, 1], seed=9)
     big = torch.cat([b["q"], b["q"][:20]])
