@@ -253,8 +253,9 @@ NVA_API size_t nva_paged_attention_fp8_workspace_bytes(int32_t max_q, int32_t nu
  *     tokens with w_i < min_p go; of the others the top_k largest stay (equals: lowest index first); of those, in
  *     falling order, a token stays while the weight before it is less than top_p times their sum
  *     ids = first index at which the running sum of the kept weights passes u times their sum
- * T <= 0: the argmax (torch's rule: lowest index, NaN above everything).  Sums are exact integer sums of weights rounded
- * to 2^-44, so a result depends on nothing but the arguments.
+ * T <= 0: the argmax (torch's rule: lowest index, NaN above everything).  With any of top_k, top_p and min_p weights are
+ * rounded to 2^-44 and summed as whole numbers; without them sums are in double precision and a weight is off by at most
+ * 4e-9 of itself.  Either way the order of a sum is fixed, so that a result depends on nothing but the arguments.
  *
  * nva_verify_sampled: rows of logits [num_seqs * (k + 1), vocab], settings and u per sequence, drafts [num_seqs, k],
  * num_drafts [num_seqs], accept_uniform [num_seqs, k].  Draft j of a sequence (j < num_drafts) is accepted when

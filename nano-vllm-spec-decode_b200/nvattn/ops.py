@@ -427,24 +427,23 @@ def verify_sampled(logits: torch.Tensor, draft_ids: torch.Tensor, num_drafts: to
     (num_accepted [S], next_token [S]) in the ids' dtype.  The rules are in include/nvattn.h."""
     _need_cuda(logits, draft_ids, num_drafts, temperatures, accept_uniforms, uniforms, top_k, top_p, min_p)
     S, K = draft_ids.shape
-    dt = draft_ids.dtype
-    assert logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32) and logits.shape[0] == S * (K + 1)
-    V = logits.shape[1]
-    assert logits.stride(1) == 1 or V == 1
+    dt, dev = draft_ids.dtype, logits.device
+    assert logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32)
+    rows, V = logits.shape
+    assert rows == S * (K + 1) and (logits.stride(1) == 1 or V == 1)
     assert dt in (torch.int32, torch.int64) and num_drafts.dtype == dt
     assert num_drafts.shape == (S,) and num_drafts.is_contiguous()
     assert K <= 1 or (draft_ids.stride(1) == 1 and accept_uniforms.stride(1) == 1)
     assert uniforms.dtype in (torch.float32, torch.float64) and uniforms.shape == (S,) and uniforms.is_contiguous()
     assert accept_uniforms.dtype == uniforms.dtype and accept_uniforms.shape == (S, K)
     assert temperatures is not None
-    assert logits.device == draft_ids.device == num_drafts.device == accept_uniforms.device == uniforms.device
-    t, k, p, m = _settings(S, logits.device, temperatures, top_k, top_p, min_p)
+    assert dev == draft_ids.device == num_drafts.device == accept_uniforms.device == uniforms.device
+    t, k, p, m = _settings(S, dev, temperatures, top_k, top_p, min_p)
     acc, nxt = torch.empty_like(num_drafts), torch.empty_like(num_drafts)
     lib = _lib.load()
-    ws_bytes = (16 * logits.shape[0] if k or p or m
-                else lib.nva_sample_workspace_bytes(logits.shape[0], V, logits.element_size()))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device)
-    with _on(logits.device):
+    ws_bytes = 16 * rows if k or p or m else lib.nva_sample_workspace_bytes(rows, V, logits.element_size())
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
         _lib.check(lib.nva_verify_sampled(
             logits.data_ptr(), max(logits.stride(0), V), S, K, V, logits.element_size(),
             draft_ids.data_ptr() if K else 0, max(draft_ids.stride(0), K) if K else 0, num_drafts.data_ptr(),

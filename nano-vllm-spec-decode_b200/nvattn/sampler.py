@@ -40,5 +40,7 @@ def verify_drafts_sampled(logits: torch.Tensor, draft_token_ids: torch.Tensor, n
     (integers), temperatures / uniforms / settings [S], accept_uniforms [S, K] -> (num_accepted [S], next_token [S])
     int64.  Sequence s keeps draft_token_ids[s, :num_accepted[s]], then next_token[s]; what comes out is distributed as
     if every token had been drawn by sample_tokens."""
-    return ops.verify_sampled(logits, draft_token_ids.to(torch.int64), num_drafts.to(torch.int64), temperatures,
-                              accept_uniforms, uniforms, top_k, top_p, min_p)
+    if draft_token_ids.dtype is not torch.int64 or num_drafts.dtype is not torch.int64:
+        draft_token_ids, num_drafts = draft_token_ids.to(torch.int64), num_drafts.to(torch.int64)
+    return ops.verify_sampled(logits, draft_token_ids, num_drafts, temperatures, accept_uniforms, uniforms, top_k, top_p,
+                              min_p)
