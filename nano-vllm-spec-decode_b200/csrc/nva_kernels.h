@@ -91,7 +91,8 @@ struct Fp8DecodeParams {
   int32_t num_kv_heads;
   int32_t group;
   int32_t max_n;        // queries per piece: tile rows / group
-  int32_t longest;      // varlen: sequences with longer query runs are left to the prefill kernel
+  int32_t shortest;     // varlen: sequences with shorter or longer query runs are left to the call's other kernels
+  int32_t longest;
   int32_t head_set;     // kv heads that as many CTAs walk side by side (divides num_kv_heads and the grid)
   int32_t block_size;
   int32_t num_blocks;
@@ -100,10 +101,11 @@ struct Fp8DecodeParams {
   int32_t page_blocks;  // scale blocks per cache block
   int32_t lg_block;     // log2 of the tokens per scale block
   float scale_log2;
-  float* part_o;        // [slots * grid, NP, 128], [slots * grid, NP] as in DecodeParams; two slots a CTA and phase
+  float* part_o;        // [slots * grid, NP, 128], [slots * grid, NP] as in DecodeParams; two slots a CTA
   float* part_lse;
-  int32_t* counters;    // [grid][4] merge tickets (one a phase): zero on entry and on exit
-  int32_t pdl;          // 1: launched with a programmatic dependency on the prefill plan, before the prefill kernel
+  int32_t* counters;    // [grid][4] merge tickets (every fourth word): zero on entry and on exit
+  int32_t pdl;          // 1: launched with a programmatic dependency on the call's preceding kernel
+  int32_t wait_primary; // 1: and waits for it (the prefill plan, behind which come the call's other inputs)
 };
 
 // Varlen prefill kernel (long query runs) — q rows tiled by 128 per (sequence, q head).

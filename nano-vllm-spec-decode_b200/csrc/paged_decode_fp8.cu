@@ -34,7 +34,8 @@
 //
 // Measured (32 q heads over 8, copy rate 6.57 TB/s): decode of 64 sequences of 512 to 4096 62 us (75%), of 8192 168 us
 // (97%), 8 of 40,000 to 65,536 139 us (95%); verify of 32 sequences of 256 to 2048, k = 4, 40 us; 4 sequences of 37 to
-// 1000 18 us, of which the start takes 6, the tiles 5 and the ends 5; 256 single queries with three prefill chunks 265 us.
+// 1000 18 us, of which the start takes 6, the tiles 5 and the ends 5; 256 single queries with three prefill chunks 243 us:
+// three kernels, each launched so that its blocks start where the last one's leave.
 #include <algorithm>
 #include <cuda_fp8.h>
 
@@ -88,9 +89,9 @@ struct Cfg8 {
   static constexpr int kAlpha = kNegM + NP * 4;                     // [NP]
   static constexpr int kRowInv = kAlpha + NP * 4;                   // [NP] 1 / sum
   static constexpr int kStart = (kRowInv + NP * 4 + 15) / 16 * 16;  // Start
-  static constexpr int kPending = kStart + 2 * 64;                  // [4] Pending
-  static constexpr int kScan = kPending + 4 * 24;                   // [2][8] int64
-  static constexpr int kTmem = kScan + 16 * 8;
+  static constexpr int kPending = kStart + 64;                      // [2] Pending
+  static constexpr int kScan = kPending + 2 * 24;                   // [8] int64
+  static constexpr int kTmem = kScan + 8 * 8;
   static constexpr int kAbort = kTmem + 4;
   static constexpr int kEnd = kAbort + 4;
   static constexpr int kBytes = kEnd + 1024;                        // + slack for 1024-byte alignment
@@ -139,7 +140,7 @@ __device__ __forceinline__ Shape8 shape_of(const Fp8DecodeParams& p, int b) {
   if (p.cu_q != nullptr) {
     const int a = __ldg(p.cu_q + b);
     s.n = max(__ldg(p.cu_q + b + 1) - a, 0);
-    if (s.n > p.longest) s.n = 0;   // (the prefill kernel's)
+    if (s.n > p.longest || s.n < p.shortest) s.n = 0;   // (another kernel's)
     s.q0 = a;
     s.L = max(__ldg(p.cu_k + b + 1) - __ldg(p.cu_k + b), 0);
   } else {
@@ -156,33 +157,24 @@ __device__ __forceinline__ int piece_keys(int n, int L, int i, int max_n) {
 }
 __device__ __forceinline__ int tiles_of(int keys) { return (keys + 127) >> 7; }
 
-// The kernel for batches of mixed lengths (kMixed) splits its work twice: phase 0 are the pieces of more than 8 packed
-// rows, which the softmax bounds, phase 1 the short ones, which HBM bounds.  Every CTA has its share of both, half of the
-// CTAs in the other order, so that the two kinds run beside each other on an SM and neither's cost has to be weighed
-// against the other's.
-template <bool kMixed>
-constexpr int kPhases = kMixed ? 2 : 1;
-
-// Calls f(first piece, count, tiles) for the runs of pieces of equal tile count of a sequence that belong to the phase, in
-// order, until it returns true.  (By tiles, not by pieces: a prompt of 16,384 has 2048 pieces but 128 tile counts.)
-template <bool kMixed, class F>
-__device__ __forceinline__ void piece_runs(const Fp8DecodeParams& p, int n, int L, int phase, F&& f) {
+// Calls f(first piece, count, tiles) for the runs of pieces of equal tile count of a sequence, in order, until it returns
+// true.  (By tiles, not by pieces: a prompt of 16,384 has 2048 pieces but 128 tile counts.)
+template <class F>
+__device__ __forceinline__ void piece_runs(const Fp8DecodeParams& p, int n, int L, F&& f) {
   const int m = p.max_n, full = n / m, before = L - n;   // piece i < full ends at key before + (i + 1) m
-  if (!kMixed || phase == 0) {                           // (whole pieces have more than 8 rows in a mixed batch)
-    int i = before + m >= 1 ? 1 : -before / m + 1;       // (1-based) the first with a key
+  int i = before + m >= 1 ? 1 : -before / m + 1;         // (1-based) the first with a key
 #pragma unroll 1
-    while (i <= full) {
-      const int t = (before + m * i + 127) >> 7;
-      const int last = min(full, (128 * t - before) / m);
-      if (f(i - 1, last - i + 1, t)) return;
-      i = last + 1;
-    }
+  while (i <= full) {
+    const int t = (before + m * i + 127) >> 7;
+    const int last = min(full, (128 * t - before) / m);
+    if (f(i - 1, last - i + 1, t)) return;
+    i = last + 1;
   }
   const int rest = n - full * m;
-  if (rest > 0 && L > 0 && (!kMixed || (rest * p.group > 8) == (phase == 0))) f(full, 1, tiles_of(L));
+  if (rest > 0 && L > 0) f(full, 1, tiles_of(L));
 }
 
-// Where a CTA starts in a phase.
+// Where a CTA starts.
 struct Start {
   long long segpos;   // cost position of the first segment
   long long x0, x1;   // the CTA's share of positions
@@ -193,18 +185,14 @@ struct Start {
 static_assert(sizeof(Start) == 64, "Start");
 
 // The tiles of one CTA in order.  Every lane of the warp holds the same state.  Tile j of a segment at segpos sits at
-// position segpos + kSegCost + j of its phase; a CTA owns the tiles whose positions are in [x0, x1).  Positions are kept
+// position segpos + kSegCost + j; a CTA owns the tiles whose positions are in [x0, x1).  Positions are kept
 // relative to x0.
-template <bool kMixed>
 struct Walk {
-  const Start* starts;
   int rel, span;      // segpos - x0, x1 - x0
   int b, piece, g, j;
   int n, L, q0;       // the sequence
   int np, Lp, nt;     // the piece: queries, keys its last query sees, tiles
-  int phase;
-  bool more;          // the other phase is still to come
-  bool fresh;         // the first tile of this CTA's share of the phase
+  bool fresh;         // the first tile of this CTA's share
   bool valid;
   int ahead, ahead_n, ahead_L, ahead_q0;   // sequences ahead .. ahead + 31, one per lane
 
@@ -219,53 +207,36 @@ struct Walk {
     Lp = piece_keys(n, L, piece, p.max_n);
     nt = tiles_of(Lp);
   }
-  // the share of the current phase, or of the other one when it is empty
-  __device__ __forceinline__ void enter(const Fp8DecodeParams& p) {
-    while (true) {
-      const Start& s = starts[phase];
-      valid = s.any != 0;
-      if (valid) {
-        rel = static_cast<int>(s.segpos - s.x0);
-        span = static_cast<int>(s.x1 - s.x0);
-        b = s.b;
-        piece = s.piece;
-        g = s.g;
-        j = s.j;
-        load_seq(p);
-        set_piece(p);
-        valid = rel + kSegCost + j < span;
-      }
-      if (valid || !more) break;
-      more = false;
-      phase ^= 1;
+  __device__ __forceinline__ void begin(const Fp8DecodeParams& p, const Start& s) {
+    ahead = -64;
+    valid = s.any != 0;
+    if (valid) {
+      rel = static_cast<int>(s.segpos - s.x0);
+      span = static_cast<int>(s.x1 - s.x0);
+      b = s.b;
+      piece = s.piece;
+      g = s.g;
+      j = s.j;
+      load_seq(p);
+      set_piece(p);
+      valid = rel + kSegCost + j < span;
     }
     fresh = valid;
   }
-  __device__ __forceinline__ void begin(const Fp8DecodeParams& p, const Start* s, int first_phase) {
-    starts = s;
-    ahead = -64;
-    phase = kMixed ? first_phase : 0;
-    more = kMixed;
-    enter(p);
-  }
-  // Whether a sequence has a piece with keys in the phase.
+  // Whether a sequence has a piece with keys.
   __device__ __forceinline__ bool has_piece(const Fp8DecodeParams& p, int n_, int L_) const {
-    const int full = n_ / p.max_n, rest = n_ - full * p.max_n;
-    const bool whole = full > 0 && L_ - n_ + full * p.max_n > 0, part = rest > 0 && L_ > 0;
-    if constexpr (!kMixed) return whole || part;
-    return phase == 0 ? whole || (part && rest * p.group > 8) : part && rest * p.group <= 8;
+    const int full = n_ / p.max_n;
+    return (full > 0 && L_ - n_ + full * p.max_n > 0) || (n_ > full * p.max_n && L_ > 0);
   }
-  // The next segment of the phase (all lanes of the warp together).
+  // The next segment (all lanes of the warp together).
   __device__ __forceinline__ void advance(const Fp8DecodeParams& p) {
     rel += nt + kSegCost;
     j = 0;
     valid = rel + kSegCost < span;
     if (!valid || ++g < p.num_kv_heads / p.head_set) return;
     g = 0;
-    bool belongs;
     do {
       ++piece;
-      if (kMixed && phase == 1) piece = max(piece, n / p.max_n);   // (whole pieces are phase 0)
       if (piece * p.max_n >= n) {
         // the next sequence that has one: 32 at a time, read once
         const int lane = threadIdx.x & 31;
@@ -295,23 +266,14 @@ struct Walk {
         n = __shfl_sync(kFull, ahead_n, src);
         L = __shfl_sync(kFull, ahead_L, src);
         q0 = __shfl_sync(kFull, ahead_q0, src);
-        piece = kMixed && phase == 1 ? n / p.max_n : 0;
+        piece = 0;
       }
       set_piece(p);
-      belongs = !kMixed || (np * p.group > 8) == (phase == 0);
-    } while (nt == 0 || !belongs);
-  }
-  __device__ __forceinline__ void other_phase(const Fp8DecodeParams& p) {
-    if (kMixed && !valid && more) {
-      more = false;
-      phase ^= 1;
-      enter(p);
-    }
+    } while (nt == 0);
   }
   __device__ __forceinline__ void next_segment(const Fp8DecodeParams& p) {
     fresh = false;
     advance(p);
-    other_phase(p);
   }
   __device__ __forceinline__ void next_tile(const Fp8DecodeParams& p) {
     fresh = false;
@@ -320,13 +282,12 @@ struct Walk {
     } else {
       advance(p);
     }
-    other_phase(p);
   }
 };
 
 // A cut segment that this CTA has to merge (c1 < 0: none).
 struct Pending {
-  int c0, c1, rows, phase;
+  int c0, c1, rows;
   int64_t out_base;
 };
 
@@ -350,17 +311,6 @@ __device__ __forceinline__ void put_q_row(uint2 x, uint8_t* qs, int half_bytes, 
   if (lane == 0) scales[r] = back;
 }
 
-// Softmax rows of a segment: NR, or 8 for the short runs of a batch of mixed lengths.  (Each further variant inside one
-// kernel costs the others registers.)
-template <int NR, bool kMixed, class F>
-__device__ __forceinline__ void with_rows8(int R, F&& f) {
-  if (kMixed && R <= 8) {
-    f(std::integral_constant<int, 8>{});
-  } else {
-    f(std::integral_constant<int, NR>{});
-  }
-}
-
 template <int HR>
 __device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, float* v) {
   if constexpr (HR == 8) {
@@ -380,7 +330,7 @@ __device__ __forceinline__ void warp_rows(const float* x, float* dst, int lane) 
   if constexpr (HR % 16 != 0) warp_columns<8, kMax>(x + HR / 16 * 16, dst + HR / 16 * 16, lane);
 }
 
-template <int NR, bool kMixed>
+template <int NR>
 __global__ void __launch_bounds__(Cfg8<NR>::kThreads, 2)
 paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const Fp8DecodeParams p) {
@@ -398,7 +348,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
   float* negm_s = reinterpret_cast<float*>(smem + C::kNegM);
   float* alpha_s = reinterpret_cast<float*>(smem + C::kAlpha);
   float* row_inv = reinterpret_cast<float*>(smem + C::kRowInv);
-  Start* start = reinterpret_cast<Start*>(smem + C::kStart);   // [phase], 64 bytes apart
+  Start* start = reinterpret_cast<Start*>(smem + C::kStart);
   Pending* pending = reinterpret_cast<Pending*>(smem + C::kPending);
   long long* scan = reinterpret_cast<long long*>(smem + C::kScan);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kTmem);
@@ -432,25 +382,23 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     for (int i = 0; i < kInfoRing; ++i) mbar_init(&bars[B_INFO + i], 1);
     mbar_init(&bars[B_KSTART], 1);
     *abort = 0;
-    for (int i = 0; i < 2; ++i) start[i].any = 0;
-    for (int i = 0; i < 4; ++i) pending[i].c1 = -1;
+    start->any = 0;
+    for (int i = 0; i < 2; ++i) pending[i].c1 = -1;
     fence_barrier_init();
     fence_proxy_async_smem();
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  // With a programmatic dependency on the prefill plan: wait for it (and what came before it), then let the call's
-  // prefill kernel start its blocks where this grid's leave.
-  if (p.pdl) {
-    griddep_wait();
-    if (tid == 0) griddep_launch_dependents();
-  }
+  // With a programmatic dependency on the prefill plan: wait for it (and what came before it).  Then let the call's next
+  // kernel start its blocks where this grid's leave.
+  if (p.wait_primary) griddep_wait();
+  if (tid == 0) griddep_launch_dependents();
   // ------------------------------------------------------------ the work split
   // Two scans over the sequences' costs: the total (hence each CTA's share), then the sequence that holds this CTA's
   // first position.  Batches of up to kThreads sequences keep the first scan's values in registers.
   {
-    constexpr int T = C::kThreads, W = T / 32, kPh = kPhases<kMixed>;
-    long long total[kPh] = {}, x0[kPh] = {}, per[kPh] = {}, before[kPh] = {}, mine[kPh] = {}, excl[kPh] = {}, sum[kPh] = {};
+    constexpr int T = C::kThreads, W = T / 32;
+    long long total = 0, x0 = 0, per = 0, before = 0, mine = 0, excl = 0, sum = 0;
     int n = 0, L = 0;
     const bool single = p.num_seqs <= T;
 #pragma unroll 1
@@ -464,77 +412,64 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             n = s.n;
             L = s.L;
           }
+          mine = 0;
+          piece_runs(p, n, L, [&](int, int count, int nt) {
+            mine += static_cast<long long>(sets) * count * (nt + kSegCost);
+            return false;
+          });
+          long long x = mine;
 #pragma unroll
-          for (int ph = 0; ph < kPh; ++ph) {
-            mine[ph] = 0;
-            piece_runs<kMixed>(p, n, L, ph, [&](int, int count, int nt) {
-              mine[ph] += static_cast<long long>(sets) * count * (nt + kSegCost);
-              return false;
-            });
-            long long x = mine[ph];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const long long y = __shfl_up_sync(kFull, x, o);
-              if (lane >= o) x += y;
-            }
-            if (lane == 31) scan[ph * W + warp] = x;
-            excl[ph] = x - mine[ph];
+          for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(kFull, x, o);
+            if (lane >= o) x += y;
           }
+          if (lane == 31) scan[warp] = x;
+          excl = x - mine;
           __syncthreads();
+          sum = 0;
 #pragma unroll
-          for (int ph = 0; ph < kPh; ++ph) {
-            sum[ph] = 0;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-              const long long v = scan[ph * W + w];
-              excl[ph] += w < warp ? v : 0;
-              sum[ph] += v;
-            }
+          for (int w = 0; w < W; ++w) {
+            const long long v = scan[w];
+            excl += w < warp ? v : 0;
+            sum += v;
           }
           __syncthreads();
         }
-#pragma unroll
-        for (int ph = 0; ph < kPh; ++ph) {
-          if (pass == 0) {
-            total[ph] += sum[ph];
-            continue;
-          }
-          // the thread whose sequence holds position x0
-          const long long lo = before[ph] + excl[ph];
-          before[ph] += sum[ph];
-          if (mine[ph] > 0 && x0[ph] >= lo && x0[ph] < lo + mine[ph]) {
-            long long rem = x0[ph] - lo;
-            piece_runs<kMixed>(p, n, L, ph, [&](int first, int count, int nt) {
-              const int seg = nt + kSegCost;
-              const long long run = static_cast<long long>(sets) * count * seg;
-              if (rem >= run) {
-                rem -= run;
-                return false;
-              }
-              const int i = static_cast<int>(rem / (sets * seg));
-              const int r = static_cast<int>(rem) - i * sets * seg, g = r / seg, o = r - g * seg;
-              Start* st = start + ph;
-              st->segpos = x0[ph] - o;
-              st->b = base + tid;
-              st->piece = first + i;
-              st->g = g;
-              st->j = max(0, o - kSegCost);
-              st->any = 1;
-              return true;
-            });
-          }
+        if (pass == 0) {
+          total += sum;
+          continue;
+        }
+        // the thread whose sequence holds position x0
+        const long long lo = before + excl;
+        before += sum;
+        if (mine > 0 && x0 >= lo && x0 < lo + mine) {
+          long long rem = x0 - lo;
+          piece_runs(p, n, L, [&](int first, int count, int nt) {
+            const int seg = nt + kSegCost;
+            const long long run = static_cast<long long>(sets) * count * seg;
+            if (rem >= run) {
+              rem -= run;
+              return false;
+            }
+            const int i = static_cast<int>(rem / (sets * seg));
+            const int r = static_cast<int>(rem) - i * sets * seg, g = r / seg, o = r - g * seg;
+            start->segpos = x0 - o;
+            start->b = base + tid;
+            start->piece = first + i;
+            start->g = g;
+            start->j = max(0, o - kSegCost);
+            start->any = 1;
+            return true;
+          });
         }
       }
       if (pass == 0) {
-#pragma unroll
-        for (int ph = 0; ph < kPh; ++ph) {
-          per[ph] = total[ph] > 0 ? (total[ph] + teams - 1) / teams : 1;
-          x0[ph] = per[ph] * team;
-          if (tid == 0) {
-            start[ph].x0 = x0[ph];
-            start[ph].x1 = min(x0[ph] + per[ph], total[ph]);
-            start[ph].per = per[ph];
-          }
+        per = total > 0 ? (total + teams - 1) / teams : 1;
+        x0 = per * team;
+        if (tid == 0) {
+          start->x0 = x0;
+          start->x1 = min(x0 + per, total);
+          start->per = per;
         }
       }
     }
@@ -551,9 +486,14 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(ss.q0 + i) * p.out_row_stride)[c] =
             make_uint4(0u, 0u, 0u, 0u);
   }
-  Walk<kMixed> w;
-  w.begin(p, start, blockIdx.x >= gridDim.x / 2 ? 1 : 0);
-  if (!w.valid) return;   // nothing for this CTA: no TMEM, no pipeline
+  Walk w;
+  w.begin(p, *start);
+  // A grid that did not wait for the one before it must not complete first: one block waits at its end.
+  const bool holds = p.pdl && !p.wait_primary && blockIdx.x == 0;
+  if (!w.valid) {         // nothing for this CTA: no TMEM, no pipeline
+    if (holds) griddep_wait();
+    return;
+  }
   if (warp < 4) {
   if (warp == 0 || warp == 3) {
     // ------------------------------------------------------------ K (warp 0) and V (warp 3) producers
@@ -569,7 +509,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       // descriptors of the next tiles, one per lane (their block-table reads overlap); a short first round, so that
       // the first copies start early
       const int round = jj == 0 ? 4 : 32;
-      int g = 0, j = 0, flags = 0, np = 0, Lp = 0, qrow = 0, nt = 0, b = 0, rel = 0, phase = 0, cnt = 0;
+      int g = 0, j = 0, flags = 0, np = 0, Lp = 0, qrow = 0, nt = 0, b = 0, rel = 0, cnt = 0;
       for (; cnt < round && w.valid; ++cnt) {
         const bool first = w.fresh || w.j == 0;
         const bool seg_end = w.j == w.nt - 1;
@@ -582,7 +522,6 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
           b = w.b;
           qrow = w.q0 + w.piece * p.max_n;
           rel = w.rel;
-          phase = w.phase;
         }
         w.next_tile(p);
         // 1: first, 2: last tile of this CTA's part of a segment, 4: of the CTA
@@ -601,7 +540,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       for (int i = 0; i < cnt; ++i, ++jj) {
         const int st = jj % stages;
         const int gi = __shfl_sync(kFull, g, i), pi = __shfl_sync(kFull, page, i), oi = __shfl_sync(kFull, off, i);
-        int ji = 0, fi = 0, ni = 0, Li = 0, qi = 0, ti = 0, ri = 0, hi = 0;
+        int ji = 0, fi = 0, ni = 0, Li = 0, qi = 0, ti = 0, ri = 0;
         if (is_k) {
           ji = __shfl_sync(kFull, j, i);
           fi = __shfl_sync(kFull, flags, i);
@@ -610,7 +549,6 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
           qi = __shfl_sync(kFull, qrow, i);
           ti = __shfl_sync(kFull, nt, i);
           ri = __shfl_sync(kFull, rel, i);
-          hi = __shfl_sync(kFull, phase, i);
         }
         if (!mbar_wait_warp(&empty[st], ((jj / stages) & 1) ^ 1, abort)) {
           stop = true;
@@ -621,7 +559,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             const int e = jj % kInfoRing;
             info[3 * e] = make_int4(ji * 128, pi, oi, gi);
             info[3 * e + 1] = make_int4(ni, Li, qi, ti);
-            info[3 * e + 2] = make_int4(fi, ri, hi, 0);
+            info[3 * e + 2] = make_int4(fi, ri, 0, 0);
             mbar_arrive(&bars[B_INFO + e]);
           }
           mbar_arrive_expect_tx(&full[st], kTile);
@@ -767,17 +705,17 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     float ks_next = 0.f, vs_next = 1.f;   // the next tile's scales of this thread's token
 
     // A piece of a cut segment is done (its rows written): take a ticket.  The CTA that brings
-    // it to the number of pieces puts the counter back to zero and merges them all; a CTA has at most two cut segments a phase,
+    // it to the number of pieces puts the counter back to zero and merges them all; a CTA has at most two cut segments,
     // so it notes them and merges after its last tile, out of the loop's registers.
-    constexpr int kSlots = 2 * kPhases<kMixed>;   // pieces a CTA may leave: two per phase
-    auto arrive_piece = [&](int phase, int p_first, int p_last, int R, int64_t out_base) {
+    constexpr int kSlots = 2;   // pieces a CTA may leave
+    auto arrive_piece = [&](int p_first, int p_last, int R, int64_t out_base) {
       named_bar_sync(bar_id, 128);
       if (ct == 0) {
         // the CTAs of the segment's first and last tile
-        const Start& st = start[phase];
+        const Start& st = *start;
         const int c0 = member * teams + static_cast<int>((st.x0 + p_first) / st.per);
         const int c1 = member * teams + static_cast<int>((st.x0 + p_last) / st.per);
-        int32_t* ticket = p.counters + kTicketStride * c0 + phase;
+        int32_t* ticket = p.counters + kTicketStride * c0;
         __threadfence();   // release: the group's partial rows before the ticket
         if (atomicAdd(ticket, 1) == c1 - c0) {
           *ticket = 0;
@@ -786,7 +724,6 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
           d->c0 = c0;
           d->c1 = c1;
           d->rows = R;
-          d->phase = phase;
           d->out_base = out_base;
         }
       }
@@ -826,17 +763,11 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     if (alive) load_scales(info[0], info[1]);
     int jj = 0;   // tile of this CTA
     for (int seg = 0; !done; ++seg) {
-      // One segment, in the variant for its rows: weights and sums live in registers of that variant only.
-      int rows = 0;
-      {
-        const int e = jj % kInfoRing;
-        alive = alive && mbar_wait_warp(&bars[B_INFO + e], (jj / kInfoRing) & 1, abort);
-        if (alive) rows = info[3 * e + 1].x * G;
-      }
+      // one segment
       const uint32_t t_o = t_lane + (2 + (seg & 1)) * NP;   // O accumulator, by segment parity
       const float* qs = qscale + (seg % kQScaleRing) * NR;
-      with_rows8<NR, kMixed>(rows, [&](auto hr_c) {
-        constexpr int HR = decltype(hr_c)::value;
+      [&] {
+        constexpr int HR = NR;
         constexpr int kChunk = HR % 16 == 0 ? 16 : 8;   // rows per TMEM load
         float l[HR], s[HR];
 #pragma unroll
@@ -1002,7 +933,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
           if (last) break;   // (a warp that gave up in the middle of a segment is caught by the next tile's vote)
         }
         warp_rows<HR, false>(l, red + wq * NP, lane);
-      });
+      }();
       if (done) break;
       // ---- the segment's end (tile jj): 1 / sum, and the rows of this CTA's part
       const int e = jj % kInfoRing;
@@ -1013,11 +944,10 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       const int R = ib.x * G;
       // positions of the segment's first and last tile relative to this CTA's share: a segment inside it is finished
       // here, one that is cut leaves a piece
-      const int phase = ic.z;
-      const int span = static_cast<int>(start[phase].x1 - start[phase].x0);
+      const int span = static_cast<int>(start->x1 - start->x0);
       const int p_first = ic.y + kSegCost, p_last = p_first + ib.w - 1;
       const bool complete = p_first >= 0 && p_last < span;
-      const int slot = kSlots * vcta + 2 * phase + (p_first < 0 ? 0 : 1);   // (of a piece)
+      const int slot = kSlots * vcta + (p_first < 0 ? 0 : 1);   // (of a piece)
       const int64_t out_base = ib.z * p.out_row_stride + static_cast<int64_t>(seg_g) * G * kHeadDim;
       if (ct < R) {
         const float lt = red[ct] + red[NP + ct] + red[2 * NP + ct] + red[3 * NP + ct];
@@ -1060,7 +990,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         }
       }
       tc_fence_before();
-      if (!complete) arrive_piece(phase, p_first, p_last, R, out_base);
+      if (!complete) arrive_piece(p_first, p_last, R, out_base);
       done = ic.x & 4;
       ++jj;
     }
@@ -1075,7 +1005,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       const int pieces = d.c1 - d.c0 + 1;
       float* table = reinterpret_cast<float*>(smem + C::kK);   // [rows][pieces] weights; the rings are idle
       auto piece_row = [&](int c, int r) {
-        return static_cast<int64_t>(kSlots * (d.c0 + c) + 2 * d.phase + (c == 0 ? 1 : 0)) * NP + r;
+        return static_cast<int64_t>(kSlots * (d.c0 + c) + (c == 0 ? 1 : 0)) * NP + r;
       };
       // weights 2^(lse - max) / sum of pieces that saw a key; partials come from other CTAs: past L1
       if (pieces <= 16) {   // (a thread per row)
@@ -1170,16 +1100,17 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(*tmem_slot, C::kTmemCols);
+    if (holds) griddep_wait();
   }
 }
 
-template <int NR, bool kMixed>
+template <int NR>
 cudaError_t launch8(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const Fp8DecodeParams& p, int grid,
                     cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(paged_decode_fp8_kernel<NR, kMixed>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaError_t e = cudaFuncSetAttribute(paged_decode_fp8_kernel<NR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        Cfg8<NR>::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_kernel(paged_decode_fp8_kernel<NR, kMixed>, dim3(grid), dim3(Cfg8<NR>::kThreads), Cfg8<NR>::kBytes, stream,
+  return launch_kernel(paged_decode_fp8_kernel<NR>, dim3(grid), dim3(Cfg8<NR>::kThreads), Cfg8<NR>::kBytes, stream,
                        p.pdl != 0, tm_k, tm_v, p);
 }
 
@@ -1202,39 +1133,42 @@ int tile_rows(int64_t rows) {
 // 164 and 150, 184 and 276; runs of 80: 49 and 36, 267 and 153, 293 and 281.
 constexpr int kMinPrefillRun = 64;
 
-// Whether a varlen call of that row count may take the kernel for mixed lengths (pieces of 32 rows, 8-row runs apart).
-bool may_mix(int nr, int group) { return nr > 16 && group <= 32; }
+// Queries of the runs that a split call leaves to the kernel of the fewest rows.
+int short_run(int group) { return std::max(1, 8 / group); }
 
-// Whether it does.  The other kernels give every run the rows of the longest, this one splits its work twice and merges
-// more; it pays where single queries outnumber the long runs' pieces, as the totals tell if all long runs are alike (runs
-// for the prefill kernel count as none).  Single queries + long runs over 2000 keys, 32 q heads over 8, mixed and not:
-// 32 + 2 x 60 93 and 81 us, 48 + 2 x 60 102 and 100, 64 + 2 x 60 112 and 122, 96 + 2 x 60 133 and 158, 256 + 16 x 20 299
-// and 378, 128 + 16 x 9 164 and 205; with the narrower rows of k = 4, 128 + 16 x 5 152 and 146, 256 + 2 x 5 212 and 233.
-bool mixed_lengths(int nr, int group, int64_t total_q, int64_t num_seqs, int64_t longest,
-                   bool prefill) {
-  if (!may_mix(nr, group)) return false;
+// Whether a varlen call runs twice, short runs (up to 8 packed rows, or one query) and the others each in a kernel of
+// their own rows: one kernel gives every run the rows of the longest.  Two have two starts, so it pays where short runs
+// outnumber the long ones' pieces, as the totals tell if all long runs are alike (runs for the prefill kernel count as
+// none).  Single queries + long runs over 2000 keys, 32 q heads over 8, one kernel and two: 32 + 2 x 60 81 and 75 us, 64 +
+// 2 x 60 122 and 99, 256 + 16 x 20 378 and 243, 128 + 16 x 9 205 and 140, 256 + 2 x 5 233 and 197, 64 + 32 x 5 107 and 104,
+// 64 + 8 x 5 82 and 83.
+bool two_kernels(int nr, int group, int64_t total_q, int64_t num_seqs, int64_t longest, bool prefill) {
+  if (nr <= tile_rows(static_cast<int64_t>(short_run(group)) * group)) return false;
   if (prefill) return true;
-  if (longest <= 1) return false;
   const int64_t runs = std::max<int64_t>((total_q - num_seqs + longest - 2) / (longest - 1), 0);
-  const int64_t pieces = runs * ((longest * group + 31) / 32);
-  return num_seqs - runs >= (nr <= 24 ? 16 : 4) * pieces;
+  const int64_t pieces = runs * ((longest * group + nr - 1) / nr);
+  return num_seqs - runs >= 2 * pieces;
 }
 
+// Two pieces of a kernel's rows per CTA of two per SM.
+size_t parts_bytes(int sms, int nr) {
+  return (2 * static_cast<size_t>(sms)) * 2 * ((nr + 15) / 16 * 16) * (kHeadDim + 1) * sizeof(float);
+}
+
+// Tickets, the pieces of the two kernels of a split call, then the prefill kernel's plan.
 size_t pieces_bytes(int sms, int nr, int group) {
-  // two pieces per CTA of two per SM, or four of 32 rows
-  const size_t rows = std::max<size_t>(2 * static_cast<size_t>((nr + 15) / 16 * 16), may_mix(nr, group) ? 4 * 32 : 0);
-  return (decode_ticket_bytes(sms) + (2 * static_cast<size_t>(sms)) * rows * (kHeadDim + 1) * sizeof(float) + 255) &
-         ~size_t(255);
+  const int first = tile_rows(static_cast<int64_t>(short_run(group)) * group);
+  return (decode_ticket_bytes(sms) + parts_bytes(sms, nr) + (nr > first ? parts_bytes(sms, first) : 0) + 255) & ~size_t(255);
 }
 
-// Tickets and pieces, then the prefill kernel's plan.
 size_t workspace8(int sms, int nr, int group) {
   return pieces_bytes(sms, nr, group) + sizeof(int32_t) * (2 + static_cast<size_t>(kMaxPrefillTiles));
 }
 
-// The part of both calls after their own checks.
+// The part of both calls after their own checks: runs of shortest to longest queries in the kernel for nr rows.  `second`:
+// behind the kernel of the short runs, beside whose last blocks its own may run (other tickets, other pieces).
 int run_attention(Fp8DecodeParams p, const void* k_cache, const void* v_cache, const float* k_scale,
-                  const float* v_scale, int32_t scale_block, int nr, bool mixed, void* workspace,
+                  const float* v_scale, int32_t scale_block, int nr, bool second, void* workspace,
                   size_t workspace_bytes, void* stream) {
   const int64_t rows = static_cast<int64_t>(p.num_blocks) * p.block_size;
   const int sms = sm_count();
@@ -1247,7 +1181,6 @@ int run_attention(Fp8DecodeParams p, const void* k_cache, const void* v_cache, c
   if ((rc = encode_rows8(&tm_k, k_cache, p.num_kv_heads, rows)) != NVA_OK) return rc;
   if ((rc = encode_rows8(&tm_v, v_cache, p.num_kv_heads, rows)) != NVA_OK) return rc;
   const int grid = 2 * sms;
-  const int rows_per_cta = mixed ? 4 * 32 : 2 * ((nr + 15) / 16 * 16);
   // (merge weights of a segment cut into as many pieces as there are CTAs fit the idle K and V rings)
   if (static_cast<size_t>(nr) * grid * sizeof(float) > 4 * kTile) return NVA_ERR_UNSUPPORTED;
   p.k_scale = k_scale;
@@ -1261,20 +1194,19 @@ int run_attention(Fp8DecodeParams p, const void* k_cache, const void* v_cache, c
       p.head_set = h;
       break;
     }
-  p.max_n = (mixed ? 32 : nr) / p.group;
-  p.counters = static_cast<int32_t*>(workspace);
-  p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + decode_ticket_bytes(sms));
-  p.part_lse = p.part_o + static_cast<size_t>(grid) * rows_per_cta * kHeadDim;
+  p.max_n = nr / p.group;
+  p.counters = static_cast<int32_t*>(workspace) + (second ? 1 : 0);
+  const size_t first = parts_bytes(sms, tile_rows(static_cast<int64_t>(short_run(p.group)) * p.group));
+  p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + decode_ticket_bytes(sms) + (second ? first : 0));
+  p.part_lse = p.part_o + static_cast<size_t>(grid) * 2 * ((nr + 15) / 16 * 16) * kHeadDim;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (p.longest == 0) p.longest = 0x7FFFFFFF;
-  switch (mixed ? 0 : nr) {
-    case 8: e = launch8<8, false>(tm_k, tm_v, p, grid, s); break;
-    case 16: e = launch8<16, false>(tm_k, tm_v, p, grid, s); break;
-    case 24: e = launch8<24, false>(tm_k, tm_v, p, grid, s); break;
-    case 32: e = launch8<32, false>(tm_k, tm_v, p, grid, s); break;
-    case 40: e = launch8<40, false>(tm_k, tm_v, p, grid, s); break;
-    default: e = launch8<32, true>(tm_k, tm_v, p, grid, s);
+  switch (nr) {
+    case 8: e = launch8<8>(tm_k, tm_v, p, grid, s); break;
+    case 16: e = launch8<16>(tm_k, tm_v, p, grid, s); break;
+    case 24: e = launch8<24>(tm_k, tm_v, p, grid, s); break;
+    case 32: e = launch8<32>(tm_k, tm_v, p, grid, s); break;
+    default: e = launch8<40>(tm_k, tm_v, p, grid, s);
   }
   return e == cudaSuccess ? NVA_OK : cuda_fail(e);
 }
@@ -1400,7 +1332,27 @@ NVA_API int nva_varlen_attention_fp8(const void* q, int64_t q_row_stride, const 
   const int64_t tiles = static_cast<int64_t>(total_q) / 128 + num_seqs + 1;
   const bool prefill = max_seqlen_q >= nva::kMinPrefillRun && num_seqs <= nva::kMaxDecodeSeqs &&
                        tiles <= nva::kMaxPrefillTiles;
-  const bool mixed = nva::mixed_lengths(nr, p.group, total_q, num_seqs, max_seqlen_q, prefill);
+  // The decode kernel's part: all runs up to the prefill kernel's at once, or the short ones and the others.
+  const bool two = nva::two_kernels(nr, p.group, total_q, num_seqs, max_seqlen_q, prefill);
+  auto decode = [&]() -> int {
+    p.shortest = 0;
+    p.longest = prefill ? nva::kMinPrefillRun - 1 : 0x7FFFFFFF;
+    p.pdl = p.wait_primary = prefill ? 1 : 0;
+    if (two) {
+      const int64_t longest = p.longest;
+      p.longest = nva::short_run(p.group);
+      const int first = nva::tile_rows(static_cast<int64_t>(p.longest) * p.group);
+      const int e = nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, first, false, workspace,
+                                       workspace_bytes, stream);
+      if (e != NVA_OK) return e;
+      p.shortest = p.longest + 1;
+      p.longest = static_cast<int32_t>(longest);
+      p.pdl = 1;
+      p.wait_primary = 0;
+    }
+    return nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, nr, two, workspace, workspace_bytes,
+                              stream);
+  };
   if (prefill) {
     const int sms = nva::sm_count();
     if (sms == 0) return nva::cuda_fail(cudaGetLastError());
@@ -1445,16 +1397,11 @@ NVA_API int nva_varlen_attention_fp8(const void* q, int64_t q_row_stride, const 
     // plan, short runs, long runs: the prefill kernel's blocks take their items from a counter as SMs come free
     cudaError_t e = nva::launch_prefill_plan(pp, s);
     if (e != cudaSuccess) return nva::cuda_fail(e);
-    p.longest = nva::kMinPrefillRun - 1;
-    p.pdl = 1;
-    rc = nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, nr, mixed, workspace, workspace_bytes,
-                            stream);
-    if (rc != NVA_OK) return rc;
+    if ((rc = decode()) != NVA_OK) return rc;
     e = nva::launch_prefill(tm_q, tm_k, tm_v, tm_o, pp, grid, s);
     return e == cudaSuccess ? NVA_OK : nva::cuda_fail(e);
   }
-  return nva::run_attention(p, k_cache, v_cache, k_scale, v_scale, scale_block, nr, mixed, workspace, workspace_bytes,
-                            stream);
+  return decode();
 }
 
 }  // extern "C"

@@ -322,3 +322,32 @@ def test_long_replays_stay_clean(cuda):
             graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and _lib.device_error() == 0
+
+
+def test_split_calls_in_a_row_and_replayed(cuda):
+    """Calls whose kernels overlap share one workspace, back to back and in a graph: every output is the first one's."""
+    from nvattn import _lib
+    batches = [make([40 + (53 * i) % 900 for i in range(len(q))], qlens=q, seed=30 + i)
+               for i, q in enumerate([[1] * 90 + [20] * 6, [1] * 70 + [5] * 9 + [130], [60] * 2 + [1] * 100, [9] * 40])]
+    want = [check(b) for b in batches]
+    outs = [torch.empty_like(w) for w in want]
+
+    def step():
+        for b, o in zip(batches, outs):
+            run(b, out=o)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(60):
+        for o in outs:
+            o.fill_(7.0)
+        graph.replay() if i % 2 else step()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w), i
+    assert _lib.device_error() == 0
