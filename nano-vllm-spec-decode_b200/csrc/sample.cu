@@ -402,9 +402,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     return nextafterf(nextafterf(max - (static_cast<float>(bin) + 1.01f) / bin_scale, -kInf), -kInf);
   };
   // A small top-k: every CTA lists its own k largest, and whatever its bound lets through, before it knows the others'
-  // (one exchange in all instead of four).  The bound: the k-th largest of its threads' maxima, to a bin, so that 512
-  // numbers are counted and not its share of the row; about k + k^2 / 1024 tokens pass it.
-  bool listed = !greedy && k > 0 && k <= kThreads / 2 && k * ranks <= kShort / 2;
+  // (one exchange in all instead of three).  The bound: the k-th largest of its threads' maxima, to a bin, so that 512
+  // numbers are counted and not its share of the row; about k + k^2 / 1024 tokens pass it.  Beyond 256 tokens in all
+  // the longer sort costs more than the exchanges (64 rows of four CTAs in bf16, this and one bound for the row: k = 50
+  // 22.7 and 22.7 us, 128 28.9 and 24.8, 256 43 and 28; one row of eight, k = 128: 24.8 and 18.5).
+  bool listed = !greedy && k > 0 && k <= kThreads / 2 && k * ranks <= kThreads / 2;
   if (listed) {
     for (int i = tid; i < kBins; i += kThreads) hist[0][i] = 0;
     if (tid == 0) list_count = 0;
