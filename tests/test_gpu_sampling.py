@@ -329,3 +329,63 @@ def test_no_rows(cuda):
     a, n = ops.verify_sampled(torch.zeros(0, 50, device="cuda"), torch.zeros(0, 2, dtype=torch.int64, device="cuda"),
                               torch.zeros(0, dtype=torch.int64, device="cuda"), e, torch.zeros(0, 2, device="cuda"), e)
     assert a.shape == n.shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_plain_verify_at_segment_edges(cuda, dtype):
+    """Drafts in the first and last tokens of a warp's segment, as the only token, without a weight and out of range."""
+    V, S, K = 9000, 12, 2
+    x, g = rows(S * (K + 1), V, dtype, 41)
+    d = torch.tensor([[0, V - 1], [1023, 1024], [2047, 2048], [4095, 4096], [8191, 8192], [V - 1, 0], [5, 5], [-1, V],
+                      [77, 78], [1024, 2048], [8999, 8998], [3, 2047]])
+    row = x.view(S, K + 1, V)
+    for s in range(8):                                     # often accepted: most of the weight
+        for j in range(K):
+            if 0 <= d[s, j] < V:
+                row[s, j, d[s, j]] = 16.0
+    row[8] = float("-inf")                                 # nothing but the draft
+    row[8, 0, 77] = row[8, 1, 78] = row[8, 2, 4] = 0.5
+    row[9, :, 1024] = float("-inf")                        # drafts without a weight
+    row[10, 0] = float("-inf")                             # nothing at all: every token alike
+    row[11, 0, :2048] = float("-inf")                      # the draft alone in its segment
+    row[11, 0, 3] = 6.0
+    nd = torch.full((S,), K)
+    one = torch.ones(S)
+    for hi in (0.5, 0.999, 1.0):
+        au, u = torch.rand(S, K, generator=g) * hi, torch.rand(S, generator=g)
+        check_verify(x, d, nd, one, au, u)
+        check_verify(x, d, nd, one * 0.6, au.double(), u.double(), torch.int32)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_plain_rows_of_any_alignment(cuda, dtype):
+    """Rows that begin at any element, with a stride of their own: the same draws as packed ones."""
+    R, V = 9, 5003
+    x, g = rows(R, V, dtype, 43)
+    u, t = torch.rand(R, generator=g), torch.rand(R, generator=g) + 0.3
+    t[4] = 0
+    want = check(x, t, u)
+    for first, stride in ((1, V + 1), (3, V + 6), (8, V + 5)):
+        big = torch.full((first + R * stride,), 50.0, dtype=dtype, device="cuda")
+        view = big[first:].as_strided((R, V), (stride, 1))
+        view.copy_(x)
+        assert torch.equal(run(view, t, u), want)
+
+
+def test_calls_on_two_streams_at_once(cuda):
+    from nvattn.sampler import sample_tokens
+    x, g = rows(40, 30011, torch.float32, 44)
+    x, u, t = x.cuda(), torch.rand(40, generator=g).cuda(), torch.rand(40, generator=g).cuda() + 0.3
+    p = torch.full((40,), 0.8, device="cuda")
+    k = torch.full((40,), 60, dtype=torch.int32, device="cuda")
+    settings = [dict(), dict(top_p=p), dict(top_k=k), dict(top_k=k, top_p=p)]
+    want = [sample_tokens(x, t, u, **s) for s in settings]
+    streams = [torch.cuda.Stream() for _ in settings]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for s, kw in zip(streams, settings):
+            with torch.cuda.stream(s):
+                got.append(sample_tokens(x, t, u, **kw))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
