@@ -158,6 +158,14 @@ __device__ __forceinline__ int64_t read_id(const void* p, int64_t at, int bytes)
   return bytes == 8 ? static_cast<const int64_t*>(p)[at] : static_cast<const int32_t*>(p)[at];
 }
 
+// Whether a row of a verify call lies behind its sequence's last draft's, where nothing is drawn.
+template <bool kVerify>
+__device__ __forceinline__ bool behind_drafts(const SampleParams& p, int row) {
+  if constexpr (!kVerify) return false;
+  const int set = row / p.group, j = row - set * p.group;
+  return j > 0 && j > read_id(p.num_drafts, set, p.id_bytes);
+}
+
 // w * 2^44 of a logit within reach of the maximum: 2^(u / 16) with u = 16 log2(e) (l - m) / T = 16 e + j + r, |r| <= 1/2,
 // from a table of 2^(j / 16 + 44), e added to its exponent, and five terms of the exponential series in r ln 2 / 16 (the
 // sixth is below 1.5e-13: a running sum is off by as little, against gaps of 1e-6 between a vocabulary's sums).
@@ -284,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     auto is_long = [&](int r) {
       const int s = r / p.group;
       const int k = p.top_k != nullptr ? __ldg(p.top_k + s) : 0;
-      return r < p.rows && __ldg(p.temperature + s) > 0.f && !(k > 0 && k <= kThreads / 2) &&
+      return __ldg(p.temperature + s) > 0.f && !behind_drafts<kVerify>(p, r) && !(k > 0 && k <= kThreads / 2) &&
              !(p.min_p != nullptr && __ldg(p.min_p + s) > 0.f);
     };
     bool is[kRowsPerThread];
@@ -304,6 +312,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     row = found_thread;
     __syncthreads();
   }
+  if (behind_drafts<kVerify>(p, row)) return;
   const int set = row / p.group;
   const float temp = __ldg(p.temperature + set);
   const bool greedy = !(temp > 0.f);
@@ -1179,7 +1188,7 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
-template <typename T>
+template <typename T, bool kVerify>
 __global__ void __launch_bounds__(256, 4) segment_kernel(const SampleParams p, Segment* __restrict__ segments,
                                                          int per_row) {
   using R = Row<T>;
@@ -1194,7 +1203,7 @@ __global__ void __launch_bounds__(256, 4) segment_kernel(const SampleParams p, S
   const int lane = threadIdx.x & 31;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int row = static_cast<int>(id / per_row), seg = static_cast<int>(id - static_cast<int64_t>(row) * per_row);
-  const bool any = row < p.rows;
+  const bool any = row < p.rows && !behind_drafts<kVerify>(p, row);
   uint4 x[kVectors];
   float temp = 0.f;
   const int e0 = seg * kSegment<T>;
@@ -1311,6 +1320,7 @@ __global__ void __launch_bounds__(kDrawThreads, 4) draw_kernel(const SampleParam
   __shared__ u64 found_rest;
   __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x;
+  if (behind_drafts<kVerify>(p, row)) return;
   const int set = row / p.group;
   const float temp = __ldg(p.temperature + set);
   const T* src = static_cast<const T*>(p.logits) + row * p.row_stride;
@@ -1568,7 +1578,7 @@ template <typename T, bool kVerify>
 cudaError_t launch_plain(const SampleParams& p, Segment* segments, cudaStream_t stream) {
   const int per_row = (p.vocab + kSegment<T> - 1) / kSegment<T>;
   const int64_t blocks = (static_cast<int64_t>(p.rows) * per_row + 7) / 8;
-  segment_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, segments, per_row);
+  segment_kernel<T, kVerify><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, segments, per_row);
   draw_kernel<T, kVerify><<<static_cast<unsigned>(p.rows), kDrawThreads, 0, stream>>>(p, segments, per_row);
   return cudaGetLastError();
 }
