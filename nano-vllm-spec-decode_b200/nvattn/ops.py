@@ -124,6 +124,12 @@ def _scale_block(k_cache, v_cache, k_scale, v_scale) -> int:
     return BS // blocks
 
 
+def _row_stride(x: torch.Tensor) -> int:
+    """The row stride of a matrix, for the C ABI, which refuses rows that overlap (an expanded view's are 0 apart).  A
+    single row has no stride to speak of: its width, whatever the view says."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
 def _is_fp8(k_cache, k_scale, v_scale) -> bool:
     return k_scale is not None or v_scale is not None or k_cache.dtype == torch.float8_e4m3fn
 
@@ -236,7 +242,7 @@ def _decode_fp8(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_tabl
         ws = _workspace(ws_bytes, q.device)
         _lib.check(lib.nva_paged_decode_fp8(
             q.data_ptr(), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            NB, BS, G, cache_seqlens.data_ptr(), block_table.data_ptr(), max(block_table.stride(0), block_table.shape[1]),
+            NB, BS, G, cache_seqlens.data_ptr(), block_table.data_ptr(), _row_stride(block_table),
             block_table.shape[1], B, n, H, KVH, D, float(softmax_scale), out.data_ptr(), out.stride(1), ws.data_ptr(),
             ws_bytes, _stream()), "paged decode (8-bit cache)")
     return out
@@ -272,7 +278,7 @@ def _varlen_fp8(q, k_cache, v_cache, k_scale, v_scale, max_seqlen_q, cu_seqlens_
         _lib.check(lib.nva_varlen_attention_fp8(
             q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
             NB, BS, G, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), B, Tq, int(max_seqlen_q),
-            block_table.data_ptr(), max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], H, KVH, D,
+            block_table.data_ptr(), _row_stride(block_table), block_table.shape[1], H, KVH, D,
             float(softmax_scale), out.data_ptr(), out.stride(0), ws.data_ptr(), ws_bytes, _stream()), "varlen attention (8-bit cache)")
     return out
 
@@ -412,7 +418,7 @@ def sample_tokens(logits: torch.Tensor, temperatures: torch.Tensor, uniforms: to
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device)
     with _on(logits.device):
         _lib.check(lib.nva_sample_tokens(
-            logits.data_ptr(), logits.stride(0) if R > 1 else max(logits.stride(0), V), R, V, logits.element_size(), t,
+            logits.data_ptr(), _row_stride(logits), R, V, logits.element_size(), t,
             k, p, m, uniforms.data_ptr(), uniforms.element_size(), ids.data_ptr(), ws.data_ptr() if ws_bytes else 0,
             ws_bytes, _stream()), "sample tokens")
     return ids
@@ -445,10 +451,10 @@ def verify_sampled(logits: torch.Tensor, draft_ids: torch.Tensor, num_drafts: to
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with _on(dev):
         _lib.check(lib.nva_verify_sampled(
-            logits.data_ptr(), max(logits.stride(0), V), S, K, V, logits.element_size(),
-            draft_ids.data_ptr() if K else 0, max(draft_ids.stride(0), K) if K else 0, num_drafts.data_ptr(),
+            logits.data_ptr(), _row_stride(logits), S, K, V, logits.element_size(),
+            draft_ids.data_ptr() if K else 0, _row_stride(draft_ids) if K else 0, num_drafts.data_ptr(),
             draft_ids.element_size(), t, k, p, m, accept_uniforms.data_ptr() if K else 0,
-            max(accept_uniforms.stride(0), K) if K else 0, uniforms.data_ptr(), uniforms.element_size(),
+            _row_stride(accept_uniforms) if K else 0, uniforms.data_ptr(), uniforms.element_size(),
             acc.data_ptr(), nxt.data_ptr(), ws.data_ptr(), ws_bytes, _stream()), "verify sampled")
     return acc, nxt
 

@@ -1,5 +1,6 @@
 """Host side of the 8-bit cache and of sampling without a GPU: what the wrappers refuse, the arguments they hand to the C
 ABI, the entry points' own refusals, and the float64 restatements against torch's e4m3 and against enumeration."""
+import ctypes
 import math
 
 import numpy as np
@@ -250,3 +251,69 @@ def test_speculative_sampling_draws_the_target_distribution(settings):
         total[d] += accepted
         # (a grid of N points is off by at most 1 / N per boundary)
         assert np.abs(total - p).max() <= 2 / N + 1e-12 or p[d] > 0.999
+
+
+# ---------------------------------------------------------------------------------------------- rows that overlap
+@pytest.fixture()
+def checked(rec, monkeypatch):
+    """The wrappers with the library's own argument checks behind them (the size queries alone, which ask for the
+    device, are answered here)."""
+    from nvattn import _lib
+    real = ctypes.CDLL(_lib.LIB_PATH)
+    for name, (res, args) in _lib.SIGNATURES.items():
+        fn = getattr(real, name)
+        fn.restype, fn.argtypes = res, args
+
+    class Checked:
+        nva_paged_attention_fp8_workspace_bytes = staticmethod(rec.nva_paged_attention_fp8_workspace_bytes)
+        nva_sample_workspace_bytes = staticmethod(rec.nva_sample_workspace_bytes)
+
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+    monkeypatch.setattr(_lib, "load", lambda: Checked())
+
+
+@pytest.mark.parametrize("what", ["block table", "varlen block table", "logits", "sample logits", "drafts", "one draft",
+                                  "accept uniforms"])
+def test_expanded_views_are_refused(checked, what):
+    """Rows that share memory have a stride of 0, which no call may take for a row's width: it would read past them."""
+    from nvattn import _lib, ops
+    c, (ks, vs) = cache()
+    q = torch.zeros(3, 2, 32, 128, dtype=torch.bfloat16)
+    lens, cu = torch.ones(3, dtype=torch.int32), torch.tensor([0, 2, 4, 6], dtype=torch.int32)
+    table = torch.zeros(1, 5, dtype=torch.int32).expand(3, -1)
+    S, K, V = 3, 1 if what == "one draft" else 2, 11
+    kw = dict(logits=torch.zeros(S * (K + 1), V), draft_ids=torch.zeros(S, K, dtype=torch.int64),
+              num_drafts=torch.ones(S, dtype=torch.int64), temperatures=torch.ones(S),
+              accept_uniforms=torch.zeros(S, K), uniforms=torch.zeros(S))
+    with pytest.raises(_lib.NvattnError, match="invalid argument"):
+        if what == "block table":
+            ops.flash_attn_with_kvcache(q, c, c, cache_seqlens=lens, block_table=table, softmax_scale=0.1, k_scale=ks,
+                                        v_scale=vs)
+        elif what == "varlen block table":
+            ops.flash_attn_varlen_func(q.view(6, 32, 128), c, c, 2, cu, 9, cu, 0.1, block_table=table, k_scale=ks,
+                                       v_scale=vs)
+        elif what == "sample logits":
+            ops.sample_tokens(torch.zeros(1, V).expand(S, V), torch.ones(S), torch.zeros(S))
+        else:
+            name = {"logits": "logits", "drafts": "draft_ids", "one draft": "draft_ids",
+                    "accept uniforms": "accept_uniforms"}[what]
+            kw[name] = kw[name][:1].expand(kw[name].shape)
+            ops.verify_sampled(**kw)
+
+
+def test_single_rows_need_no_stride(rec):
+    """One sequence: its rows' stride says nothing, also where a view makes it 0."""
+    from nvattn import ops
+    c, (ks, vs) = cache()
+    table = torch.zeros(5, dtype=torch.int32).as_strided((1, 5), (0, 1))
+    ops.flash_attn_with_kvcache(torch.zeros(1, 2, 32, 128, dtype=torch.bfloat16), c, c,
+                                cache_seqlens=torch.ones(1, dtype=torch.int32), block_table=table, softmax_scale=0.1,
+                                k_scale=ks, v_scale=vs)
+    ops.sample_tokens(torch.zeros(11).as_strided((1, 11), (0, 1)), torch.ones(1), torch.zeros(1))
+    ops.verify_sampled(torch.zeros(3, 11), torch.zeros(2, dtype=torch.int64).as_strided((1, 2), (0, 1)),
+                       torch.ones(1, dtype=torch.int64), torch.ones(1), torch.zeros(2).as_strided((1, 2), (0, 1)),
+                       torch.zeros(1))
+    (_, a), (_, s), (_, v) = rec.calls
+    assert a[11:13] == (5, 5) and s[1] == 11 and v[1] == 11 and v[7] == 2 and v[15] == 2
