@@ -10,9 +10,9 @@
 The first three also take an 8-bit cache: float8_e4m3fn k_cache / v_cache with k_scale= / v_scale= (float32
 [NB, KVH, BS / G], a power of two for each block of G consecutive slots and kv head; kvcache_scales() makes them).
 
-Every op runs on the caller's current CUDA stream, allocates only its output and never syncs.  The attention ops
-share one workspace per device (split-KV partials and the merge tickets, see _workspace); there is no CPU path:
-non-CUDA tensors raise.
+Every op runs on the caller's current CUDA stream, allocates only its output and never syncs (but for the first call of
+a size, which allocates).  The attention ops keep one workspace per device and stream and one per device for captured
+graphs (split-KV partials and the merge tickets, see _workspace); there is no CPU path: non-CUDA tensors raise.
 """
 import contextlib
 
@@ -43,55 +43,89 @@ def _need_cuda(*ts):
             raise ValueError("nvattn ops run on CUDA tensors only (no CPU fallback)")
 
 
-# device index -> the attention workspace in use; earlier (smaller) ones stay referenced because captured CUDA
-# graphs hold their addresses
-_WORKSPACES: dict[int, torch.Tensor] = {}
+# The attention workspaces in use, per device index i:
+#   i                   of calls on the default stream
+#   (i, stream)         of calls on another stream (its number)
+#   (i, _GRAPH)         of captured calls
+#   (i, _GRAPH, stream) of calls captured on a stream that reserve_workspace was given
+# Earlier (smaller) ones stay referenced because captured CUDA graphs hold their addresses.
+_WORKSPACES: dict = {}
 _RETIRED: list[torch.Tensor] = []
+_GRAPH = "graph"
 
 
-def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
-    """The decode / varlen workspace of a device.  Its merge-ticket words must be zero when a call starts and every
-    call leaves them zero, so it is allocated zero-filled once (grown, zero-filled, when a call needs more) and then
-    reused by every call and every captured graph.  Calls on one device are ordered by the stream they run on:
-    nano-vllm runs attention from one stream; concurrent streams on one device need their own workspaces through
-    the C ABI.  Growing it while a CUDA graph is being captured would allocate from the graph's pool and record the
-    zero-fill into every replay, so that raises instead: size it first with reserve_workspace (the nano-vllm drop-in
-    does so when the KV cache is allocated)."""
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    ws = _WORKSPACES.get(idx)
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _grow(key, nbytes: int, device: torch.device) -> torch.Tensor:
+    """The workspace under `key`, allocated zero-filled if there is none of that size."""
+    ws = _WORKSPACES.get(key)
     if ws is None or ws.numel() < nbytes:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError(f"nvattn: the attention workspace of cuda:{idx} must grow to {nbytes} bytes during a "
-                               "CUDA graph capture; call nvattn.ops.reserve_workspace(...) before capturing")
         if ws is not None:
             _RETIRED.append(ws)
         ws = torch.zeros(max(nbytes, 16), dtype=torch.uint8, device=device)
-        _WORKSPACES[idx] = ws
+        if isinstance(key, tuple) and key[1] is _GRAPH and ws.is_cuda:
+            torch.cuda.current_stream(device).synchronize()   # a replay may run on any stream: filled before it can
+        _WORKSPACES[key] = ws
+    return ws
+
+
+def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+    """The decode / varlen workspace of a call.  Its merge-ticket words must be zero when a call starts and every
+    call leaves them zero, so it is allocated zero-filled once (grown, zero-filled, when a call needs more) and then
+    reused.  Calls that may overlap must not share one: each stream has its own, and captured calls use another one of
+    the device, whatever stream their graph is replayed on.  Graphs share that one and are replayed one after another
+    (as those that share a memory pool are); to replay two at once, capture each on a stream of its own that
+    reserve_workspace was given.  Growing a workspace while a CUDA graph is being captured would allocate from the
+    graph's pool and record the zero-fill into every replay, so that raises instead: size it first with
+    reserve_workspace (the nano-vllm drop-in does so when the KV cache is allocated) or an eager call."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    stream = _raw_stream(idx)
+    if stream != 0 and torch.cuda.is_current_stream_capturing():
+        ws = _WORKSPACES.get((idx, _GRAPH, stream))
+        if ws is None:
+            ws = _WORKSPACES.get((idx, _GRAPH))
+        if ws is None or ws.numel() < nbytes:
+            raise RuntimeError(f"nvattn: the attention workspace of cuda:{idx} must grow to {nbytes} bytes during a "
+                               "CUDA graph capture; call nvattn.ops.reserve_workspace(...) before capturing")
+        return ws
+    key = (idx, stream) if stream != 0 else idx
+    ws = _WORKSPACES.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _grow(key, nbytes, device)
+        _grow((idx, _GRAPH), nbytes, device)
     return ws
 
 
 def reserve_workspace(max_num_seqs: int, max_num_tokens: int, num_heads: int, num_kv_heads: int,
-                      head_dim: int = 128, device: torch.device | None = None, fp8_cache: bool = False) -> int:
+                      head_dim: int = 128, device: torch.device | None = None, fp8_cache: bool = False,
+                      stream: torch.cuda.Stream | None = None) -> int:
     """Allocate (zero-filled) the workspace every later decode / verify / varlen call of up to max_num_seqs
-    sequences and max_num_tokens query rows needs on `device`, so that no call, captured or not, allocates; with
-    fp8_cache, also for calls over an 8-bit cache.  Returns its size in bytes.  nano-vllm: max_num_seqs and
-    max_num_batched_tokens of its Config."""
+    sequences and max_num_tokens query rows needs on `device`, so that no call on the current stream, and no captured
+    one, allocates; with fp8_cache, also for calls over an 8-bit cache.  With `stream`, calls captured on that stream
+    get a workspace of their own: a graph captured there may be replayed beside other graphs.  Returns its size in
+    bytes.  nano-vllm: max_num_seqs and max_num_batched_tokens of its Config."""
     device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     lib = _lib.load()
-    with torch.cuda.device(device):
+    with _on(device):
         need = max(lib.nva_varlen_workspace_bytes(max_num_seqs, max_num_tokens, num_heads, num_kv_heads, head_dim),
                    max(lib.nva_paged_decode_workspace_bytes(max_num_seqs, n, num_heads, num_kv_heads, head_dim)
                        for n in range(1, 49)))
         if fp8_cache:
             need = max(need, lib.nva_paged_attention_fp8_workspace_bytes(max_num_tokens, num_heads, num_kv_heads,
                                                                          head_dim))
-    return _workspace(need, device).numel()
+        size = _workspace(need, device).numel()
+        if stream is not None:
+            idx = device.index if device.index is not None else torch.cuda.current_device()
+            _grow((idx, _GRAPH, stream.cuda_stream), need, device)
+    return size
 
 
 def reset_workspaces() -> None:
     """Zero-fill every workspace again.  A call that gave up on a pipeline wait (bit 2 of the device error word) may
     leave merge tickets non-zero, after which later calls could merge split pieces wrongly; call this (outside any
-    graph capture, after clearing the error word) before going on."""
+    graph capture, with no call in flight, after clearing the error word) before going on."""
     for ws in list(_WORKSPACES.values()) + _RETIRED:
         ws.zero_()
 
