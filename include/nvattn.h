@@ -69,8 +69,9 @@ NVA_API int nva_store_kvcache(const void* key, int64_t key_row_stride, const voi
  * workspace >= nva_paged_decode_workspace_bytes().
  * Workspace contract: zero-fill it once before its first use (cudaMemset); every call leaves its first 256-byte
  * aligned block of merge tickets at zero again, so the same workspace serves every later call in stream order (also
- * nva_varlen_attention calls, and captured CUDA graphs).  Calls that may overlap on one device (different streams)
- * need separate workspaces.
+ * nva_varlen_attention calls, and captured CUDA graphs).  Calls that may overlap on one device (different streams,
+ * replays of two graphs) need separate workspaces, and a varlen call enqueues several kernels: host threads that share a
+ * workspace and a stream make their calls one after another.
  */
 NVA_API int nva_paged_decode(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
                              int32_t num_blocks, int32_t block_size, const int32_t* context_lens,

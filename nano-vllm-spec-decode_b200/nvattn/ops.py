@@ -15,6 +15,7 @@ a size, which allocates).  The attention ops keep one workspace per device and s
 graphs (split-KV partials and the merge tickets, see _workspace); there is no CPU path: non-CUDA tensors raise.
 """
 import contextlib
+import threading
 
 import torch
 
@@ -52,6 +53,11 @@ def _need_cuda(*ts):
 _WORKSPACES: dict = {}
 _RETIRED: list[torch.Tensor] = []
 _GRAPH = "graph"
+
+# Held from taking a workspace to the end of the call that uses it: a call is up to four kernels that pass pieces and a
+# plan on through its workspace, and another host thread's on the same stream must not come between them (ctypes lets
+# other threads run during a call).
+_CALL = threading.RLock()
 
 
 def _raw_stream(index: int) -> int:
@@ -115,10 +121,11 @@ def reserve_workspace(max_num_seqs: int, max_num_tokens: int, num_heads: int, nu
         if fp8_cache:
             need = max(need, lib.nva_paged_attention_fp8_workspace_bytes(max_num_tokens, num_heads, num_kv_heads,
                                                                          head_dim))
-        size = _workspace(need, device).numel()
-        if stream is not None:
-            idx = device.index if device.index is not None else torch.cuda.current_device()
-            _grow((idx, _GRAPH, stream.cuda_stream), need, device)
+        with _CALL:
+            size = _workspace(need, device).numel()
+            if stream is not None:
+                idx = device.index if device.index is not None else torch.cuda.current_device()
+                _grow((idx, _GRAPH, stream.cuda_stream), need, device)
     return size
 
 
@@ -242,11 +249,12 @@ def flash_attn_with_kvcache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     ws_bytes = lib.nva_paged_decode_workspace_bytes(B, n, H, KVH, D)
     if ws_bytes == 0:
         raise _lib.NvattnError(f"paged decode does not support q_per_seq={n} with {H // KVH} q heads per kv head")
-    ws = _workspace(ws_bytes, q.device)
-    _lib.check(lib.nva_paged_decode(
-        q.data_ptr(), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), NB, BS, cache_seqlens.data_ptr(),
-        block_table.data_ptr(), block_table.stride(0), B, n, H, KVH, D, float(softmax_scale), out.data_ptr(),
-        out.stride(1), ws.data_ptr(), ws_bytes, _stream()), "paged decode")
+    with _CALL:
+        ws = _workspace(ws_bytes, q.device)
+        _lib.check(lib.nva_paged_decode(
+            q.data_ptr(), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), NB, BS, cache_seqlens.data_ptr(),
+            block_table.data_ptr(), block_table.stride(0), B, n, H, KVH, D, float(softmax_scale), out.data_ptr(),
+            out.stride(1), ws.data_ptr(), ws_bytes, _stream()), "paged decode")
     return out
 
 
@@ -273,12 +281,13 @@ def _decode_fp8(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_tabl
         if ws_bytes == 0:
             raise _lib.NvattnError(f"paged decode over an 8-bit cache does not support {H // KVH} q heads per kv head "
                                    f"with head_dim {D}")
-        ws = _workspace(ws_bytes, q.device)
-        _lib.check(lib.nva_paged_decode_fp8(
-            q.data_ptr(), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            NB, BS, G, cache_seqlens.data_ptr(), block_table.data_ptr(), _row_stride(block_table),
-            block_table.shape[1], B, n, H, KVH, D, float(softmax_scale), out.data_ptr(), out.stride(1), ws.data_ptr(),
-            ws_bytes, _stream()), "paged decode (8-bit cache)")
+        with _CALL:
+            ws = _workspace(ws_bytes, q.device)
+            _lib.check(lib.nva_paged_decode_fp8(
+                q.data_ptr(), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                v_scale.data_ptr(), NB, BS, G, cache_seqlens.data_ptr(), block_table.data_ptr(),
+                _row_stride(block_table), block_table.shape[1], B, n, H, KVH, D, float(softmax_scale), out.data_ptr(),
+                out.stride(1), ws.data_ptr(), ws_bytes, _stream()), "paged decode (8-bit cache)")
     return out
 
 
@@ -308,12 +317,14 @@ def _varlen_fp8(q, k_cache, v_cache, k_scale, v_scale, max_seqlen_q, cu_seqlens_
         if ws_bytes == 0:
             raise _lib.NvattnError(f"varlen attention over an 8-bit cache does not support {H // KVH} q heads per kv "
                                    f"head with head_dim {D}")
-        ws = _workspace(ws_bytes, q.device)
-        _lib.check(lib.nva_varlen_attention_fp8(
-            q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            NB, BS, G, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), B, Tq, int(max_seqlen_q),
-            block_table.data_ptr(), _row_stride(block_table), block_table.shape[1], H, KVH, D,
-            float(softmax_scale), out.data_ptr(), out.stride(0), ws.data_ptr(), ws_bytes, _stream()), "varlen attention (8-bit cache)")
+        with _CALL:
+            ws = _workspace(ws_bytes, q.device)
+            _lib.check(lib.nva_varlen_attention_fp8(
+                q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                v_scale.data_ptr(), NB, BS, G, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), B, Tq,
+                int(max_seqlen_q), block_table.data_ptr(), _row_stride(block_table), block_table.shape[1], H, KVH, D,
+                float(softmax_scale), out.data_ptr(), out.stride(0), ws.data_ptr(), ws_bytes, _stream()),
+                "varlen attention (8-bit cache)")
     return out
 
 
@@ -357,11 +368,13 @@ def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ma
         kp, kst, vp, vst = k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0)
         kc, vc, bt, bts = 0, 0, 0, 0
     ws_bytes = lib.nva_varlen_workspace_bytes(B, Tq, H, KVH, D)
-    ws = _workspace(ws_bytes, q.device)
-    _lib.check(lib.nva_varlen_attention(
-        q.data_ptr(), q.stride(0), kp, kst, vp, vst, kc, vc, NB, BS, cu_seqlens_q.data_ptr(),
-        cu_seqlens_k.data_ptr(), B, Tq, Tk, int(max_seqlen_q), int(max_seqlen_k), bt, bts, H, KVH, D,
-        float(softmax_scale), out.data_ptr(), out.stride(0), ws.data_ptr(), ws_bytes, _stream()), "varlen attention")
+    with _CALL:
+        ws = _workspace(ws_bytes, q.device)
+        _lib.check(lib.nva_varlen_attention(
+            q.data_ptr(), q.stride(0), kp, kst, vp, vst, kc, vc, NB, BS, cu_seqlens_q.data_ptr(),
+            cu_seqlens_k.data_ptr(), B, Tq, Tk, int(max_seqlen_q), int(max_seqlen_k), bt, bts, H, KVH, D,
+            float(softmax_scale), out.data_ptr(), out.stride(0), ws.data_ptr(), ws_bytes, _stream()),
+            "varlen attention")
     return out
 
 

@@ -91,7 +91,49 @@ def test_growing_keeps_what_graphs_hold(at):
     assert ops._workspace(128, DEV) is not small and any(x is small for x in ops._RETIRED)
 
 
-# ---------------------------------------------------------------------------------------------- calls in flight together
+@pytest.mark.parametrize("fp8", [True, False])
+def test_host_threads_take_turns(at, monkeypatch, fp8):
+    """The kernels of a call follow one another through one workspace: no other thread's call begins between them."""
+    import threading
+    import time
+    from nvattn import _lib, ops
+    inside, worst = [0], [0]
+
+    class Lib(_Sizes):
+        def __getattr__(self, name):
+            def call(*args):
+                inside[0] += 1
+                worst[0] = max(worst[0], inside[0])
+                time.sleep(0.01)
+                inside[0] -= 1
+                return 0
+            return call
+
+    monkeypatch.setattr(_lib, "load", lambda: Lib())
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: None)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    at(0)
+    workspace = ops._workspace
+    monkeypatch.setattr(ops, "_workspace", lambda nbytes, device: workspace(nbytes, DEV))
+    c = torch.zeros(2, 256, 8, 128, dtype=torch.float8_e4m3fn if fp8 else torch.bfloat16)
+    kw = dict(zip(("k_scale", "v_scale"), ops.kvcache_scales(c))) if fp8 else {}
+    q, lens = torch.zeros(3, 1, 32, 128, dtype=torch.bfloat16), torch.ones(3, dtype=torch.int32)
+    cu, table = torch.arange(4, dtype=torch.int32), torch.zeros(3, 2, dtype=torch.int32)
+
+    def work():
+        for _ in range(3):
+            ops.flash_attn_with_kvcache(q, c, c, cache_seqlens=lens, block_table=table, softmax_scale=0.1, **kw)
+            ops.flash_attn_varlen_func(q[:, 0], c, c, 1, cu, 1, cu, 0.1, block_table=table, **kw)
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert worst[0] == 1
+
+
+# ------------------------------------------------------------------------------------------- calls in flight together
 def calls(seed, fp8):
     """A decode batch and a mixed one whose sequences are cut over many CTAs; returns a function that runs both."""
     from nvattn import ops
