@@ -1541,6 +1541,18 @@ __global__ void __launch_bounds__(128) verify_merge_kernel(const int2* __restric
   next[s] = static_cast<I>(r.x);
 }
 
+constexpr int kShareWords = 38 * kThreads;   // of a row per CTA, while more CTAs can be had
+
+// Words per thread of a CTA that holds `words` of a row.
+constexpr int run_words(int words) { return ((words + kThreads - 1) / kThreads) | 1; }
+constexpr int share_bytes(int words) {
+  return std::max(run_words(words) * kThreads * 4, kShort * static_cast<int>(sizeof(u64)));
+}
+// The most that a call of the type needs: an eighth of the largest vocabulary, or a CTA's share.
+template <typename T>
+constexpr int kMostBytes = share_bytes(
+    std::max(kShareWords, (NVA_MAX_SAMPLE_VOCAB / Row<T>::kPerWord + kMaxCluster - 1) / kMaxCluster));
+
 template <typename T, bool kVerify>
 cudaError_t launch_rows(SampleParams p, int sms, cudaStream_t stream) {
   constexpr int kPer = Row<T>::kPerWord;
@@ -1550,20 +1562,20 @@ cudaError_t launch_rows(SampleParams p, int sms, cudaStream_t stream) {
   // a cluster's lie in one part of the chip.  151,936 in bf16, 4 and 8 CTAs a row: top-p 12 rows 50 and 35 us, 16 rows 50
   // and 49; top-k 12 rows 17.7 and 16.6, 16 rows 17.2 and 20.7.
   int cluster = 1;
-  while (cluster < kMaxCluster && (words > cluster * 38 * kThreads ||
+  while (cluster < kMaxCluster && (words > cluster * kShareWords ||
                                    (3 * static_cast<int64_t>(p.rows) * cluster <= sms && words >= cluster * 2048)))
     cluster *= 2;
   const int per_cta = (words + cluster - 1) / cluster;
-  p.run_words = ((per_cta + kThreads - 1) / kThreads) | 1;
+  p.run_words = run_words(per_cta);
   p.by_work = static_cast<int64_t>(p.rows) * cluster > 2 * sms && p.rows <= kRowsPerThread * kThreads ? 1 : 0;
-  const size_t smem = std::max(static_cast<size_t>(p.run_words) * kThreads * 4, kShort * sizeof(u64));
   auto kernel = sample_kernel<T, kVerify>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  // (the same for every call: the limit is the function's, and another thread's smaller call may come before the launch)
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes<T>);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * cluster);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = static_cast<size_t>(share_bytes(per_cta));
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -389,3 +389,36 @@ def test_calls_on_two_streams_at_once(cuda):
                 got.append(sample_tokens(x, t, u, **kw))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_calls_of_two_host_threads(cuda):
+    """Calls of very different sizes from threads at once: the shared memory that one asks for does not limit the
+    other's.  Through the C ABI, so that the threads are in the library at the same time for the most part."""
+    import threading
+    from nvattn import _lib
+    from nvattn.sampler import sample_tokens
+    lib = _lib.load()
+    cases = []
+    for R, V in ((1, 151936), (70, 1000), (1, 151936), (70, 1000)):
+        x, g = rows(R, V, torch.float32, V)
+        x, t, p, u = (a.cuda() for a in (x, torch.ones(R), torch.full((R,), 0.9), torch.rand(R, generator=g)))
+        cases.append((x, t, u, p, sample_tokens(x, t, u, top_p=p), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(x, t, u, p, want, stream):
+        ids = torch.empty_like(want)
+        args = (x.data_ptr(), x.shape[1], x.shape[0], x.shape[1], 4, t.data_ptr(), 0, p.data_ptr(), 0, u.data_ptr(), 4,
+                ids.data_ptr(), 0, 0, stream.cuda_stream)
+        torch.cuda.set_device(0)
+        status = [lib.nva_sample_tokens(*args) for _ in range(8000)]
+        stream.synchronize()
+        if any(status) or not torch.equal(ids, want):
+            failed.append((x.shape, sum(s != 0 for s in status)))
+
+    threads = [threading.Thread(target=work, args=c) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert failed == []
