@@ -422,3 +422,17 @@ def test_calls_of_two_host_threads(cuda):
     for t in threads:
         t.join()
     assert failed == []
+
+
+@pytest.mark.parametrize("V,dtype", [(393216, torch.float32), (393216, torch.bfloat16), (262144, torch.float32)])
+def test_the_largest_vocabularies(cuda, V, dtype):
+    """Up to the largest that the calls take (include/nvattn.h), whose rows fill the shared memory of eight CTAs."""
+    R = 2
+    x, g = rows(R, V, dtype, 77)
+    u, t = torch.rand(R, generator=g, dtype=torch.float64), torch.rand(R, generator=g) + 0.4
+    check(x, t, u)
+    check(x, t, u, top_p=torch.full((R,), 0.95))
+    check(x, t, u, top_k=torch.tensor([50, 6000]).int(), min_p=torch.full((R,), 0.001))
+    d = torch.stack([x[0].argmax(), x[1].argmin()]).view(2, 1)
+    check_verify(x.repeat_interleave(2, 0), d, torch.ones(2, dtype=torch.int64), t, torch.full((2, 1), 0.001), u.float(),
+                 top_p=torch.full((R,), 0.95))
