@@ -1127,6 +1127,10 @@ int tile_rows(int64_t rows) {
   return rows <= 8 ? 8 : rows >= kMaxRows8 ? kMaxRows8 : static_cast<int>((rows + 7) / 8 * 8);
 }
 
+// The kernel for runs of up to max_q queries: one at least (a bound of 0 says nothing about the runs there are), so that a
+// tile holds a query's whole group.
+int rows_for(int32_t max_q, int group) { return tile_rows(static_cast<int64_t>(std::max(max_q, 1)) * group); }
+
 // Query runs of at least this many tokens take the prefill kernel, which gives each q head 128 rows of its own and costs
 // the same for 33 queries as for 128, while here every 32 packed rows are walked anew.  32 q heads over 8, here and there:
 // 4 runs of 64 over 1000 keys 45 and 35 us, 32 such runs 219 and 152, 8 over 8000 keys 239 and 277; runs of 48: 40 and 35,
@@ -1248,7 +1252,7 @@ NVA_API size_t nva_paged_attention_fp8_workspace_bytes(int32_t max_q, int32_t nu
     return 0;
   const int sms = nva::sm_count();
   const int group = num_heads / num_kv_heads;
-  return sms == 0 ? 0 : nva::workspace8(sms, nva::tile_rows(static_cast<int64_t>(max_q) * group), group);
+  return sms == 0 ? 0 : nva::workspace8(sms, nva::rows_for(max_q, group), group);
 }
 
 NVA_API int nva_paged_decode_fp8(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
@@ -1269,7 +1273,7 @@ NVA_API int nva_paged_decode_fp8(const void* q, int64_t q_row_stride, const void
   if (rc != NVA_OK) return rc;
   if (context_lens == nullptr) return NVA_ERR_INVALID_ARGUMENT;
   if (static_cast<int64_t>(num_seqs) * q_per_seq >= (int64_t(1) << 31)) return NVA_ERR_UNSUPPORTED;
-  const int nr = nva::tile_rows(static_cast<int64_t>(q_per_seq) * (num_heads / num_kv_heads));
+  const int nr = nva::rows_for(q_per_seq, num_heads / num_kv_heads);
   nva::Fp8DecodeParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_row_stride = q_row_stride;
@@ -1327,7 +1331,7 @@ NVA_API int nva_varlen_attention_fp8(const void* q, int64_t q_row_stride, const 
   p.block_size = block_size;
   p.num_blocks = num_blocks;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  const int nr = nva::tile_rows(static_cast<int64_t>(max_seqlen_q) * p.group);
+  const int nr = nva::rows_for(max_seqlen_q, p.group);
   // Long runs: the prefill kernel, as far as its plan holds the call (1024 sequences, 4096 query tiles).
   const int64_t tiles = static_cast<int64_t>(total_q) / 128 + num_seqs + 1;
   const bool prefill = max_seqlen_q >= nva::kMinPrefillRun && num_seqs <= nva::kMaxDecodeSeqs &&

@@ -351,3 +351,16 @@ def test_split_calls_in_a_row_and_replayed(cuda):
         for o, w in zip(outs, want):
             assert torch.equal(o, w), i
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("H", [16, 9, 40, 8])
+def test_varlen_bound_of_zero(cuda, H):
+    """A bound of 0 on runs that are there, with more q heads per kv head than the smallest tile has rows."""
+    from nvattn import _lib, ops
+    lib = _lib.load()
+    assert lib.nva_paged_attention_fp8_workspace_bytes(0, H, 1, 128) == \
+        lib.nva_paged_attention_fp8_workspace_bytes(1, H, 1, 128)
+    b = make([300, 77, 5], H=H, KVH=1, qlens=[90, 3, 1], seed=40)
+    check(b, got=ops.flash_attn_varlen_func(b["q"], *b["c"], max_seqlen_q=0, cu_seqlens_q=b["cu_q"], max_seqlen_k=300,
+                                            cu_seqlens_k=b["cu_k"], softmax_scale=b["scale"], block_table=b["table"],
+                                            k_scale=b["s"][0], v_scale=b["s"][1]))
