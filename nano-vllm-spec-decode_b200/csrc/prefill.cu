@@ -461,7 +461,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             const int64_t at = (page * static_cast<int64_t>(p.num_kv_heads) + kvh) * p.page_blocks +
                                ((j * 128 % p.block_size + t) >> p.lg_block);
             ks = __ldg(p.k_scale + at);
-            vs = __ldg(p.v_scale + at);
+            vs = fminf(fmaxf(__ldg(p.v_scale + at), 9.094947e-13f), 1.0995116e12f);   // 2^-40 .. 2^40, as for short runs
           }
         };
         load_scales(0, page_of(0));

@@ -364,3 +364,16 @@ def test_varlen_bound_of_zero(cuda, H):
     check(b, got=ops.flash_attn_varlen_func(b["q"], *b["c"], max_seqlen_q=0, cu_seqlens_q=b["cu_q"], max_seqlen_k=300,
                                             cu_seqlens_k=b["cu_k"], softmax_scale=b["scale"], block_table=b["table"],
                                             k_scale=b["s"][0], v_scale=b["s"][1]))
+
+
+@pytest.mark.parametrize("scale,taken", [(0.0, 2.0 ** -40), (2.0 ** -60, 2.0 ** -40), (float("nan"), 2.0 ** -40),
+                                         (2.0 ** 50, 2.0 ** 40), (float("inf"), 2.0 ** 40)])
+@pytest.mark.parametrize("qlen", [3, 63, 64, 200])
+def test_v_scales_out_of_range(cuda, scale, taken, qlen):
+    """They count as the bounds of the range, whichever kernel takes the run."""
+    b = make([300], qlens=[qlen], seed=41)
+    b["s"][1].fill_(taken)
+    want, bound = ref(b)
+    b["s"][1].fill_(scale)
+    got = run(b)
+    assert ((got.double() - want).abs() <= bound).all()
