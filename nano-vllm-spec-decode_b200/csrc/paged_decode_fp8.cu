@@ -5,16 +5,20 @@
 // The cache holds e4m3 values c with a float32 scale per (block of tokens, kv head): k = kc * ks, v = vc * vs.
 //     x[r, t]  = (q[r] . kc[t]) * ks[t] * softmax_scale * log2(e)         score in log2 units
 //     y[r, t]  = x[r, t] + log2 vs[t]                                     the scale of v moved into the exponent
-//     w[r, t]  = 2^(y - m[r] + 8)         m: running row maximum of y
+//     w[r, t]  = 2^(y - m[r] + 12)        m: running row maximum of y
 //     out[r]   = sum_t w[r, t] vc[t] / sum_t w[r, t] / vs[t]
 // so neither k nor v is ever multiplied out: both products read the cache's own bytes on the 8-bit tensor pipe, and one
 // pass over K and V serves every q head of the group and every query row.  The other operand of each product is split
-// into two 8-bit parts that accumulate into the same TMEM columns, which keeps the 16-bit kernels' accuracy:
+// into 8-bit parts that accumulate into the same TMEM columns, which keeps the 16-bit kernels' accuracy:
 //   q  = (hi + lo) * 2^e, both e4m3, e from the row's largest value: four significant bits each, together all eight of a
 //        bf16 value (exact for values down to 2^-10 of the row's largest, off by at most 2^-18 of that below);
-//   w  = hi + lo, hi rounded to e5m2 (three bits, range to 2^-16), lo the rest in e4m3: off by at most 2^-7 of w
-//        (0.12% rms, bf16's rounding is 0.16%) and never below 2^-17 where the row's largest is 2^8 to 2^11, so tokens
-//        down to 2^-25 of the largest weight still count.  Sums of weights stay in float32, unrounded.
+//   w  rounded to float16, whose eleven bits are the sum of three e5m2 parts of three bits and their signs (the upper
+//        byte of a float16 is an e5m2 value, so that splitting takes integer operations on pairs): off by at most 2^-11
+//        of w (bf16's rounding: 2^-8) and by 2^-17, the parts' smallest step, where the row's largest is 2^12 to 2^15.
+//        So weights keep seven bits down to 2^-22 of the largest, and the 2^-17 of every one of 100,000 tokens that are
+//        all rounded the same way come to 2^-12 of it.  Two parts, e5m2 and a rest in e4m3, had no more than three bits
+//        below 2^-15 of the largest: a long flat tail behind one heavy token was off by up to a tenth of itself.  Sums of
+//        weights stay in float32, unrounded.
 //
 // Bound: HBM, one byte per cached value (decode of 64 sequences, contexts 512 to 4096: 303 MB, 46 us at the copy rate).  A 128-token tile then takes 0.74 us of an SM's share of the bandwidth, half of the bf16 cache's, which is
 // less than one tile's chain S -> weights -> PV takes; so two CTAs share an SM and their chains overlap.
@@ -54,9 +58,9 @@ constexpr int kInfoRing = 8;            // tile descriptors; the producer is at 
 constexpr int kQScaleRing = 8;          // row scales by segment; the Q loader is at most 4 segments ahead
 constexpr int kMaxRows8 = 40;           // packed query rows (queries x group) of a tile
 constexpr int kSegCost = 3;             // a segment's start and end, in tiles
-constexpr float kBase = 8.0f;           // the largest weight of a row is 2^kBase when its maximum is exact ...
+constexpr float kBase = 12.0f;          // the largest weight of a row is 2^kBase when its maximum is exact ...
 constexpr float kSlack = 3.0f;          // ... and may pass it by this much (log2) before the maximum moves
-constexpr float kWeightMax = 2048.0f;   // 2^(kBase + kSlack): lo <= 2^-3 w stays inside e4m3's range
+constexpr float kWeightMax = 32768.0f;  // 2^(kBase + kSlack): inside float16's range
 
 // NR: the most query rows a softmax thread carries.  One softmax group of 128 threads at 128 registers each: at 40 rows
 // (weights and sums of 40 rows, 80 registers) nothing spills; with more rows they spill past an L1 that two CTAs' shared
@@ -69,11 +73,11 @@ struct Cfg8 {
   static constexpr int kKStages = NP == 16 ? 3 : 2;
   static constexpr int kVStages = 2;
   static constexpr int kQBuf = 2;
-  static constexpr int kPBuf = 2;
-  // hi and lo of Q: NR rows (a UMMA wider than that reads the bytes behind them into columns nobody looks at); of P^T:
-  // 16-row chunks
+  static constexpr int kPBuf = NP == 48 ? 1 : 2;
+  // hi and lo of Q: NR rows (a UMMA wider than that reads the bytes behind them into columns nobody looks at); the three
+  // parts of P^T: 16-row chunks
   static constexpr int kQHalf = (NR < 16 ? 16 : NR) * 128, kQBytes = 2 * kQHalf;
-  static constexpr int kPHalf = NP * 128, kPBytes = 2 * kPHalf;
+  static constexpr int kPPart = NP * 128, kPBytes = 3 * kPPart;
   static constexpr int kTmemCols = NP == 16 ? 64 : NP == 32 ? 128 : 256;   // S, O double buffered: 4 NP, a power of two
   static constexpr int kK = 0;
   static constexpr int kV = kK + kKStages * kTile;
@@ -104,7 +108,7 @@ enum {
   B_QFULL = 18, B_QEMPTY = 20, B_INFO = 22, B_KSTART = 30
 };
 
-// The f8f6f4 instruction descriptor: float32 accumulator, A e4m3, B e4m3 or e5m2.
+// The f8f6f4 instruction descriptor: float32 accumulator, A e4m3, B e4m3 (q) or e5m2 (weights).
 __host__ __device__ constexpr uint32_t idesc_f8(int N, bool b_e5m2, bool mn_major) {
   return (1u << 4) | (0u << 7) | (static_cast<uint32_t>(b_e5m2) << 10) | (static_cast<uint32_t>(mn_major) << 15) |
          (static_cast<uint32_t>(mn_major) << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (8u << 24);
@@ -119,16 +123,21 @@ __device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t a, uint64_t
       : "memory");
 }
 
-// Two floats to two packed 8-bit values, the first in the low byte (nearest even, saturating).
+// Two floats to two packed e4m3 values, the first in the low byte (nearest even, saturating).
 __device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
-}
-__device__ __forceinline__ uint32_t pack_e5m2(float lo, float hi) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E5M2);
 }
 __device__ __forceinline__ float2 unpack_e4m3(uint32_t v) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v & 0xFFFFu), __NV_E4M3);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// A pair of float16 numbers to the nearest ones of three significant bits (half up in magnitude; subnormal ones to
+// multiples of 2^-16): their upper bytes as e5m2.  No carry leaves a number: magnitudes are at most 2^15.
+__device__ __forceinline__ uint32_t round_e5m2(uint32_t h2) { return (h2 + 0x00800080u) & 0xFF00FF00u; }
+__device__ __forceinline__ uint32_t sub_h2(uint32_t a, uint32_t b) {
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&d);
 }
 
 struct Shape8 {
@@ -624,18 +633,18 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       const int flags = info[3 * e + 2].x;
       if ((flags & 1) && pv > 0) oseg ^= 1;
       const int width = min(NP, mma_width(info[3 * e + 1].x * G));
-      const uint32_t idesc_hi = idesc_f8(width, true, true), idesc_lo = idesc_f8(width, false, true);
+      const uint32_t idesc = idesc_f8(width, true, true);
       tc_fence_after();
       if (elect_one()) {
         const uint64_t a = v_desc0 + ((st * kTile) >> 4);
-        const uint64_t b = p_desc0 + ((pb * C::kPBytes) >> 4);
+        const uint64_t b = p_desc0 + ((pv % C::kPBuf * C::kPBytes) >> 4);
         const uint32_t d = tmem + (2 + oseg) * NP;
         const uint32_t fresh = (flags & 1) ? 0u : 1u;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)   // 32 tokens a step: four groups of 8 (V: 1024 bytes each, P^T: 128)
-          umma_f8_ss(d, a + 256 * k, b + 32 * k, idesc_hi, k > 0 ? 1u : fresh);
+        for (int part = 0; part < 3; ++part)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_f8_ss(d, a + 256 * k, b + (C::kPHalf >> 4) + 32 * k, idesc_lo, 1u);
+          for (int k = 0; k < 4; ++k)   // 32 tokens a step: four groups of 8 (V: 1024 bytes each, P^T: 128)
+            umma_f8_ss(d, a + 256 * k, b + ((part * C::kPPart) >> 4) + 32 * k, idesc, part + k > 0 ? 1u : fresh);
         umma_commit(&bars[B_OFULL + pb]);
         umma_commit(&bars[B_VEMPTY + st]);
       }
@@ -894,8 +903,9 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
               tc_fence_before();
             }
           }
-          // P(jj) goes where PV(jj - 2) read
-          if (jj >= 2) alive = alive && mbar_wait_warp(&bars[B_OFULL + buf], ((jj - 2) >> 1) & 1, abort);
+          // P(jj) goes where PV(jj - kPBuf) read
+          if (jj >= C::kPBuf)
+            alive = alive && mbar_wait_warp(&bars[B_OFULL + ((jj - C::kPBuf) & 1)], ((jj - C::kPBuf) >> 1) & 1, abort);
           // rows past the piece's keys may hold anything, NaN too: zero V there, so that no weight of 0 meets it
           if (L - tok0 < kTileTokens) {
             alive = alive && mbar_wait_warp(&bars[B_VFULL + st], (jj / C::kVStages) & 1, abort);
@@ -906,26 +916,33 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             }
           }
           if (alive) {
-            // P^T: hi rounded to three significant bits (half up), lo = w - hi exactly; 8 rows of token ct are 8 bytes
-            uint8_t* pb = smem + C::kP + buf * C::kPBytes + ct * 16;
+            // P^T: the three parts of the weights in float16; 8 rows of token ct are 8 bytes
+            uint8_t* pb = smem + C::kP + jj % C::kPBuf * C::kPBytes + ct * 16;
 #pragma unroll
             for (int m = 0; m < HR / 8; ++m) {
-              uint32_t hi[2], lo[2];
+              uint32_t part[3][2];
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                float t[4], u[4];
+                uint32_t x[2], y[2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float w = s[8 * m + 4 * h + i];
-                  t[i] = __uint_as_float((__float_as_uint(w) + 0x00100000u) & 0xFFE00000u);
-                  u[i] = w - t[i];
+                for (int i = 0; i < 2; ++i) {
+                  const int r = 8 * m + 4 * h + 2 * i;
+                  const __half2 w = __floats2half2_rn(s[r], s[r + 1]);
+                  x[i] = *reinterpret_cast<const uint32_t*>(&w);
                 }
-                hi[h] = pack_e5m2(t[0], t[1]) | (pack_e5m2(t[2], t[3]) << 16);
-                lo[h] = pack_e4m3(u[0], u[1]) | (pack_e4m3(u[2], u[3]) << 16);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) {
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) y[i] = k < 2 ? round_e5m2(x[i]) : x[i] + 0x00800080u;
+                  part[k][h] = __byte_perm(y[0], y[1], 0x7531);   // the upper bytes
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) x[i] = sub_h2(x[i], y[i]);   // (exact; the last one is not used)
+                }
               }
               uint8_t* at = pb + (m >> 1) * 2048 + (m & 1) * 8;
-              *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
-              *reinterpret_cast<uint2*>(at + C::kPHalf) = make_uint2(lo[0], lo[1]);
+#pragma unroll
+              for (int k = 0; k < 3; ++k)
+                *reinterpret_cast<uint2*>(at + k * C::kPPart) = make_uint2(part[k][0], part[k][1]);
             }
             fence_proxy_async_smem();
             mbar_arrive(&bars[B_PFULL + buf]);

@@ -64,11 +64,12 @@ def values(cache: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
 def attention_ref(q, k, v, scale):
     """q [n, H, D], k / v [L, KVH, D] (float64) -> (out, bound) [n, H, D], causal from the bottom right.
 
-    The bound, per element: the output is rounded to bf16 (half a step, 2^-8 relative).  The kernel's weights are each
-    off by at most 2^-7 relative (an e5m2 part, half a step 2^-3, and its rest in e4m3, half a step 2^-4), so the
-    weighted sum by at most 2^-7 of sum p |v|; a weight below 2^-25 of the row's largest may vanish (2^-24 is taken for
-    each token: L * 2^-24 of the largest |v|).  Scores are float32 sums of 128 exact products: off by at most
-    130 * 2^-24 of sum |q k| (in natural units after the scale), and the exponential and the running sums by 2^-20."""
+    The bound, per element: the output is rounded to bf16 (half a step, 2^-8 relative).  The kernels' weights are
+    rounded to bf16 (long runs: half a step, 2^-8 of a weight, as its leading bit may be the least) or to float16, kept
+    as three e5m2 parts (short runs: 2^-11), so the weighted sum is off by at most 2^-8 of sum p |v|; the parts' smallest
+    step is 2^-16 where the row's largest weight is 2^12 at least: half of it, 2^-29 of the largest, for each token, times
+    the largest |v|.  Scores are float32 sums of 128 exact products: off by at most 130 * 2^-24 of sum |q k| (in natural
+    units after the scale), and the exponential and the running sums by 2^-20."""
     n, H, D = q.shape
     L, KVH, _ = k.shape
     G = H // KVH
@@ -90,7 +91,7 @@ def attention_ref(q, k, v, scale):
         mass = p @ vh.abs()
         score = 130 * 2.0 ** -24 * scale * (q[:, h].abs() @ kh.abs().T).masked_fill(hidden, 0).amax(-1, keepdim=True)
         big = vh.abs().amax() * p.amax(-1, keepdim=True)
-        bound[:, h] = 2.0 ** -8 * out[:, h].abs() + (2.0 ** -7 + 2 * score + 2.0 ** -20) * mass + L * 2.0 ** -24 * big
+        bound[:, h] = 2.0 ** -8 * out[:, h].abs() + (2.0 ** -8 + 2 * score + 2.0 ** -20) * mass + L * 2.0 ** -29 * big
     return out, bound + 1e-30
 
 

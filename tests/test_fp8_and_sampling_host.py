@@ -253,6 +253,28 @@ def test_speculative_sampling_draws_the_target_distribution(settings):
         assert np.abs(total - p).max() <= 2 / N + 1e-12 or p[d] > 0.999
 
 
+def test_three_parts_of_a_weight():
+    """The 8-bit attention kernels' weights, bit by bit: float16, then three times the nearest number of three
+    significant bits (the upper byte, an e5m2 value) and the rest.  float16 loses 2^-11 of the weight at most (2^-25 of
+    subnormal ones), the parts half their smallest step, 2^-17."""
+    w = np.concatenate([np.exp2(np.random.default_rng(0).uniform(-30, 15, 200000)), np.exp2(np.arange(-30, 16.0)),
+                        np.float16(np.arange(0x7801, dtype=np.uint16).view(np.float16)).astype(np.float64)])
+    w = w.astype(np.float32)
+    x = w.astype(np.float16)
+    total = np.zeros_like(w, dtype=np.float64)
+    for part in range(3):
+        bits = x.view(np.uint16).astype(np.uint32) + 0x80
+        assert (bits < 0x10000).all()
+        y = (bits & 0xFF00).astype(np.uint16).view(np.float16)
+        e5m2 = torch.from_numpy((bits >> 8).astype(np.uint8)).view(torch.float8_e5m2).double().numpy()
+        assert np.array_equal(e5m2, y.astype(np.float64))
+        rest = x.astype(np.float64) - e5m2
+        assert np.array_equal(rest, (x - y).astype(np.float64))
+        total += e5m2
+        x = x - y
+    assert (np.abs(total - w) <= np.maximum(2.0 ** -11 * w, 2.0 ** -25) + 2.0 ** -17).all()
+
+
 # ---------------------------------------------------------------------------------------------- rows that overlap
 @pytest.fixture()
 def checked(rec, monkeypatch):

@@ -377,3 +377,37 @@ def test_v_scales_out_of_range(cuda, scale, taken, qlen):
     b["s"][1].fill_(scale)
     got = run(b)
     assert ((got.double() - want).abs() <= bound).all()
+
+
+def far_token_and_tails(gaps, B, L, spread, seed, varlen=False):
+    """B sequences of L tokens; in row i of each the first token's score lies gaps[i] above those of the others (apart
+    from each other by `spread`), whose values are around 1 where the first one's are 0: the output is the tail's share."""
+    n = len(gaps)
+    b = make([L] * B, H=1, KVH=1, n=n, qlens=[n] * B if varlen else None, seed=seed)
+    q = b["q"].view(B, n, 128)
+    q.zero_()
+    q[..., 0] = torch.tensor([g * 128 ** 0.5 / 16 for g in gaps])
+    q[..., 1] = spread * 128 ** 0.5
+    c = [x.view(torch.uint8).zero_().view(torch.float8_e4m3fn) for x in b["c"]]
+    for s in b["s"]:
+        s.fill_(2.0 ** -4)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    c[0][..., 1] = (torch.randn(c[0].shape[:3], generator=g, device="cuda") * 16).to(torch.float8_e4m3fn)
+    c[1].copy_((torch.rand(c[1].shape, generator=g, device="cuda") * 8 + 12).to(torch.float8_e4m3fn))
+    for page in b["table"][:, 0].long().tolist():
+        c[0].view(torch.uint8)[page, 0, 0, :2] = torch.tensor([0x78, 0], dtype=torch.uint8)    # 256 * 2^-4 = 16, 0
+        c[1].view(torch.uint8)[page, 0, 0] = 0
+    return dict(b, c=c)
+
+
+@pytest.mark.parametrize("B,L,spread", [(300, 4000, 0.0), (300, 4000, 0.05), (300, 700, 1.0), (1, 60000, 0.0)])
+@pytest.mark.parametrize("rows", [8, 16, 24, 32, 40, 80])
+def test_the_tail_behind_a_far_token_keeps_its_weight(cuda, B, L, spread, rows):
+    """Gaps that put the tail's weights at every place between two powers of two, by every kernel (80 rows: the prefill
+    kernel's) and with few enough CTAs a sequence that one CTA has both.  The tail's weights are all rounded alike, so
+    their errors add up; without the tail the output would be 0."""
+    gaps = [4 + 11 * i / rows for i in range(rows)]
+    b = far_token_and_tails(gaps, B, L, spread, seed=rows, varlen=rows == 80)
+    want, bound = ref(b)
+    assert (want > 20 * bound).all()
+    check(b)
