@@ -74,11 +74,16 @@ struct Cfg8 {
   static constexpr int kVStages = 2;
   static constexpr int kQBuf = 2;
   static constexpr int kPBuf = NP == 48 ? 1 : 2;
-  // hi and lo of Q: NR rows (a UMMA wider than that reads the bytes behind them into columns nobody looks at); the three
-  // parts of P^T: 16-row chunks
+  // The three parts of P^T, 16-row chunks: each a product of its own onto the same columns of O, or, for 8 rows, side by
+  // side (two to a chunk) in one product of 32 columns that are added up at the segment's end.  A product of few columns
+  // takes as long as reading V for it, and decode over long contexts has no time left for twelve a tile (XXX).
+  static constexpr int kOParts = NR == 8 ? 3 : 1;
+  static constexpr int kOCols = kOParts == 3 ? 32 : NP;
+  // hi and lo of Q: NR rows (a UMMA wider than that reads the bytes behind them into columns nobody looks at)
   static constexpr int kQHalf = (NR < 16 ? 16 : NR) * 128, kQBytes = 2 * kQHalf;
-  static constexpr int kPPart = NP * 128, kPBytes = 3 * kPPart;
-  static constexpr int kTmemCols = NP == 16 ? 64 : NP == 32 ? 128 : 256;   // S, O double buffered: 4 NP, a power of two
+  static constexpr int kPPart = NP * 128, kPBytes = kOParts == 3 ? kOCols * 128 : 3 * kPPart;
+  // S, O double buffered, in all a power of two
+  static constexpr int kTmemCols = 2 * (NP + kOCols) <= 64 ? 64 : 2 * (NP + kOCols) <= 128 ? 128 : 256;
   static constexpr int kK = 0;
   static constexpr int kV = kK + kKStages * kTile;
   static constexpr int kQ = kV + kVStages * kTile;
@@ -633,15 +638,15 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       const int flags = info[3 * e + 2].x;
       if ((flags & 1) && pv > 0) oseg ^= 1;
       const int width = min(NP, mma_width(info[3 * e + 1].x * G));
-      const uint32_t idesc = idesc_f8(width, true, true);
+      const uint32_t idesc = idesc_f8(C::kOParts == 3 ? C::kOCols : width, true, true);
       tc_fence_after();
       if (elect_one()) {
         const uint64_t a = v_desc0 + ((st * kTile) >> 4);
         const uint64_t b = p_desc0 + ((pv % C::kPBuf * C::kPBytes) >> 4);
-        const uint32_t d = tmem + (2 + oseg) * NP;
+        const uint32_t d = tmem + 2 * NP + oseg * C::kOCols;
         const uint32_t fresh = (flags & 1) ? 0u : 1u;
 #pragma unroll
-        for (int part = 0; part < 3; ++part)
+        for (int part = 0; part < (C::kOParts == 3 ? 1 : 3); ++part)
 #pragma unroll
           for (int k = 0; k < 4; ++k)   // 32 tokens a step: four groups of 8 (V: 1024 bytes each, P^T: 128)
             umma_f8_ss(d, a + 256 * k, b + ((part * C::kPPart) >> 4) + 32 * k, idesc, part + k > 0 ? 1u : fresh);
@@ -773,7 +778,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     int jj = 0;   // tile of this CTA
     for (int seg = 0; !done; ++seg) {
       // one segment
-      const uint32_t t_o = t_lane + (2 + (seg & 1)) * NP;   // O accumulator, by segment parity
+      const uint32_t t_o = t_lane + 2 * NP + (seg & 1) * C::kOCols;   // O accumulator, by segment parity
       const float* qs = qscale + (seg % kQScaleRing) * NR;
       [&] {
         constexpr int HR = NR;
@@ -893,11 +898,12 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             alive = alive && mbar_wait_warp(&bars[B_OFULL + (buf ^ 1)], ((jj - 1) >> 1) & 1, abort);
             if (alive) {
               tc_fence_after();
-              for (int c = 0; c < R; c += 8) {
+              for (int c = 0; c < (C::kOParts == 3 ? 24 : R); c += 8) {
+                const float* alpha = alpha_s + (C::kOParts == 3 ? 0 : c);
                 float ot[8];
                 tmem_ld8(t_o + c, ot);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) ot[i] *= alpha_s[c + i];
+                for (int i = 0; i < 8; ++i) ot[i] *= alpha[i];
                 tmem_st8(t_o + c, ot);
               }
               tc_fence_before();
@@ -942,7 +948,8 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
               uint8_t* at = pb + (m >> 1) * 2048 + (m & 1) * 8;
 #pragma unroll
               for (int k = 0; k < 3; ++k)
-                *reinterpret_cast<uint2*>(at + k * C::kPPart) = make_uint2(part[k][0], part[k][1]);
+                *reinterpret_cast<uint2*>(at + (C::kOParts == 3 ? (k >> 1) * 2048 + (k & 1) * 8 : k * C::kPPart)) =
+                    make_uint2(part[k][0], part[k][1]);
             }
             fence_proxy_async_smem();
             mbar_arrive(&bars[B_PFULL + buf]);
@@ -981,6 +988,13 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
       for (int c = 0; c < R; c += 8) {
         float ot[8];
         tmem_ld8(t_o + c, ot);
+#pragma unroll
+        for (int k = 1; k < C::kOParts; ++k) {
+          float more[8];
+          tmem_ld8(t_o + 8 * k, more);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ot[i] += more[i];
+        }
 #pragma unroll
         for (int i = 0; i < 8; i += 4) {
           const float4 inv = *reinterpret_cast<const float4*>(row_inv + c + i);
