@@ -34,7 +34,8 @@ install_fused_prologue()
     Qwen3's attention prologue in one kernel (`nva_qk_norm_rope_store`): the q / k RMSNorm and rotary embedding of
     Qwen3Attention.pre_attn (nanovllm/models/qwen3.py:88-97) and the KV scatter of Attention.forward
     (attention.py:61-62) become one pass over the projection output.  Qwen3Attention.forward (whole-model steps:
-    prefill, decode / verify and their CUDA graphs) scatters in the same kernel; pre_attn (the piecewise segments of
+    prefill, decode / verify and their CUDA graphs) scatters in the same kernel (an 8-bit cache is written by
+    store_kvcache behind it); pre_attn (the piecewise segments of
     mixed steps, recorded without a Context) fuses the norms and rotary only and leaves the scatter to the
     attention call, as the reference does.  Needs install_attention.
 
