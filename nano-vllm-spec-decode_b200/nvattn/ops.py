@@ -45,14 +45,14 @@ def _need_cuda(*ts):
 
 
 # The attention workspaces in use, per device index i:
-#   i                   of calls on the default stream
-#   (i, stream)         of calls on another stream (its number)
-#   (i, _GRAPH)         of captured calls
-#   (i, _GRAPH, stream) of calls captured on a stream that reserve_workspace was given
+#   i             of calls on the default stream
+#   (i, stream)   of calls on another stream (its number)
+#   (i, _GRAPH)   of captured calls
 # Earlier (smaller) ones stay referenced because captured CUDA graphs hold their addresses.
 _WORKSPACES: dict = {}
 _RETIRED: list[torch.Tensor] = []
 _GRAPH = "graph"
+_OWN = threading.local()    # .workspace: the one that this thread's calls are to use (own_workspace)
 
 # Held from taking a workspace to the end of the call that uses it: a call is up to four kernels that pass pieces and a
 # plan on through its workspace, and another host thread's on the same stream must not come between them (ctypes lets
@@ -82,16 +82,21 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     call leaves them zero, so it is allocated zero-filled once (grown, zero-filled, when a call needs more) and then
     reused.  Calls that may overlap must not share one: each stream has its own, and captured calls use another one of
     the device, whatever stream their graph is replayed on.  Graphs share that one and are replayed one after another
-    (as those that share a memory pool are); to replay two at once, capture each on a stream of its own that
-    reserve_workspace was given.  Growing a workspace while a CUDA graph is being captured would allocate from the
-    graph's pool and record the zero-fill into every replay, so that raises instead: size it first with
-    reserve_workspace (the nano-vllm drop-in does so when the KV cache is allocated) or an eager call."""
+    (as those that share a memory pool are); a graph that is replayed beside others is captured inside own_workspace.
+    (Not a workspace per capturing stream: torch hands the same 32 streams out again and again.)  Growing a
+    workspace while a CUDA graph is being captured would allocate from the graph's pool and record the zero-fill into
+    every replay, so that raises instead: size it first with reserve_workspace (the nano-vllm drop-in does so when the
+    KV cache is allocated) or an eager call."""
+    own = getattr(_OWN, "workspace", None)
+    if own is not None:
+        if own.numel() < nbytes or own.device != device:
+            raise RuntimeError(f"nvattn: a call on {device} that needs {nbytes} bytes inside own_workspace of "
+                               f"{own.numel()} bytes on {own.device}")
+        return own
     idx = device.index if device.index is not None else torch.cuda.current_device()
     stream = _raw_stream(idx)
     if stream != 0 and torch.cuda.is_current_stream_capturing():
-        ws = _WORKSPACES.get((idx, _GRAPH, stream))
-        if ws is None:
-            ws = _WORKSPACES.get((idx, _GRAPH))
+        ws = _WORKSPACES.get((idx, _GRAPH))
         if ws is None or ws.numel() < nbytes:
             raise RuntimeError(f"nvattn: the attention workspace of cuda:{idx} must grow to {nbytes} bytes during a "
                                "CUDA graph capture; call nvattn.ops.reserve_workspace(...) before capturing")
@@ -104,35 +109,51 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return ws
 
 
+def workspace_bytes(max_num_seqs: int, max_num_tokens: int, num_heads: int, num_kv_heads: int, head_dim: int = 128,
+                    fp8_cache: bool = False) -> int:
+    """Bytes of workspace that every decode / verify / varlen call of up to max_num_seqs sequences and max_num_tokens
+    query rows fits in on the current device; with fp8_cache, also calls over an 8-bit cache."""
+    lib = _lib.load()
+    need = max(lib.nva_varlen_workspace_bytes(max_num_seqs, max_num_tokens, num_heads, num_kv_heads, head_dim),
+               max(lib.nva_paged_decode_workspace_bytes(max_num_seqs, n, num_heads, num_kv_heads, head_dim)
+                   for n in range(1, 49)))
+    if fp8_cache:
+        need = max(need, lib.nva_paged_attention_fp8_workspace_bytes(max_num_tokens, num_heads, num_kv_heads, head_dim))
+    return need
+
+
 def reserve_workspace(max_num_seqs: int, max_num_tokens: int, num_heads: int, num_kv_heads: int,
-                      head_dim: int = 128, device: torch.device | None = None, fp8_cache: bool = False,
-                      stream: torch.cuda.Stream | None = None) -> int:
+                      head_dim: int = 128, device: torch.device | None = None, fp8_cache: bool = False) -> int:
     """Allocate (zero-filled) the workspace every later decode / verify / varlen call of up to max_num_seqs
     sequences and max_num_tokens query rows needs on `device`, so that no call on the current stream, and no captured
-    one, allocates; with fp8_cache, also for calls over an 8-bit cache.  With `stream`, calls captured on that stream
-    get a workspace of their own: a graph captured there may be replayed beside other graphs.  Returns its size in
-    bytes.  nano-vllm: max_num_seqs and max_num_batched_tokens of its Config."""
+    one, allocates; with fp8_cache, also for calls over an 8-bit cache.  Returns its size in bytes.  nano-vllm:
+    max_num_seqs and max_num_batched_tokens of its Config."""
     device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-    lib = _lib.load()
-    with _on(device):
-        need = max(lib.nva_varlen_workspace_bytes(max_num_seqs, max_num_tokens, num_heads, num_kv_heads, head_dim),
-                   max(lib.nva_paged_decode_workspace_bytes(max_num_seqs, n, num_heads, num_kv_heads, head_dim)
-                       for n in range(1, 49)))
-        if fp8_cache:
-            need = max(need, lib.nva_paged_attention_fp8_workspace_bytes(max_num_tokens, num_heads, num_kv_heads,
-                                                                         head_dim))
-        with _CALL:
-            size = _workspace(need, device).numel()
-            if stream is not None:
-                idx = device.index if device.index is not None else torch.cuda.current_device()
-                _grow((idx, _GRAPH, stream.cuda_stream), need, device)
-    return size
+    with _on(device), _CALL:
+        need = workspace_bytes(max_num_seqs, max_num_tokens, num_heads, num_kv_heads, head_dim, fp8_cache)
+        return _workspace(need, device).numel()
+
+
+@contextlib.contextmanager
+def own_workspace(workspace: torch.Tensor):
+    """Attention calls that this thread makes inside use `workspace`: uint8, zero-filled once, of workspace_bytes(...).
+    For a CUDA graph that is replayed beside other graphs: capture it inside, with a workspace of its own that lives as
+    long as the graph does and is filled before the first replay."""
+    _need_cuda(workspace)
+    assert workspace.dtype == torch.uint8 and workspace.is_contiguous()
+    before = getattr(_OWN, "workspace", None)
+    _OWN.workspace = workspace
+    try:
+        yield
+    finally:
+        _OWN.workspace = before
 
 
 def reset_workspaces() -> None:
     """Zero-fill every workspace again.  A call that gave up on a pipeline wait (bit 2 of the device error word) may
     leave merge tickets non-zero, after which later calls could merge split pieces wrongly; call this (outside any
-    graph capture, with no call in flight, after clearing the error word) before going on."""
+    graph capture, with no call in flight, after clearing the error word) before going on.  Those given to own_workspace
+    are the caller's to fill."""
     for ws in list(_WORKSPACES.values()) + _RETIRED:
         ws.zero_()
 

@@ -1,5 +1,7 @@
 """Which workspace an attention call takes (nvattn.ops._workspace): calls that may overlap never share one.  The host
 side without a GPU, and calls in flight together on one."""
+import contextlib
+
 import pytest
 import torch
 
@@ -63,20 +65,29 @@ def test_captured_calls_share_none_with_eager_ones(at):
         ops._workspace(65, DEV)
 
 
-def test_a_reserved_stream_captures_into_its_own(at):
+def test_own_workspace(at, monkeypatch):
+    """Whatever the stream's number: torch gives the same ones out again."""
+    import threading
     from nvattn import ops
-
-    class Stream:
-        cuda_stream = 9
-
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: None)
     at(0)
-    assert ops.reserve_workspace(4, 64, 32, 8, device=DEV, fp8_cache=True, stream=Stream) == 300
+    assert ops.reserve_workspace(4, 64, 32, 8, device=DEV) == 200
+    assert ops.reserve_workspace(4, 64, 32, 8, device=DEV, fp8_cache=True) == 300
+    mine = torch.zeros(ops.workspace_bytes(4, 64, 32, 8, fp8_cache=True), dtype=torch.uint8).view(-1)
+    dev = mine.device
+    other = []
     at(9, capturing=True)
-    own = ops._workspace(300, DEV)
-    at(7, capturing=True)
-    assert ops._workspace(300, DEV) is not own
-    at(9)
-    assert ops._workspace(300, DEV) is not own
+    shared = ops._workspace(300, DEV)
+    with ops.own_workspace(mine):
+        assert ops._workspace(300, dev) is mine
+        with pytest.raises(RuntimeError, match="301 bytes"):
+            ops._workspace(301, dev)
+        with pytest.raises(RuntimeError, match="cpu:0"):
+            ops._workspace(300, DEV)                                   # (another device)
+        thread = threading.Thread(target=lambda: other.append(ops._workspace(300, DEV)))
+        thread.start()
+        thread.join()
+    assert other[0] is shared and ops._workspace(300, DEV) is shared
 
 
 def test_growing_keeps_what_graphs_hold(at):
@@ -190,19 +201,19 @@ def test_streams_at_once(cuda, fp8):
 @pytest.mark.gpu
 @pytest.mark.parametrize("fp8", [True, False])
 def test_replays_beside_eager_calls_and_beside_each_other(cuda, fp8):
-    """A graph on one stream, eager calls on another, and a second graph, captured on a reserved stream, on a third."""
+    """A graph on one stream, eager calls on another, a second graph, captured in a workspace of its own, on a third;
+    both captured on the same stream."""
     from nvattn import _lib, ops
     runs = [calls(s, fp8) for s in (1, 2, 3)]
     want = [[x.clone() for x in r()] for r in runs]
     streams = [torch.cuda.Stream() for _ in range(3)]
-    capture = torch.cuda.Stream()
     ops.reserve_workspace(8, 512, 32, 8, fp8_cache=fp8)
-    ops.reserve_workspace(8, 512, 32, 8, fp8_cache=fp8, stream=capture)
+    own = torch.zeros(ops.workspace_bytes(8, 512, 32, 8, fp8_cache=fp8), dtype=torch.uint8, device="cuda")
     graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
-    for graph, run, w, kw in zip(graphs, runs, want, ({}, dict(stream=capture))):
+    for graph, run, w, within in zip(graphs, runs, want, (contextlib.nullcontext(), ops.own_workspace(own))):
         outs.append([torch.empty_like(x) for x in w])
         torch.cuda.synchronize()
-        with torch.cuda.graph(graph, **kw):
+        with within, torch.cuda.graph(graph):
             run(outs[-1])
     torch.cuda.synchronize()
     for _ in range(10):
