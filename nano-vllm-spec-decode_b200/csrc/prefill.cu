@@ -461,13 +461,15 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             const int64_t at = (page * static_cast<int64_t>(p.num_kv_heads) + kvh) * p.page_blocks +
                                ((j * 128 % p.block_size + t) >> p.lg_block);
             ks = __ldg(p.k_scale + at);
-            vs = fminf(fmaxf(__ldg(p.v_scale + at), 9.094947e-13f), 1.0995116e12f);   // 2^-40 .. 2^40, as for short runs
+            vs = __ldg(p.v_scale + at);
           }
         };
         load_scales(0, page_of(0));
         for (int j = 0; j < i0.w && ok; ++j, ++g) {
           const int next_page = page_of(j + 1);
-          const float scale[2] = {ks, vs};
+          // v's within 2^-40 .. 2^40, as for short runs (here, not where it is loaded a tile ahead: waiting for the load there
+          // made chunks of 600 over 1000 keys 114 us instead of 109)
+          const float scale[2] = {ks, fminf(fmaxf(vs, 9.094947e-13f), 1.0995116e12f)};
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             const int st = g & 1;
