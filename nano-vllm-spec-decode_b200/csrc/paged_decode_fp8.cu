@@ -74,15 +74,17 @@ struct Cfg8 {
   static constexpr int kVStages = 2;
   static constexpr int kQBuf = 2;
   static constexpr int kPBuf = NP == 48 ? 1 : 2;
-  // The three parts of P^T, 16-row chunks: each a product of its own onto the same columns of O, or, for 8 rows, side by
-  // side (two to a chunk) in one product of 32 columns that are added up at the segment's end.  A product of few columns
-  // takes as long as reading V for it, and decode over long contexts has no time for twelve a tile (8 sequences of 40,000
-  // to 65,536: 156 us with three products of 16 columns, 141 with one of 32).
-  static constexpr int kOParts = NR == 8 ? 3 : 1;
-  static constexpr int kOCols = kOParts == 3 ? 32 : NP;
+  // The three parts of P^T, in chunks of 16 rows: up to 16 rows side by side in one product (8 rows: two parts to a chunk),
+  // whose columns are added up at the segment's end; a product of few columns takes as long as reading V for it, so that
+  // three of them onto the same columns cost more (8 rows, 8 sequences of 40,000 to 65,536: 156 us, one product 141; 16
+  // rows, 64 sequences of 4000: 108 and 106).  With more rows three are as fast (20 rows, 4000 tokens: 131, one product
+  // 133; 32 sequences of 256 to 2048: 43.4 and 42.9), and at 40 TMEM has no room for one.
+  static constexpr int kOParts = NP == 16 ? 3 : 1;
+  static constexpr int kOStep = NR == 8 ? 8 : NP;      // from a part's columns of O to the next one's
+  static constexpr int kOCols = NR == 8 ? 32 : kOParts * NP;
   // hi and lo of Q: NR rows (a UMMA wider than that reads the bytes behind them into columns nobody looks at)
   static constexpr int kQHalf = (NR < 16 ? 16 : NR) * 128, kQBytes = 2 * kQHalf;
-  static constexpr int kPPart = NP * 128, kPBytes = kOParts == 3 ? kOCols * 128 : 3 * kPPart;
+  static constexpr int kPPart = NP * 128, kPBytes = NR == 8 ? kOCols * 128 : 3 * kPPart;
   // S, O double buffered, in all a power of two
   static constexpr int kTmemCols = 2 * (NP + kOCols) <= 64 ? 64 : 2 * (NP + kOCols) <= 128 ? 128 : 256;
   static constexpr int kK = 0;
@@ -899,14 +901,15 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             alive = alive && mbar_wait_warp(&bars[B_OFULL + (buf ^ 1)], ((jj - 1) >> 1) & 1, abort);
             if (alive) {
               tc_fence_after();
-              for (int c = 0; c < (C::kOParts == 3 ? 24 : R); c += 8) {
-                const float* alpha = alpha_s + (C::kOParts == 3 ? 0 : c);
-                float ot[8];
-                tmem_ld8(t_o + c, ot);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) ot[i] *= alpha[i];
-                tmem_st8(t_o + c, ot);
-              }
+              for (int k = 0; k < C::kOParts * C::kOStep; k += C::kOStep)
+                for (int c = 0; c < R; c += 8) {
+                  float ot[8];
+                  tmem_ld8(t_o + k + c, ot);
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) ot[i] *= alpha_s[c + i];
+                  tmem_st8(t_o + k + c, ot);
+                }
               tc_fence_before();
             }
           }
@@ -949,7 +952,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
               uint8_t* at = pb + (m >> 1) * 2048 + (m & 1) * 8;
 #pragma unroll
               for (int k = 0; k < 3; ++k)
-                *reinterpret_cast<uint2*>(at + (C::kOParts == 3 ? (k >> 1) * 2048 + (k & 1) * 8 : k * C::kPPart)) =
+                *reinterpret_cast<uint2*>(at + (NR == 8 ? (k >> 1) * 2048 + (k & 1) * 8 : k * C::kPPart)) =
                     make_uint2(part[k][0], part[k][1]);
             }
             fence_proxy_async_smem();
@@ -992,7 +995,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
 #pragma unroll
         for (int k = 1; k < C::kOParts; ++k) {
           float more[8];
-          tmem_ld8(t_o + 8 * k, more);
+          tmem_ld8(t_o + k * C::kOStep + c, more);
 #pragma unroll
           for (int i = 0; i < 8; ++i) ot[i] += more[i];
         }
