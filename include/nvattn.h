@@ -210,11 +210,15 @@ NVA_API int nva_paged_decode_noalloc(const void* q, int64_t q_row_stride, const 
  *
  * nva_paged_decode_fp8, nva_varlen_attention_fp8: nva_paged_decode and the paged nva_varlen_attention over such a cache
  * (bf16 q and out).  Scales outside [2^-40, 2^40] are taken as those bounds for v.  bt_width is the number of entries
- * in a row of block_tables: a sequence that needs more, or names a block outside the cache, sets bit 4 of the error
- * word and reads zeros there.  Neither the number of sequences nor the length of a query run is bounded; max_seqlen_q and
- * total_q only pick the kernels (from 64 queries on a run takes the prefill kernel, which rounds k * scale to bf16: exact
- * for the scales that nva_store_kvcache_fp8 writes).  num_heads / num_kv_heads <= 40.  Workspace: the same
- * zero-filled-once contract, and the same one may serve all attention calls.
+ * in a row of block_tables (rows do not overlap): a sequence that needs more, or names a block outside the cache, sets
+ * bit 4 of the error word and reads zeros there.  Neither the number of sequences nor the length of a query run is
+ * bounded; total_q is the number of rows of q and out, and max_seqlen_q only picks the kernels.  From 64 queries on a run
+ * takes the prefill kernel, which rounds k * scale and the softmax weights to bf16 (the first exactly for the scales that
+ * nva_store_kvcache_fp8 writes).  Shorter runs, and all runs of a call of more than 1024 sequences or 4096 query tiles
+ * (total_q / 128 + num_seqs + 1), take the decode kernel, which walks a run's keys once for every 40 packed rows: its
+ * weights are rounded to float16, and q is whole down to 2^-10 of a row's largest value, off by at most 2^-18 of it below.
+ * num_heads / num_kv_heads <= 40.  Workspace: the same zero-filled-once contract, and the same one may serve all
+ * attention calls.
  */
 #define NVA_MIN_SCALE_BLOCK 8
 #define NVA_MAX_SCALE_BLOCK 256

@@ -411,3 +411,18 @@ def test_the_tail_behind_a_far_token_keeps_its_weight(cuda, B, L, spread, rows):
     want, bound = ref(b)
     assert (want > 20 * bound).all()
     check(b)
+
+
+@pytest.mark.parametrize("n", [1, 4, 5, 10])
+@pytest.mark.parametrize("far", [2.0 ** 6, 2.0 ** 11, 2.0 ** 15])
+def test_queries_with_one_large_value(cuda, n, far):
+    """q's two e4m3 parts hold values down to 2^-10 of their row's largest whole and are off by 2^-18 of it at most below
+    (include/nvattn.h): scores by that times the sum of |k|, weights by twice as much of themselves."""
+    b = make([700, 1300, n], n=n, seed=50 + n, size=0.3)
+    b["c"][0].view(torch.uint8)[..., 7] = 0                     # (the large value meets no key: the small ones decide)
+    b["q"][..., 7] = far
+    want, bound = ref(b)
+    size, _ = ref(dict(b, c=(b["c"][0], (b["c"][1].view(torch.uint8) & 0x7F).view(torch.float8_e4m3fn))))
+    keys = fp8_cache.values(b["c"][0], b["s"][0]).abs().sum(-1).max()
+    bound = bound + 2 * 2.0 ** -18 * far * keys * b["scale"] * size
+    assert ((run(b).double() - want).abs() <= bound).all()
