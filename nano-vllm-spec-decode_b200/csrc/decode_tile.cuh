@@ -1,6 +1,6 @@
-// Row-tile helpers shared by the paged decode kernels (paged_decode.cu, paged_decode_fp8.cu): both put a KV tile's 128
-// tokens on the TMEM lanes and a kv head's query rows on the UMMA N columns, reduce over tokens across lanes, and merge
-// the pieces of a segment that the work split cut.
+// Row-tile helpers of the paged decode kernels, which put a KV tile's 128 tokens on the TMEM lanes and a kv head's query
+// rows on the UMMA N columns and reduce over tokens across lanes.  Both (paged_decode.cu, paged_decode_fp8.cu) use the
+// constants, warp_columns and mma_width; the choice of a row width and merge_pieces are the bf16 kernel's alone.
 #pragma once
 #include <cstdint>
 #include <type_traits>

@@ -20,8 +20,9 @@
 //        below 2^-15 of the largest: a long flat tail behind one heavy token was off by up to a tenth of itself.  Sums of
 //        weights stay in float32, unrounded.
 //
-// Bound: HBM, one byte per cached value (decode of 64 sequences, contexts 512 to 4096: 303 MB, 46 us at the copy rate).  A 128-token tile then takes 0.74 us of an SM's share of the bandwidth, half of the bf16 cache's, which is
-// less than one tile's chain S -> weights -> PV takes; so two CTAs share an SM and their chains overlap.
+// Bound: HBM, one byte per cached value (decode of 64 sequences, contexts 512 to 4096: 303 MB, 46 us at the copy rate).  A
+// 128-token tile then takes 0.74 us of an SM's share of the bandwidth, half of the bf16 cache's, which is less than one
+// tile's chain S -> weights -> PV takes; so two CTAs share an SM and their chains overlap.
 //
 // Orientation, roles and the merge of split segments are those of paged_decode.cu: tokens on the TMEM lanes (UMMA M),
 // query rows on N; warp 0 = K producer, 1 = TMEM + UMMA issuer, 2 = Q loader, 3 = V producer, 4.. = softmax groups.
@@ -29,17 +30,17 @@
 // without swizzle, 16 rows of a token per 16 bytes.
 //
 // Work split: heads go in sets of 8 (or 4, 2, 1) that as many CTAs walk side by side, tile for tile, so that the rows of
-// a token, 128 bytes a head, are fetched as the 1 KB that lies together (contexts of 50,000 of 8 sequences: 201 us a head
+// a token, 128 bytes a head, are fetched as the 1 KB that lies together (contexts of 50,000 of 8 sequences: 196 us a head
 // alone, 135 in sets; short ones 28.0 and 28.8).  Every set owns an equal share of cost positions (tiles + 3 per segment)
 // in (sequence, piece, set, tile) order, where a piece is a run of at most max_n queries of a sequence: a longer run is
 // walked piece by piece, each over the keys its last query sees, up to where the prefill kernel takes it (kMinPrefillRun).
 // A set finds its start with one scan over the lengths and walks on from there, so there is no table of sequences on the
 // chip and no bound on their number.
 //
-// Measured (32 q heads over 8, copy rate 6.57 TB/s): decode of 64 sequences of 512 to 4096 62 us (75%), of 8192 168 us
-// (97%), 8 of 40,000 to 65,536 139 us (95%); verify of 32 sequences of 256 to 2048, k = 4, 40 us; 4 sequences of 37 to
-// 1000 18 us, of which the start takes 6, the tiles 5 and the ends 5; 256 single queries with three prefill chunks 243 us:
-// three kernels, each launched so that its blocks start where the last one's leave.
+// Measured (32 q heads over 8, copy rate 6.57 TB/s): decode of 64 sequences of 512 to 4096 60 to 65 us (71 to 77%), of 8192
+// 167 us (97%), 8 of 40,000 to 65,536 141 us (93%); verify of 32 sequences of 256 to 2048, k = 4, 41 to 43 us (7 to 10 tiles
+// a CTA); 4 sequences of 37 to 1000 18 us, of which the start takes 6, the tiles 5 and the ends 5; 256 single queries with
+// three prefill chunks 247 us: three kernels, each launched so that its blocks start where the last one's leave.
 #include <algorithm>
 #include <cuda_fp8.h>
 
@@ -1167,9 +1168,14 @@ int tile_rows(int64_t rows) {
 int rows_for(int32_t max_q, int group) { return tile_rows(static_cast<int64_t>(std::max(max_q, 1)) * group); }
 
 // Query runs of at least this many tokens take the prefill kernel, which gives each q head 128 rows of its own and costs
-// the same for 33 queries as for 128, while here every 32 packed rows are walked anew.  32 q heads over 8, here and there:
-// 4 runs of 64 over 1000 keys 45 and 35 us, 32 such runs 219 and 152, 8 over 8000 keys 239 and 277; runs of 48: 40 and 35,
-// 164 and 150, 184 and 276; runs of 80: 49 and 36, 267 and 153, 293 and 281.
+// the same for 33 queries as for 128, while here every 40 packed rows are walked anew.  us here and there, with 1, 4 and 8
+// q heads per kv head (8 kv heads):
+//                                runs of 48                   runs of 64                   runs of 96
+//   4 runs over 1000 keys    29/37   42/39   55/57       29/38   47/39   66/58       34/39   56/40   90/60
+//   32 runs over 1000 keys   71/60  165/155 311/287      73/61  219/156 406/289     102/62  319/159 618/293
+//   8 runs over 8000 keys    96/150 198/278 364/533      98/150 262/279 466/534     133/153 368/284 707/543
+// So the bound suits many runs and short contexts; few runs over long contexts would do better here up to 70 tokens (4 q
+// heads a kv head) or 96 (one).
 constexpr int kMinPrefillRun = 64;
 
 // Queries of the runs that a split call leaves to the kernel of the fewest rows.
@@ -1178,9 +1184,9 @@ int short_run(int group) { return std::max(1, 8 / group); }
 // Whether a varlen call runs twice, short runs (up to 8 packed rows, or one query) and the others each in a kernel of
 // their own rows: one kernel gives every run the rows of the longest.  Two have two starts, so it pays where short runs
 // outnumber the long ones' pieces, as the totals tell if all long runs are alike (runs for the prefill kernel count as
-// none).  Single queries + long runs over 2000 keys, 32 q heads over 8, one kernel and two: 32 + 2 x 60 81 and 75 us, 64 +
-// 2 x 60 122 and 99, 256 + 16 x 20 378 and 243, 128 + 16 x 9 205 and 140, 256 + 2 x 5 233 and 197, 64 + 32 x 5 107 and 104,
-// 64 + 8 x 5 82 and 83.
+// none).  Single queries + long runs over 2000 keys, 32 q heads over 8, one kernel and two: 32 + 2 x 60 79 and 77 us, 64 +
+// 2 x 60 121 and 100, 256 + 16 x 20 371 and 245, 128 + 16 x 9 200 and 140, 256 + 2 x 5 236 and 195, 64 + 32 x 5 109 and 105,
+// 64 + 8 x 5 83 and 84.
 bool two_kernels(int nr, int group, int64_t total_q, int64_t num_seqs, int64_t longest, bool prefill) {
   if (nr <= tile_rows(static_cast<int64_t>(short_run(group)) * group)) return false;
   if (prefill) return true;

@@ -68,8 +68,9 @@ def attention_ref(q, k, v, scale):
     rounded to bf16 (long runs: half a step, 2^-8 of a weight, as its leading bit may be the least) or to float16, kept
     as three e5m2 parts (short runs: 2^-11), so the weighted sum is off by at most 2^-8 of sum p |v|; the parts' smallest
     step is 2^-16 where the row's largest weight is 2^12 at least: half of it, 2^-29 of the largest, for each token, times
-    the largest |v|.  Scores are float32 sums of 128 exact products: off by at most 130 * 2^-24 of sum |q k| (in natural
-    units after the scale), and the exponential and the running sums by 2^-20."""
+    the largest |v|.  Scores are float32 sums of 128 products (exact where a row's values lie within 2^10 of each other):
+    off by at most 130 * 2^-24 of sum |q k| (in natural units after the scale), and the exponential and the running sums
+    by 2^-20."""
     n, H, D = q.shape
     L, KVH, _ = k.shape
     G = H // KVH
