@@ -64,7 +64,7 @@ constexpr float kSlack = 3.0f;          // ... and may pass it by this much (log
 constexpr float kWeightMax = 32768.0f;  // 2^(kBase + kSlack): inside float16's range
 
 // NR: the most query rows a softmax thread carries.  One softmax group of 128 threads at 128 registers each: at 40 rows
-// (weights and sums of 40 rows, 80 registers) three words spill; with more rows they spill past an L1 that two CTAs' shared
+// (weights and sums of 40 rows, 80 registers) a few words spill; with more rows they spill past an L1 that two CTAs' shared
 // memory leaves next to nothing, and a tile takes four times as long.
 template <int NR>
 struct Cfg8 {
